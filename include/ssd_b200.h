@@ -358,6 +358,119 @@ SSD_API int32_t ssd_rmsnorm_backward(const SsdNormDims* dims, const void* in, co
                                      void* cuda_stream);
 
 /*
+ * Selective scan with a decay per channel and state (the Mamba-1 form; ssd_forward above has one per head).  Per batch row b,
+ * channel d with group g = d*ngroups/channels, time t, state h [N]:
+ *     s[b,t,d] = act(dt_in[b,t,d] + dt_bias[d])          act = softplus if dims.dt_softplus else identity; dt_bias optional
+ *     h_t[n] = exp(s A[d,n]) h_{t-1}[n] + s x[b,t,d] B[b,t,g,n]
+ *     y_t = (sum_n C[b,t,g,n] h_t[n] + D[d] x[b,t,d])    (then y_t *= silu(z_t) if z given)
+ * Any channel count and any strides between rows (channels of a row dense); dstate <= 64.  Storage fp32 or bf16 for x, dt, B, C,
+ * z, y and their gradients (ddt included); A, D, dt_bias, states and their gradients fp32.  All arithmetic is fp32.
+ * `lengths` (optional, device int32 [batch], taken as 0 .. seqlen): tokens at or past a row's length are not read, leave its
+ * state as it is, and get zeros as output and as gradient; the final state is the one after the row's last token.
+ */
+typedef struct SsdSelDims {
+  int32_t batch, seqlen, channels, dstate, ngroups;
+  int32_t dtype, device;            /* as in SsdDims */
+  int32_t dt_softplus;
+  int64_t x_stride_b, x_stride_l;   /* elements; 0 = dense */
+  int64_t dt_stride_b, dt_stride_l;
+  int64_t b_stride_b, b_stride_l;
+  int64_t c_stride_b, c_stride_l;
+  int64_t z_stride_b, z_stride_l;
+  int64_t y_stride_b, y_stride_l;   /* y in forward, dy in backward */
+} SsdSelDims;
+
+typedef struct SsdSelFwdPtrs {
+  const void* x;           /* [B,L,D] */
+  const void* dt;          /* [B,L,D] */
+  const float* A;          /* [D,N], negative */
+  const void* Bm;          /* [B,L,G,N] */
+  const void* Cm;          /* [B,L,G,N] */
+  const float* D;          /* [D], optional */
+  const void* z;           /* [B,L,D], optional */
+  const float* init_state; /* [B,D,N], optional */
+  void* y;                 /* [B,L,D], out */
+  float* final_state;      /* [B,D,N], out, optional */
+  const float* dt_bias;    /* [D], optional */
+  const int32_t* lengths;  /* [B], optional */
+} SsdSelFwdPtrs;
+
+typedef struct SsdSelBwdPtrs {
+  const void* x; const void* dt; const float* A; const void* Bm; const void* Cm;
+  const float* D; const void* z; const float* init_state;
+  const void* dy;            /* [B,L,D] */
+  const float* dfinal_state; /* [B,D,N], optional */
+  void* dx; void* ddt;       /* [B,L,D], dense */
+  float* dA;                 /* [D,N] */
+  void* dB; void* dC;        /* [B,L,G,N], dense */
+  float* dD;                 /* [D], required iff D given */
+  void* dz;                  /* [B,L,D], dense, required iff z given */
+  float* dinit_state;        /* [B,D,N], optional */
+  const float* dt_bias;
+  float* ddt_bias;           /* [D], required iff dt_bias given */
+  const int32_t* lengths;
+  int64_t fwd_saved;         /* 1: `workspace` had the backward's size when ssd_selscan_forward ran in it for these same inputs
+                                (the states it kept are used); 0: they are computed again */
+} SsdSelBwdPtrs;
+
+typedef struct SsdSelStepDims {
+  int32_t streams, channels, dstate, ngroups, dtype, device, dt_softplus, reserved;
+  int64_t x_stride_s, dt_stride_s, b_stride_s, c_stride_s, z_stride_s, y_stride_s;   /* elements; 0 = dense */
+} SsdSelStepDims;
+
+SSD_API size_t ssd_selscan_workspace_bytes(const SsdSelDims* dims, int32_t pass);
+SSD_API int32_t ssd_selscan_forward(const SsdSelDims* dims, const SsdSelFwdPtrs* p, void* workspace, size_t workspace_bytes,
+                                    void* cuda_stream);
+SSD_API int32_t ssd_selscan_backward(const SsdSelDims* dims, const SsdSelBwdPtrs* p, void* workspace, size_t workspace_bytes,
+                                     void* cuda_stream);
+/* One timestep, in place on `state` [S,D,N]; A is [D,N], the other fields of SsdStepPtrs as named there with [S,D] for [S,H,P]. */
+SSD_API int32_t ssd_selscan_step(const SsdSelStepDims* dims, const SsdStepPtrs* p, void* cuda_stream);
+
+/*
+ * The convolution above with the history it needs to go on where another call stopped.  `history` is [batch, width-1, channels]
+ * (dense, storage dtype, oldest row first; NULL = zeros), and with ext = history followed by in:
+ *     out[b,t,c] = act(bias[c] + sum_k weight[c,k] * ext[b,t+k,c]),   new_history[b,j,c] = ext[b,len_b+j,c]  (j < width-1)
+ * where len_b = lengths[b] (optional, device int32, taken as 0 .. seqlen) or seqlen.  Rows at or past len_b are not read; their
+ * outputs and gradients are zeros.  The backward takes the gradients of both outputs and gives those of in, history, weight and
+ * bias.  history and new_history must not overlap.  ssd_conv1d_step is one token per stream (batch = streams, seqlen = 1,
+ * in_stride_b / out_stride_b between streams), in place on `history`.  Channels, strides and alignment as above.
+ */
+SSD_API int32_t ssd_conv1d_carry_forward(const SsdConvDims* dims, const void* in, const float* weight,
+                                         const float* bias /* optional */, const void* history /* optional */,
+                                         const int32_t* lengths /* optional */, void* out, void* new_history /* optional */,
+                                         void* cuda_stream);
+SSD_API size_t ssd_conv1d_carry_workspace_bytes(const SsdConvDims* dims);   /* backward only */
+SSD_API int32_t ssd_conv1d_carry_backward(const SsdConvDims* dims, const void* in, const float* weight, const float* bias,
+                                          const void* history, const int32_t* lengths, const void* dout, int64_t dout_stride_b,
+                                          int64_t dout_stride_l, const void* dnew_history /* optional */, void* din /* dense */,
+                                          void* dhistory /* dense, iff history */, float* dweight, float* dbias /* optional */,
+                                          void* workspace, size_t workspace_bytes, void* cuda_stream);
+SSD_API int32_t ssd_conv1d_step(const SsdConvDims* dims, const void* in, const float* weight, const float* bias, void* history,
+                                void* out, void* cuda_stream);
+
+/*
+ * A layer's projection: out = act(x W^T + bias) + residual, x [rows, in_features], W [out_features, in_features] dense, all of one
+ * storage dtype; products are added in fp32 and the result is rounded once.  bf16 operands whose rows are 16-byte aligned run on
+ * the tensor cores; all other sizes, strides and fp32 on the CUDA cores in fp32.  `pre` (optional, dense, storage dtype) receives
+ * x W^T + bias for the backward, which needs it where act is not NONE.  Backward: dpre = dout * act'(pre), dx = dpre W,
+ * dweight = dpre^T x, dbias = sum of dpre over the rows; each of the three is optional.
+ */
+typedef enum SsdAct { SSD_ACT_NONE = 0, SSD_ACT_SILU = 1, SSD_ACT_SOFTPLUS = 2, SSD_ACT_RELU2 = 3 } SsdAct;   /* RELU2: max(v,0)^2 */
+typedef struct SsdLinearDims {
+  int64_t rows;
+  int32_t in_features, out_features;
+  int32_t dtype, device, activation, reserved;
+  int64_t x_stride_row, out_stride_row, residual_stride_row;   /* elements; 0 = dense */
+} SsdLinearDims;
+SSD_API size_t ssd_linear_workspace_bytes(const SsdLinearDims* dims, int32_t pass);
+SSD_API int32_t ssd_linear_forward(const SsdLinearDims* dims, const void* x, const void* weight, const void* bias /* optional */,
+                                   const void* residual /* optional */, void* out, void* pre /* optional */, void* workspace,
+                                   size_t workspace_bytes, void* cuda_stream);
+SSD_API int32_t ssd_linear_backward(const SsdLinearDims* dims, const void* x, const void* weight, const void* pre,
+                                    const void* dout, int64_t dout_stride_row, void* dx, void* dweight, void* dbias,
+                                    void* workspace, size_t workspace_bytes, void* cuda_stream);
+
+/*
  * Failure detection.  Every wait inside the pipelined kernels (on a TMA transfer, an MMA completion, another warp role)
  * is bounded: when it runs out the kernel writes a code into the first 4 bytes of the workspace (0 = healthy), skips its
  * remaining waits and returns, and later kernels on the same workspace return at once; the context stays usable.

@@ -12,7 +12,7 @@ use std::env;
 use std::path::{Path, PathBuf};
 use std::process::Command;
 
-const SOURCES: [&str; 7] = [
+const SOURCES: [&str; 9] = [
     "ssd_api.cu",
     "ssd_simt.cu",
     "ssd_decode.cu",
@@ -20,6 +20,8 @@ const SOURCES: [&str; 7] = [
     "ssd_noalloc.cu",
     "ssd_prepost.cu",
     "ssd_sp.cu",
+    "ssd_selscan.cu",
+    "ssd_linear.cu",
 ];
 
 fn nvcc() -> String {

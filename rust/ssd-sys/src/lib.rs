@@ -41,6 +41,10 @@ pub const SSD_STAGE_LOCAL_REST: i32 = 16;
 
 pub const SSD_SP_UNIQUE_ID_BYTES: usize = 128;
 pub const SSD_NOALLOC_MAX_BYTES: usize = 32 << 20;
+pub const SSD_ACT_NONE: i32 = 0;
+pub const SSD_ACT_SILU: i32 = 1;
+pub const SSD_ACT_SOFTPLUS: i32 = 2;
+pub const SSD_ACT_RELU2: i32 = 3;
 
 // ---- structs ---------------------------------------------------------------------------------------------------
 #[repr(C)]
@@ -191,6 +195,109 @@ pub struct SsdNormDims {
     pub eps: f32,
     pub in_stride_row: i64,
     pub out_stride_row: i64,
+}
+
+#[repr(C)]
+#[derive(Debug, Clone, Copy, Default)]
+pub struct SsdSelDims {
+    pub batch: i32,
+    pub seqlen: i32,
+    pub channels: i32,
+    pub dstate: i32,
+    pub ngroups: i32,
+    pub dtype: i32,
+    pub device: i32,
+    pub dt_softplus: i32,
+    pub x_stride_b: i64,
+    pub x_stride_l: i64,
+    pub dt_stride_b: i64,
+    pub dt_stride_l: i64,
+    pub b_stride_b: i64,
+    pub b_stride_l: i64,
+    pub c_stride_b: i64,
+    pub c_stride_l: i64,
+    pub z_stride_b: i64,
+    pub z_stride_l: i64,
+    pub y_stride_b: i64,
+    pub y_stride_l: i64,
+}
+
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct SsdSelFwdPtrs {
+    pub x: *const c_void,
+    pub dt: *const c_void,
+    pub A: *const f32,
+    pub Bm: *const c_void,
+    pub Cm: *const c_void,
+    pub D: *const f32,
+    pub z: *const c_void,
+    pub init_state: *const f32,
+    pub y: *mut c_void,
+    pub final_state: *mut f32,
+    pub dt_bias: *const f32,
+    pub lengths: *const i32,
+}
+
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct SsdSelBwdPtrs {
+    pub x: *const c_void,
+    pub dt: *const c_void,
+    pub A: *const f32,
+    pub Bm: *const c_void,
+    pub Cm: *const c_void,
+    pub D: *const f32,
+    pub z: *const c_void,
+    pub init_state: *const f32,
+    pub dy: *const c_void,
+    pub dfinal_state: *const f32,
+    pub dx: *mut c_void,
+    pub ddt: *mut c_void,
+    pub dA: *mut f32,
+    pub dB: *mut c_void,
+    pub dC: *mut c_void,
+    pub dD: *mut f32,
+    pub dz: *mut c_void,
+    pub dinit_state: *mut f32,
+    pub dt_bias: *const f32,
+    pub ddt_bias: *mut f32,
+    pub lengths: *const i32,
+    pub fwd_saved: i64,
+}
+
+#[repr(C)]
+#[derive(Debug, Clone, Copy, Default)]
+pub struct SsdSelStepDims {
+    pub streams: i32,
+    pub channels: i32,
+    pub dstate: i32,
+    pub ngroups: i32,
+    pub dtype: i32,
+    pub device: i32,
+    pub dt_softplus: i32,
+    pub reserved: i32,
+    pub x_stride_s: i64,
+    pub dt_stride_s: i64,
+    pub b_stride_s: i64,
+    pub c_stride_s: i64,
+    pub z_stride_s: i64,
+    pub y_stride_s: i64,
+}
+
+#[repr(C)]
+#[derive(Debug, Clone, Copy, Default)]
+pub struct SsdLinearDims {
+    pub rows: i64,
+    pub in_features: i32,
+    pub out_features: i32,
+    pub dtype: i32,
+    pub device: i32,
+    pub activation: i32,
+    pub reserved: i32,
+    pub x_stride_row: i64,
+    pub out_stride_row: i64,
+    pub residual_stride_row: i64,
 }
 
 // ---- functions (header order) ------------------------------------------------------------------------------------
@@ -346,6 +453,89 @@ extern "C" {
         din: *mut c_void,
         din_stride_row: i64,
         dweight: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: size_t,
+        cuda_stream: *mut c_void,
+    ) -> i32;
+    pub fn ssd_selscan_workspace_bytes(dims: *const SsdSelDims, pass: i32) -> size_t;
+    pub fn ssd_selscan_forward(
+        dims: *const SsdSelDims,
+        p: *const SsdSelFwdPtrs,
+        workspace: *mut c_void,
+        workspace_bytes: size_t,
+        cuda_stream: *mut c_void,
+    ) -> i32;
+    pub fn ssd_selscan_backward(
+        dims: *const SsdSelDims,
+        p: *const SsdSelBwdPtrs,
+        workspace: *mut c_void,
+        workspace_bytes: size_t,
+        cuda_stream: *mut c_void,
+    ) -> i32;
+    pub fn ssd_selscan_step(dims: *const SsdSelStepDims, p: *const SsdStepPtrs, cuda_stream: *mut c_void) -> i32;
+    pub fn ssd_conv1d_carry_forward(
+        dims: *const SsdConvDims,
+        r#in: *const c_void,
+        weight: *const f32,
+        bias: *const f32,
+        history: *const c_void,
+        lengths: *const i32,
+        out: *mut c_void,
+        new_history: *mut c_void,
+        cuda_stream: *mut c_void,
+    ) -> i32;
+    pub fn ssd_conv1d_carry_workspace_bytes(dims: *const SsdConvDims) -> size_t;
+    pub fn ssd_conv1d_carry_backward(
+        dims: *const SsdConvDims,
+        r#in: *const c_void,
+        weight: *const f32,
+        bias: *const f32,
+        history: *const c_void,
+        lengths: *const i32,
+        dout: *const c_void,
+        dout_stride_b: i64,
+        dout_stride_l: i64,
+        dnew_history: *const c_void,
+        din: *mut c_void,
+        dhistory: *mut c_void,
+        dweight: *mut f32,
+        dbias: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: size_t,
+        cuda_stream: *mut c_void,
+    ) -> i32;
+    pub fn ssd_conv1d_step(
+        dims: *const SsdConvDims,
+        r#in: *const c_void,
+        weight: *const f32,
+        bias: *const f32,
+        history: *mut c_void,
+        out: *mut c_void,
+        cuda_stream: *mut c_void,
+    ) -> i32;
+    pub fn ssd_linear_workspace_bytes(dims: *const SsdLinearDims, pass: i32) -> size_t;
+    pub fn ssd_linear_forward(
+        dims: *const SsdLinearDims,
+        x: *const c_void,
+        weight: *const c_void,
+        bias: *const c_void,
+        residual: *const c_void,
+        out: *mut c_void,
+        pre: *mut c_void,
+        workspace: *mut c_void,
+        workspace_bytes: size_t,
+        cuda_stream: *mut c_void,
+    ) -> i32;
+    pub fn ssd_linear_backward(
+        dims: *const SsdLinearDims,
+        x: *const c_void,
+        weight: *const c_void,
+        pre: *const c_void,
+        dout: *const c_void,
+        dout_stride_row: i64,
+        dx: *mut c_void,
+        dweight: *mut c_void,
+        dbias: *mut c_void,
         workspace: *mut c_void,
         workspace_bytes: size_t,
         cuda_stream: *mut c_void,

@@ -36,6 +36,9 @@ EXPORTS = [
     "ssd_workspace_status", "ssd_workspace_status_async", "ssd_status_check", "ssd_noalloc_status",
     "ssd_sp_unique_id", "ssd_sp_comm_new", "ssd_sp_comm_wrap", "ssd_sp_comm_world", "ssd_sp_comm_rank", "ssd_sp_comm_free",
     "ssd_sp_comm_abort", "ssd_sp_exchange_bytes", "ssd_sp_exchange_fwd", "ssd_sp_exchange_bwd", "ssd_sp_allreduce_params",
+    "ssd_selscan_workspace_bytes", "ssd_selscan_forward", "ssd_selscan_backward", "ssd_selscan_step",
+    "ssd_conv1d_carry_workspace_bytes", "ssd_conv1d_carry_forward", "ssd_conv1d_carry_backward", "ssd_conv1d_step",
+    "ssd_linear_workspace_bytes", "ssd_linear_forward", "ssd_linear_backward",
 ]
 
 
@@ -84,6 +87,35 @@ class SsdConvGrad(C.Structure):
 class SsdNormDims(C.Structure):
     _fields_ = [("rows", C.c_int64), ("width", C.c_int32), ("dtype", C.c_int32), ("device", C.c_int32), ("eps", C.c_float),
                 ("in_stride_row", C.c_int64), ("out_stride_row", C.c_int64)]
+
+
+class SsdSelDims(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "seqlen", "channels", "dstate", "ngroups", "dtype", "device", "dt_softplus")] + \
+               [(n, C.c_int64) for n in ("x_stride_b", "x_stride_l", "dt_stride_b", "dt_stride_l", "b_stride_b", "b_stride_l",
+                                         "c_stride_b", "c_stride_l", "z_stride_b", "z_stride_l", "y_stride_b", "y_stride_l")]
+
+
+class SsdSelFwdPtrs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "dt", "A", "Bm", "Cm", "D", "z", "init_state", "y", "final_state", "dt_bias",
+                                          "lengths")]
+
+
+class SsdSelBwdPtrs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "dt", "A", "Bm", "Cm", "D", "z", "init_state", "dy", "dfinal_state", "dx", "ddt",
+                                          "dA", "dB", "dC", "dD", "dz", "dinit_state", "dt_bias", "ddt_bias", "lengths")] + \
+               [("fwd_saved", C.c_int64)]
+
+
+class SsdSelStepDims(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("streams", "channels", "dstate", "ngroups", "dtype", "device", "dt_softplus",
+                                         "reserved")] + \
+               [(n, C.c_int64) for n in ("x_stride_s", "dt_stride_s", "b_stride_s", "c_stride_s", "z_stride_s", "y_stride_s")]
+
+
+class SsdLinearDims(C.Structure):
+    _fields_ = [("rows", C.c_int64)] + [(n, C.c_int32) for n in ("in_features", "out_features", "dtype", "device", "activation",
+                                                                 "reserved")] + \
+               [(n, C.c_int64) for n in ("x_stride_row", "out_stride_row", "residual_stride_row")]
 
 
 class SsdError(RuntimeError):
@@ -180,6 +212,28 @@ def load() -> C.CDLL:
     lib.ssd_rmsnorm_forward.argtypes = [C.POINTER(SsdNormDims), vp, vp, vp, vp, vp]
     lib.ssd_rmsnorm_backward.restype = i32
     lib.ssd_rmsnorm_backward.argtypes = [C.POINTER(SsdNormDims), vp, vp, vp, vp, i64, vp, i64, vp, vp, sz, vp]
+    lib.ssd_selscan_workspace_bytes.restype = sz
+    lib.ssd_selscan_workspace_bytes.argtypes = [C.POINTER(SsdSelDims), i32]
+    lib.ssd_selscan_forward.restype = i32
+    lib.ssd_selscan_forward.argtypes = [C.POINTER(SsdSelDims), C.POINTER(SsdSelFwdPtrs), vp, sz, vp]
+    lib.ssd_selscan_backward.restype = i32
+    lib.ssd_selscan_backward.argtypes = [C.POINTER(SsdSelDims), C.POINTER(SsdSelBwdPtrs), vp, sz, vp]
+    lib.ssd_selscan_step.restype = i32
+    lib.ssd_selscan_step.argtypes = [C.POINTER(SsdSelStepDims), C.POINTER(SsdStepPtrs), vp]
+    lib.ssd_conv1d_carry_forward.restype = i32
+    lib.ssd_conv1d_carry_forward.argtypes = [C.POINTER(SsdConvDims)] + [vp] * 8
+    lib.ssd_conv1d_carry_workspace_bytes.restype = sz
+    lib.ssd_conv1d_carry_workspace_bytes.argtypes = [C.POINTER(SsdConvDims)]
+    lib.ssd_conv1d_carry_backward.restype = i32
+    lib.ssd_conv1d_carry_backward.argtypes = [C.POINTER(SsdConvDims)] + [vp] * 6 + [i64, i64] + [vp] * 6 + [sz, vp]
+    lib.ssd_conv1d_step.restype = i32
+    lib.ssd_conv1d_step.argtypes = [C.POINTER(SsdConvDims)] + [vp] * 6
+    lib.ssd_linear_workspace_bytes.restype = sz
+    lib.ssd_linear_workspace_bytes.argtypes = [C.POINTER(SsdLinearDims), i32]
+    lib.ssd_linear_forward.restype = i32
+    lib.ssd_linear_forward.argtypes = [C.POINTER(SsdLinearDims)] + [vp] * 7 + [sz, vp]
+    lib.ssd_linear_backward.restype = i32
+    lib.ssd_linear_backward.argtypes = [C.POINTER(SsdLinearDims)] + [vp] * 4 + [i64] + [vp] * 4 + [sz, vp]
     lib.ssd_version.restype = i32
     lib.ssd_compiled_arch.restype = i32
     _lib = lib
@@ -204,7 +258,9 @@ def host():
     names = ("ssd_workspace_bytes", "ssd_forward_staged", "ssd_backward_staged", "ssd_state_update", "ssd_state_update_host",
              "ssd_last_error",
              "ssd_conv1d_workspace_bytes", "ssd_conv1d_forward", "ssd_conv1d_backward", "ssd_rmsnorm_workspace_bytes",
-             "ssd_rmsnorm_forward", "ssd_rmsnorm_backward")
+             "ssd_rmsnorm_forward", "ssd_rmsnorm_backward", "ssd_selscan_workspace_bytes", "ssd_selscan_forward", "ssd_selscan_backward",
+             "ssd_selscan_step", "ssd_conv1d_carry_workspace_bytes", "ssd_conv1d_carry_forward", "ssd_conv1d_carry_backward",
+             "ssd_conv1d_step", "ssd_linear_workspace_bytes", "ssd_linear_forward", "ssd_linear_backward")
     mod.bind(tuple(C.cast(getattr(lib, n), C.c_void_p).value for n in names), SsdError, torch.OutOfMemoryError)
     _host = mod
     return mod

@@ -21,6 +21,7 @@
 #include <cstring>
 #include <sstream>
 #include <string>
+#include <vector>
 
 #include "../../include/ssd_b200.h"
 
@@ -44,6 +45,17 @@ struct Api {
   decltype(&::ssd_rmsnorm_workspace_bytes) rmsnorm_workspace_bytes;
   decltype(&::ssd_rmsnorm_forward) rmsnorm_forward;
   decltype(&::ssd_rmsnorm_backward) rmsnorm_backward;
+  decltype(&::ssd_selscan_workspace_bytes) selscan_workspace_bytes;
+  decltype(&::ssd_selscan_forward) selscan_forward;
+  decltype(&::ssd_selscan_backward) selscan_backward;
+  decltype(&::ssd_selscan_step) selscan_step;
+  decltype(&::ssd_conv1d_carry_workspace_bytes) conv1d_carry_workspace_bytes;
+  decltype(&::ssd_conv1d_carry_forward) conv1d_carry_forward;
+  decltype(&::ssd_conv1d_carry_backward) conv1d_carry_backward;
+  decltype(&::ssd_conv1d_step) conv1d_step;
+  decltype(&::ssd_linear_workspace_bytes) linear_workspace_bytes;
+  decltype(&::ssd_linear_forward) linear_forward;
+  decltype(&::ssd_linear_backward) linear_backward;
 } api;
 PyObject *ssd_error = nullptr, *oom_error = nullptr;   // _lib.SsdError, torch.OutOfMemoryError
 constexpr int32_t kAllStages = SSD_STAGE_LOCAL | SSD_STAGE_FINISH;
@@ -397,6 +409,269 @@ void norm_backward(const Tensor& in, const Tensor* weight, const Tensor& rstd, c
                                 ws.defined() ? (size_t)ws.numel() : 0, stream_of(dev)));
 }
 
+// ---- selective scan, convolution with history, projection ---------------------------------------------------------------
+// Distance between rows along `dim`; 0 ("dense") where there is one row, whose stride says nothing.
+int64_t apart(const Tensor& t, int dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+// A [.., rows, inner] operand whose inner dims (all from `outer` on) are dense and whose rows lie apart.
+void check_rows(const char* name, const Tensor& t, at::IntArrayRef shape, int outer, at::ScalarType dtype, const at::Device& dev) {
+  if (!same(t, shape)) fail(name, ": expected shape ", shape, ", got ", t.sizes());
+  if (t.scalar_type() != dtype) fail(name, ": expected dtype ", dtype, ", got ", t.scalar_type());
+  if (t.device() != dev) fail(name, ": expected device ", dev, ", got ", t.device());
+  int64_t dense = 1;
+  for (int i = (int)t.dim() - 1; i >= outer; --i) {
+    if (t.size(i) > 1 && t.stride(i) != dense) fail(name, ": the dims from ", (int64_t)outer, " on must be dense");
+    dense *= t.size(i);
+  }
+  if (overlaid(t, outer)) fail(name, ": expanded over a dim (stride 0); make it contiguous");
+}
+void check_lengths(const Tensor* t, int64_t batch, const at::Device& dev) {
+  if (t && (t->dim() != 1 || t->size(0) != batch || t->scalar_type() != at::kInt || t->device() != dev || !t->is_contiguous()))
+    fail("lengths: expected ", batch, " contiguous int32 values on ", dev, ", got ", t->sizes(), " ", t->scalar_type(), " on ", t->device());
+}
+// An incoming gradient as the kernels read it: storage type, dense channels, rows apart.
+Tensor usable_rows(const Tensor& g, const Tensor& like, int outer) {
+  if (!g.defined()) return at::zeros(like.sizes(), like.options().requires_grad(false));
+  Tensor d = g.scalar_type() == like.scalar_type() ? g : g.to(like.scalar_type());
+  int64_t dense = 1;
+  bool ok = !overlaid(d, outer);
+  for (int i = (int)d.dim() - 1; i >= outer; --i) {
+    ok = ok && (d.size(i) <= 1 || d.stride(i) == dense);
+    dense *= d.size(i);
+  }
+  return ok ? d : d.contiguous();
+}
+
+struct Sel {
+  const Tensor &x, &dt, &A, &Bm, &Cm;
+  const Tensor *D, *z, *init, *bias, *lengths;
+  bool softplus;
+};
+SsdSelDims sel_dims(const Sel& s, const Tensor* y) {
+  if (!s.x.is_cuda()) fail("x must be a CUDA tensor (there is no CPU path)");
+  if (s.x.dim() != 3) fail("x must be [batch, seqlen, channels]");
+  const int32_t dtype = storage_type(s.x);
+  const at::Device dev = s.x.device();
+  const at::ScalarType st = s.x.scalar_type();
+  const int64_t B = s.x.size(0), L = s.x.size(1), D = s.x.size(2);
+  if (s.A.dim() != 2) fail("A must be [channels, dstate]");
+  const int64_t N = s.A.size(1);
+  if (s.Bm.dim() != 3 && s.Bm.dim() != 4) fail("B must be [batch, seqlen, ngroups, dstate] or [batch, seqlen, dstate]");
+  const int64_t G = s.Bm.dim() == 4 ? s.Bm.size(2) : 1;
+  if (G <= 0 || D % G) fail("channels (", D, ") must be a multiple of ngroups (", G, ")");
+  check_rows("x", s.x, Shape(B, L, D), 2, st, dev);
+  check_rows("dt", s.dt, Shape(B, L, D), 2, st, dev);
+  for (const Tensor* t : {&s.Bm, &s.Cm}) {
+    const char* name = t == &s.Bm ? "B" : "C";
+    if (s.Bm.dim() == 4) check_rows(name, *t, Shape(B, L, G, N), 2, st, dev);
+    else check_rows(name, *t, Shape(B, L, N), 2, st, dev);
+  }
+  check_dense_f32("A", &s.A, Shape(D, N), dev);
+  check_dense_f32("D", s.D, Shape(D), dev);
+  check_dense_f32("dt_bias", s.bias, Shape(D), dev);
+  check_dense_f32("init_state", s.init, Shape(B, D, N), dev);
+  check_lengths(s.lengths, B, dev);
+  SsdSelDims d;
+  std::memset(&d, 0, sizeof d);
+  d.batch = (int32_t)B; d.seqlen = (int32_t)L; d.channels = (int32_t)D; d.dstate = (int32_t)N; d.ngroups = (int32_t)G;
+  d.dtype = dtype; d.device = dev.index(); d.dt_softplus = s.softplus ? 1 : 0;
+  d.x_stride_b = apart(s.x, 0); d.x_stride_l = apart(s.x, 1);
+  d.dt_stride_b = apart(s.dt, 0); d.dt_stride_l = apart(s.dt, 1);
+  d.b_stride_b = apart(s.Bm, 0); d.b_stride_l = apart(s.Bm, 1);
+  d.c_stride_b = apart(s.Cm, 0); d.c_stride_l = apart(s.Cm, 1);
+  if (s.z) {
+    check_rows("z", *s.z, Shape(B, L, D), 2, st, dev);
+    d.z_stride_b = apart(*s.z, 0); d.z_stride_l = apart(*s.z, 1);
+  }
+  if (y) {
+    check_rows("y/dy", *y, Shape(B, L, D), 2, st, dev);
+    d.y_stride_b = apart(*y, 0); d.y_stride_l = apart(*y, 1);
+  }
+  return d;
+}
+Tensor bytes_on(size_t n, const at::Device& dev) {
+  if (!n) throw LibError(-1, api.last_error());
+  return empty(Shape((int64_t)n), at::kByte, dev);
+}
+void sel_forward(const Sel& s, Tensor& y, Tensor& fin, Tensor& ws, bool for_backward) {
+  SsdSelDims d = sel_dims(s, nullptr);
+  const at::Device dev = s.x.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  y = empty(s.x.sizes(), s.x.scalar_type(), dev);
+  fin = empty(Shape(d.batch, d.channels, d.dstate), at::kFloat, dev);
+  const size_t need = api.selscan_workspace_bytes(&d, for_backward ? SSD_PASS_BWD : SSD_PASS_FWD);
+  if (ws.defined()) check_workspace(ws, dev); else ws = bytes_on(need, dev);
+  SsdSelFwdPtrs p;
+  std::memset(&p, 0, sizeof p);
+  p.x = ptr(&s.x); p.dt = ptr(&s.dt); p.A = fptr(&s.A); p.Bm = ptr(&s.Bm); p.Cm = ptr(&s.Cm); p.D = fptr(s.D); p.z = ptr(s.z);
+  p.init_state = fptr(s.init); p.y = ptr(&y); p.final_state = fptr(&fin); p.dt_bias = fptr(s.bias); p.lengths = (const int32_t*)ptr(s.lengths);
+  check_rc(api.selscan_forward(&d, &p, ws.data_ptr(), (size_t)ws.nbytes(), stream_of(dev)));
+}
+struct SelGrads { Tensor dx, ddt, dA, dB, dC, dD, dz, dinit, dbias; };
+void sel_backward(const Sel& s, const Tensor& dy, const Tensor* dfin, Tensor& ws, bool saved, SelGrads& o) {
+  const SsdSelDims d = sel_dims(s, &dy);
+  const at::Device dev = s.x.device();
+  const at::ScalarType st = s.x.scalar_type();
+  check_dense_f32("dfinal_state", dfin, Shape(d.batch, d.channels, d.dstate), dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  o.dx = empty(s.x.sizes(), st, dev); o.ddt = empty(s.x.sizes(), st, dev);
+  o.dA = empty(s.A.sizes(), at::kFloat, dev);
+  o.dB = empty(s.Bm.sizes(), st, dev); o.dC = empty(s.Cm.sizes(), st, dev);
+  if (s.D) o.dD = empty(s.D->sizes(), at::kFloat, dev);
+  if (s.z) o.dz = empty(s.x.sizes(), st, dev);
+  if (s.init) o.dinit = empty(s.init->sizes(), at::kFloat, dev);
+  if (s.bias) o.dbias = empty(s.bias->sizes(), at::kFloat, dev);
+  if (ws.defined()) {
+    check_workspace(ws, dev);
+  } else {
+    saved = false;
+    ws = bytes_on(api.selscan_workspace_bytes(&d, SSD_PASS_BWD), dev);
+  }
+  SsdSelBwdPtrs p;
+  std::memset(&p, 0, sizeof p);
+  p.x = ptr(&s.x); p.dt = ptr(&s.dt); p.A = fptr(&s.A); p.Bm = ptr(&s.Bm); p.Cm = ptr(&s.Cm); p.D = fptr(s.D); p.z = ptr(s.z);
+  p.init_state = fptr(s.init); p.dy = ptr(&dy); p.dfinal_state = fptr(dfin); p.dx = ptr(&o.dx); p.ddt = ptr(&o.ddt); p.dA = fptr(&o.dA);
+  p.dB = ptr(&o.dB); p.dC = ptr(&o.dC); p.dD = fptr(&o.dD); p.dz = ptr(&o.dz); p.dinit_state = fptr(&o.dinit); p.dt_bias = fptr(s.bias);
+  p.ddt_bias = fptr(&o.dbias); p.lengths = (const int32_t*)ptr(s.lengths); p.fwd_saved = saved ? 1 : 0;
+  check_rc(api.selscan_backward(&d, &p, ws.data_ptr(), (size_t)ws.nbytes(), stream_of(dev)));
+}
+
+void check_history(const char* name, const Tensor* h, const Tensor& in, int64_t width) {
+  if (!h) return;
+  const Shape shape(in.size(0), width - 1, in.size(-1));
+  if (!same(*h, shape) || h->scalar_type() != in.scalar_type() || h->device() != in.device() || !h->is_contiguous())
+    fail("conv1d: ", name, ": expected a contiguous ", at::IntArrayRef(shape), " ", in.scalar_type(), " tensor on ", in.device(), ", got ",
+         h->sizes(), " ", h->scalar_type(), " on ", h->device());
+}
+SsdConvDims carry_dims(const Tensor& in, const Tensor& weight, const Tensor* bias, bool activation) {
+  if (!in.is_cuda() || in.dim() != 3) fail("conv1d: input must be a CUDA [batch, seqlen, channels] bf16/fp32 tensor");
+  check_conv_weights(in, weight, bias);
+  storage_type(in);
+  check_rows("conv1d: input", in, Shape(in.size(0), in.size(1), in.size(2)), 2, in.scalar_type(), in.device());
+  SsdConvDims d = conv_dims(in, in, weight.size(1), activation);
+  const int64_t C = in.size(2);
+  d.out_stride_l = C; d.out_stride_b = C * in.size(1);
+  if (in.size(1) <= 1) d.in_stride_l = C;
+  if (in.size(0) <= 1) d.in_stride_b = d.in_stride_l * in.size(1);
+  return d;
+}
+void carry_forward(const Tensor& in, const Tensor& weight, const Tensor* bias, const Tensor* hist, const Tensor* lengths, bool activation,
+                   Tensor& out, Tensor& nh) {
+  const SsdConvDims d = carry_dims(in, weight, bias, activation);
+  const at::Device dev = in.device();
+  check_history("history", hist, in, d.width);
+  check_lengths(lengths, d.batch, dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  out = empty(in.sizes(), in.scalar_type(), dev);
+  nh = empty(Shape(d.batch, d.width - 1, d.channels), in.scalar_type(), dev);
+  check_rc(api.conv1d_carry_forward(&d, ptr(&in), fptr(&weight), fptr(bias), ptr(hist), (const int32_t*)ptr(lengths), ptr(&out), ptr(&nh),
+                                    stream_of(dev)));
+}
+struct CarryGrads { Tensor din, dweight, dbias, dhist; };
+CarryGrads carry_backward(const Tensor& in, const Tensor& weight, const Tensor* bias, const Tensor* hist, const Tensor& dout,
+                          const Tensor* dnew, const Tensor* lengths, bool activation) {
+  const SsdConvDims d = carry_dims(in, weight, bias, activation);
+  const at::Device dev = in.device();
+  check_history("history", hist, in, d.width);
+  check_history("gradient of the new history", dnew, in, d.width);
+  check_lengths(lengths, d.batch, dev);
+  check_rows("conv1d: dout", dout, in.sizes(), 2, in.scalar_type(), dev);
+  const c10::cuda::CUDAGuard guard(dev);
+  CarryGrads g;
+  g.din = empty(in.sizes(), in.scalar_type(), dev);
+  g.dweight = empty(weight.sizes(), at::kFloat, dev);
+  if (bias) g.dbias = empty(bias->sizes(), at::kFloat, dev);
+  if (hist) g.dhist = empty(hist->sizes(), in.scalar_type(), dev);
+  Tensor ws = bytes_on(api.conv1d_carry_workspace_bytes(&d), dev);
+  const int64_t sl = dout.size(1) > 1 ? dout.stride(1) : (int64_t)d.channels, sb = dout.size(0) > 1 ? dout.stride(0) : sl * dout.size(1);
+  check_rc(api.conv1d_carry_backward(&d, ptr(&in), fptr(&weight), fptr(bias), ptr(hist), (const int32_t*)ptr(lengths), ptr(&dout), sb, sl,
+                                     ptr(dnew), ptr(&g.din), ptr(&g.dhist), fptr(&g.dweight), fptr(&g.dbias), ws.data_ptr(),
+                                     (size_t)ws.numel(), stream_of(dev)));
+  return g;
+}
+
+// [.., features] as rows of `features` dense values; a copy only where the rows have no one distance.
+Tensor as_rows(const char* name, const Tensor& t, int64_t features) {
+  if (t.dim() < 1 || t.size(-1) != features) fail("linear: ", name, ": expected ", features, " values in the last dim, got ", t.sizes());
+  Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / features, features});
+  if ((features > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < features)) r = r.contiguous();
+  return r;
+}
+SsdLinearDims linear_dims(const Tensor& x, const Tensor& w, int64_t act) {
+  if (!x.is_cuda()) fail("x must be a CUDA tensor (there is no CPU path)");
+  const int32_t dtype = storage_type(x);
+  if (w.dim() != 2 || w.scalar_type() != x.scalar_type() || w.device() != x.device() || !w.is_contiguous())
+    fail("linear: weight must be a contiguous [out_features, in_features] ", x.scalar_type(), " tensor on ", x.device());
+  SsdLinearDims d;
+  std::memset(&d, 0, sizeof d);
+  d.in_features = (int32_t)w.size(1); d.out_features = (int32_t)w.size(0);
+  d.dtype = dtype; d.device = x.device().index(); d.activation = (int32_t)act;
+  return d;
+}
+Tensor like_rows(const Tensor& x, int64_t features, at::ScalarType st) {   // x's leading dims with `features` in the last one
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = features;
+  return empty(shape, st, x.device());
+}
+void check_vec(const char* name, const Tensor* t, int64_t n, const Tensor& x) {
+  if (t && (t->numel() != n || t->scalar_type() != x.scalar_type() || t->device() != x.device() || !t->is_contiguous()))
+    fail("linear: ", name, ": expected ", n, " contiguous ", x.scalar_type(), " values on ", x.device(), ", got ", t->sizes(), " ",
+         t->scalar_type(), " on ", t->device());
+}
+void linear_fwd(const Tensor& x, const Tensor& w, const Tensor* bias, const Tensor* res, int64_t act, bool for_backward, Tensor& out, Tensor& pre) {
+  SsdLinearDims d = linear_dims(x, w, act);
+  const at::Device dev = x.device();
+  const int64_t N = d.out_features;
+  check_vec("bias", bias, N, x);
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor xr = as_rows("x", x, d.in_features);
+  d.rows = xr.size(0); d.x_stride_row = apart(xr, 0);
+  Tensor rr;
+  if (res) {
+    if (res->scalar_type() != x.scalar_type() || res->device() != dev || res->dim() != x.dim() || res->numel() != d.rows * N || res->size(-1) != N)
+      fail("linear: residual: expected x's leading dims with ", N, " values in the last, ", x.scalar_type(), " on ", dev, ", got ", res->sizes(),
+           " ", res->scalar_type(), " on ", res->device());
+    for (int64_t i = 0; i + 1 < x.dim(); ++i) if (res->size(i) != x.size(i)) fail("linear: residual: leading dims ", res->sizes(), " do not match x's ", x.sizes());
+    rr = as_rows("residual", *res, N);
+    d.residual_stride_row = apart(rr, 0);
+  }
+  if (out.defined()) {
+    if (out.scalar_type() != x.scalar_type() || out.device() != dev || !out.is_contiguous() || out.dim() != x.dim() || out.numel() != d.rows * N || out.size(-1) != N)
+      fail("linear: out: expected a contiguous tensor of x's leading dims with ", N, " values in the last, ", x.scalar_type(), " on ", dev,
+           ", got ", out.sizes(), " ", out.scalar_type(), " on ", out.device());
+  } else {
+    out = like_rows(x, N, x.scalar_type());
+  }
+  if (for_backward && act) pre = like_rows(x, N, x.scalar_type());
+  Tensor ws = bytes_on(api.linear_workspace_bytes(&d, SSD_PASS_FWD), dev);
+  check_rc(api.linear_forward(&d, ptr(&xr), ptr(&w), ptr(bias), ptr(&rr), ptr(&out), ptr(&pre), ws.data_ptr(), (size_t)ws.numel(), stream_of(dev)));
+}
+struct LinGrads { Tensor dx, dw, db; };
+LinGrads linear_bwd(const Tensor& dout, const Tensor& x, const Tensor& w, const Tensor* pre, int64_t act, bool want_dx, bool want_dw, bool want_db) {
+  SsdLinearDims d = linear_dims(x, w, act);
+  const at::Device dev = x.device();
+  const int64_t N = d.out_features;
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor xr = as_rows("x", x, d.in_features);
+  d.rows = xr.size(0); d.x_stride_row = apart(xr, 0);
+  auto check = [&](const char* name, const Tensor& t) {
+    if (t.scalar_type() != x.scalar_type() || t.device() != dev || t.dim() < 1 || t.size(-1) != N || t.numel() != d.rows * N)
+      fail("linear: ", name, ": expected x's leading dims with ", N, " values in the last, ", x.scalar_type(), " on ", dev, ", got ", t.sizes(), " ",
+           t.scalar_type(), " on ", t.device());
+  };
+  check("dout", dout);
+  if (act && !pre) fail("linear: an activation needs the pre that the forward returned with for_backward");
+  if (pre) { check("pre", *pre); if (!pre->is_contiguous()) fail("linear: pre must be contiguous"); }
+  const Tensor gr = as_rows("dout", dout, N);
+  LinGrads g;
+  if (want_dx) g.dx = empty(x.sizes(), x.scalar_type(), dev);
+  if (want_dw) g.dw = empty(w.sizes(), x.scalar_type(), dev);
+  if (want_db) g.db = empty(Shape(N), x.scalar_type(), dev);
+  Tensor ws = bytes_on(api.linear_workspace_bytes(&d, SSD_PASS_BWD), dev);
+  check_rc(api.linear_backward(&d, ptr(&xr), ptr(&w), ptr(pre), ptr(&gr), apart(gr, 0), ptr(&g.dx), ptr(&g.dw), ptr(&g.db), ws.data_ptr(),
+                               (size_t)ws.numel(), stream_of(dev)));
+  return g;
+}
+
 // ---- autograd nodes ----------------------------------------------------------------------------------------------------
 bool any_requires_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
@@ -495,6 +770,74 @@ struct MixerNode : public torch::autograd::Function<MixerNode> {
     ConvGrads c = conv_backward(xBC, cw, or_null(v[4]), douts, 3, true);
     return {c.din, as_type(g.ddt, dt.scalar_type()), g.dz, c.dweight, v[4].defined() ? c.dbias : Tensor(), g.dbias, g.dA, g.dD, dnw, g.dinit,
             Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct SelNode : public torch::autograd::Function<SelNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& Bm, const Tensor& Cm,
+                               const Opt& D, const Opt& z, const Opt& init, const Opt& bias, const Opt& lengths, bool softplus) {
+    const Sel s{x, dt, A, Bm, Cm, or_null(D), or_null(z), or_null(init), or_null(bias), or_null(lengths), softplus};
+    Tensor y, fin, ws;
+    sel_forward(s, y, fin, ws, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, dt, A, Bm, Cm, or_undefined(D), or_undefined(z), or_undefined(init), or_undefined(bias), or_undefined(lengths), ws});
+    ctx->saved_data["softplus"] = softplus;
+    return {y, fin};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list v = ctx->get_saved_variables();
+    const Sel s{v[0], v[1], v[2], v[3], v[4], or_null(v[5]), or_null(v[6]), or_null(v[7]), or_null(v[8]), or_null(v[9]),
+                ctx->saved_data["softplus"].toBool()};
+    const Tensor dy = usable_rows(grads[0], s.x, 2);
+    const Tensor dfin = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    Tensor ws = v[10];
+    SelGrads g;
+    sel_backward(s, dy, or_null(dfin), ws, true, g);
+    return {g.dx, g.ddt, g.dA, g.dB, g.dC, g.dD, g.dz, g.dinit, g.dbias, Tensor(), Tensor()};
+  }
+};
+
+struct CarryNode : public torch::autograd::Function<CarryNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& in, const Tensor& w, const Opt& b, const Opt& hist, const Opt& lengths,
+                               bool activation) {
+    Tensor out, nh;
+    carry_forward(in, w, or_null(b), or_null(hist), or_null(lengths), activation, out, nh);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({in, w, or_undefined(b), or_undefined(hist), or_undefined(lengths)});
+    ctx->saved_data["activation"] = activation;
+    return {out, nh};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list v = ctx->get_saved_variables();
+    Tensor dout = usable_rows(grads[0], v[0], 2);
+    const int64_t e = dout.element_size();
+    if ((uintptr_t)dout.data_ptr() % 16 || apart(dout, 1) * e % 16 || apart(dout, 0) * e % 16) dout = dout.contiguous().clone();
+    const Tensor dnew = grads[1].defined() ? as_type(grads[1], v[0].scalar_type()).contiguous() : Tensor();
+    CarryGrads g = carry_backward(v[0], v[1], or_null(v[2]), or_null(v[3]), dout, or_null(dnew), or_null(v[4]), ctx->saved_data["activation"].toBool());
+    return {g.din, g.dweight, g.dbias, g.dhist, Tensor(), Tensor()};
+  }
+};
+
+struct LinearNode : public torch::autograd::Function<LinearNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Opt& b, const Opt& res, int64_t act) {
+    Tensor out, pre;
+    linear_fwd(x, w, or_null(b), or_null(res), act, true, out, pre);
+    ctx->save_for_backward({x, w, pre});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["bias"] = b.has_value() ? b->sizes().vec() : std::vector<int64_t>{};
+    ctx->saved_data["given"] = (int64_t)(b.has_value() + 2 * res.has_value());
+    return {out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list v = ctx->get_saved_variables();
+    const Tensor dout = as_type(grads[0], v[0].scalar_type());
+    const int64_t given = ctx->saved_data["given"].toInt();   // absent operands have no place in the node's list of inputs
+    const bool want_db = (given & 1) && ctx->needs_input_grad(2), want_dr = (given & 2) && ctx->needs_input_grad(given & 1 ? 3 : 2);
+    LinGrads g;
+    if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1) || want_db)
+      g = linear_bwd(dout, v[0], v[1], or_null(v[2]), ctx->saved_data["act"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1), want_db);
+    if (want_db) g.db = g.db.view(ctx->saved_data["bias"].toIntVector());
+    return {g.dx, g.dw, g.db, want_dr ? dout : Tensor(), Tensor()};
   }
 };
 
@@ -738,6 +1081,187 @@ PyObject* py_norm_backward(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   });
 }
 
+Sel sel_of(const Args& a, int at, int bias, int softplus, int lengths) {
+  return {a.tensor(at, "x"), a.tensor(at + 1, "dt"), a.tensor(at + 2, "A"), a.tensor(at + 3, "B"), a.tensor(at + 4, "C"), a.opt(at + 5, "D"),
+          a.opt(at + 6, "z"), a.opt(at + 7, "init_state"), a.opt(bias, "dt_bias"), a.opt(lengths, "lengths"), a.flag(softplus)};
+}
+// x, dt, A, B, C, D, z, init_state, dt_bias, dt_softplus, lengths, for_backward, workspace -> y, final_state, workspace
+PyObject* py_sel_forward(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  return guarded([&]() -> PyObject* {
+    const Args a(argv, argc, 13);
+    Tensor y, fin, ws = or_undefined(a.opt(12, "workspace"));
+    sel_forward(sel_of(a, 0, 8, 9, 10), y, fin, ws, a.flag(11));
+    return triple(y, fin, ws);
+  });
+}
+// dy, x, dt, A, B, C, D, z, init_state, dfinal_state, dt_bias, dt_softplus, lengths, workspace -> dict
+PyObject* py_sel_backward(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  return guarded([&]() -> PyObject* {
+    const Args a(argv, argc, 14);
+    const Sel s = sel_of(a, 1, 10, 11, 12);
+    Tensor ws = or_undefined(a.opt(13, "workspace"));
+    SelGrads g;
+    sel_backward(s, a.tensor(0, "dy"), a.opt(9, "dfinal_state"), ws, true, g);
+    PyObject* out = PyDict_New();
+    if (!out) throw std::runtime_error("out of memory");
+    struct { const char* key; const Tensor* t; } const slots[] = {{"dx", &g.dx}, {"ddt", &g.ddt}, {"dA", &g.dA}, {"dB", &g.dB}, {"dC", &g.dC},
+        {"dD", &g.dD}, {"dz", &g.dz}, {"dinit", &g.dinit}, {"ddt_bias", &g.dbias}};
+    for (const auto& e : slots) {
+      if (!e.t->defined()) continue;
+      PyObject* o = wrap(*e.t);
+      const int bad = !o || PyDict_SetItemString(out, e.key, o);
+      Py_XDECREF(o);
+      if (bad) { Py_DECREF(out); throw std::runtime_error("cannot store a result"); }
+    }
+    return out;
+  });
+}
+// x, dt, A, B, C, D, z, init_state, dt_bias, dt_softplus, lengths -> y, final_state (differentiable)
+PyObject* py_sel_scan(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  return guarded([&]() -> PyObject* {
+    const Args a(argv, argc, 11);
+    const Sel s = sel_of(a, 0, 8, 9, 10);
+    if (!any_requires_grad({&s.x, &s.dt, &s.A, &s.Bm, &s.Cm, s.D, s.z, s.init, s.bias})) {
+      Tensor y, fin, ws;
+      sel_forward(s, y, fin, ws, false);
+      return pair(y, fin);
+    }
+    const variable_list r = SelNode::apply(s.x, s.dt, s.A, s.Bm, s.Cm, optional(s.D), optional(s.z), optional(s.init), optional(s.bias),
+                                           optional(s.lengths), s.softplus);
+    return pair(r[0], r[1]);
+  });
+}
+// state, x, dt, A, B, C, D, z, y, dt_bias, dt_softplus -> y
+PyObject* py_sel_step(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  return guarded([&]() -> PyObject* {
+    const Args a(argv, argc, 11);
+    const Tensor &state = a.tensor(0, "state"), &x = a.tensor(1, "x"), &dt = a.tensor(2, "dt"), &A = a.tensor(3, "A"), &Bm = a.tensor(4, "B"),
+                 &Cm = a.tensor(5, "C");
+    const Tensor *D = a.opt(6, "D"), *z = a.opt(7, "z"), *y_in = a.opt(8, "y"), *bias = a.opt(9, "dt_bias");
+    if (!state.is_cuda()) fail("state must be a CUDA tensor (there is no CPU path)");
+    const at::Device dev = state.device();
+    if (state.dim() != 3 || state.scalar_type() != at::kFloat || !state.is_contiguous())
+      fail("state must be a contiguous float32 [streams, channels, dstate] tensor");
+    const int64_t S = state.size(0), C = state.size(1), N = state.size(2);
+    const at::ScalarType st = x.scalar_type();
+    SsdSelStepDims d;
+    std::memset(&d, 0, sizeof d);
+    d.dtype = storage_type(x);
+    if (Bm.dim() != 2 && Bm.dim() != 3) fail("B must be [streams, ngroups, dstate] or [streams, dstate]");
+    const int64_t G = Bm.dim() == 3 ? Bm.size(1) : 1;
+    if (G <= 0 || C % G) fail("channels (", C, ") must be a multiple of ngroups (", G, ")");
+    check_rows("x", x, Shape(S, C), 1, st, dev);
+    check_rows("dt", dt, Shape(S, C), 1, st, dev);
+    for (const Tensor* t : {&Bm, &Cm}) {
+      const char* name = t == &Bm ? "B" : "C";
+      if (Bm.dim() == 3) check_rows(name, *t, Shape(S, G, N), 1, st, dev);
+      else check_rows(name, *t, Shape(S, N), 1, st, dev);
+    }
+    if (z) check_rows("z", *z, Shape(S, C), 1, st, dev);
+    check_dense_f32("A", &A, Shape(C, N), dev);
+    check_dense_f32("D", D, Shape(C), dev);
+    check_dense_f32("dt_bias", bias, Shape(C), dev);
+    const c10::cuda::CUDAGuard guard(dev);
+    if (y_in) check_rows("y", *y_in, Shape(S, C), 1, st, dev);
+    Tensor y = y_in ? *y_in : empty(Shape(S, C), st, dev);
+    d.streams = (int32_t)S; d.channels = (int32_t)C; d.dstate = (int32_t)N; d.ngroups = (int32_t)G; d.device = dev.index();
+    d.dt_softplus = a.flag(10) ? 1 : 0;
+    d.x_stride_s = apart(x, 0); d.dt_stride_s = apart(dt, 0); d.b_stride_s = apart(Bm, 0); d.c_stride_s = apart(Cm, 0);
+    d.z_stride_s = z ? apart(*z, 0) : 0; d.y_stride_s = apart(y, 0);
+    SsdStepPtrs p;
+    std::memset(&p, 0, sizeof p);
+    p.state = fptr(&state); p.x = ptr(&x); p.dt = ptr(&dt); p.A = fptr(&A); p.Bm = ptr(&Bm); p.Cm = ptr(&Cm); p.D = fptr(D); p.z = ptr(z);
+    p.y = ptr(&y); p.dt_bias = fptr(bias);
+    check_rc(api.selscan_step(&d, &p, stream_of(dev)));
+    return wrap(y);
+  });
+}
+// in, weight, bias, history, lengths, activation -> out, new_history
+PyObject* py_carry_forward(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  return guarded([&]() -> PyObject* {
+    const Args a(argv, argc, 6);
+    Tensor out, nh;
+    carry_forward(a.tensor(0, "input"), a.tensor(1, "weight"), a.opt(2, "bias"), a.opt(3, "history"), a.opt(4, "lengths"), a.flag(5), out, nh);
+    return pair(out, nh);
+  });
+}
+// in, weight, bias, history, dout, dnew_history, lengths, activation -> din, dweight, dbias, dhistory
+PyObject* py_carry_backward(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  return guarded([&]() -> PyObject* {
+    const Args a(argv, argc, 8);
+    const CarryGrads g = carry_backward(a.tensor(0, "input"), a.tensor(1, "weight"), a.opt(2, "bias"), a.opt(3, "history"), a.tensor(4, "dout"),
+                                        a.opt(5, "dnew_history"), a.opt(6, "lengths"), a.flag(7));
+    return Py_BuildValue("(NNNN)", wrap(g.din), wrap(g.dweight), wrap(g.dbias), wrap(g.dhist));
+  });
+}
+// in, weight, bias, history, lengths, activation -> out, new_history (differentiable)
+PyObject* py_carry(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  return guarded([&]() -> PyObject* {
+    const Args a(argv, argc, 6);
+    const Tensor &in = a.tensor(0, "input"), &w = a.tensor(1, "weight");
+    const Tensor *b = a.opt(2, "bias"), *h = a.opt(3, "history"), *l = a.opt(4, "lengths");
+    if (!any_requires_grad({&in, &w, b, h})) {
+      Tensor out, nh;
+      carry_forward(in, w, b, h, l, a.flag(5), out, nh);
+      return pair(out, nh);
+    }
+    const variable_list r = CarryNode::apply(in, w, optional(b), optional(h), optional(l), a.flag(5));
+    return pair(r[0], r[1]);
+  });
+}
+// history, in, weight, bias, activation, out -> out
+PyObject* py_conv_step(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  return guarded([&]() -> PyObject* {
+    const Args a(argv, argc, 6);
+    const Tensor &hist = a.tensor(0, "history"), &in = a.tensor(1, "input"), &w = a.tensor(2, "weight");
+    const Tensor *b = a.opt(3, "bias"), *out_in = a.opt(5, "out");
+    if (!in.is_cuda() || in.dim() != 2) fail("conv1d: input of a step must be a CUDA [streams, channels] bf16/fp32 tensor");
+    const at::Device dev = in.device();
+    check_rows("conv1d: input", in, Shape(in.size(0), in.size(1)), 1, in.scalar_type(), dev);
+    const Tensor in3 = in.unsqueeze(1);
+    SsdConvDims d = carry_dims(in3, w, b, a.flag(4));
+    check_history("history", &hist, in, d.width);
+    const c10::cuda::CUDAGuard guard(dev);
+    if (out_in) check_rows("conv1d: out", *out_in, Shape(in.size(0), in.size(1)), 1, in.scalar_type(), dev);
+    Tensor out = out_in ? *out_in : empty(Shape(in.size(0), in.size(1)), in.scalar_type(), dev);
+    d.out_stride_b = out.size(0) > 1 ? out.stride(0) : out.size(1);
+    if (out.size(0) > 1 && out.stride(0) < out.size(1)) fail("conv1d: out: rows must lie apart");
+    check_rc(api.conv1d_step(&d, ptr(&in), fptr(&w), fptr(b), ptr(&hist), ptr(&out), stream_of(dev)));
+    return wrap(out);
+  });
+}
+// x, weight, bias, residual, activation, for_backward, out -> out, pre
+PyObject* py_linear_forward(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  return guarded([&]() -> PyObject* {
+    const Args a(argv, argc, 7);
+    Tensor out = or_undefined(a.opt(6, "out")), pre;
+    linear_fwd(a.tensor(0, "x"), a.tensor(1, "weight"), a.opt(2, "bias"), a.opt(3, "residual"), a.integer(4), a.flag(5), out, pre);
+    return pair(out, pre);
+  });
+}
+// dout, x, weight, pre, activation, want_dx, want_dweight, want_dbias -> dx, dweight, dbias
+PyObject* py_linear_backward(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  return guarded([&]() -> PyObject* {
+    const Args a(argv, argc, 8);
+    const LinGrads g = linear_bwd(a.tensor(0, "dout"), a.tensor(1, "x"), a.tensor(2, "weight"), a.opt(3, "pre"), a.integer(4), a.flag(5), a.flag(6), a.flag(7));
+    return triple(g.dx, g.dw, g.db);
+  });
+}
+// x, weight, bias, residual, activation -> out (differentiable)
+PyObject* py_linear(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
+  return guarded([&]() -> PyObject* {
+    const Args a(argv, argc, 5);
+    const Tensor &x = a.tensor(0, "x"), &w = a.tensor(1, "weight");
+    const Tensor *b = a.opt(2, "bias"), *r = a.opt(3, "residual");
+    if (!any_requires_grad({&x, &w, b, r})) {
+      Tensor out, pre;
+      linear_fwd(x, w, b, r, a.integer(4), false, out, pre);
+      return wrap(out);
+    }
+    return wrap(LinearNode::apply(x, w, optional(b), optional(r), a.integer(4))[0]);
+  });
+}
+
 // addresses (a tuple in Api's order), SsdError, torch.OutOfMemoryError
 PyObject* py_bind(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   return guarded([&]() -> PyObject* {
@@ -758,7 +1282,11 @@ PyObject* py_bind(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
 PyMethodDef methods[] = {FAST("bind", py_bind), FAST("dims", py_dims), FAST("state_update", py_state_update), FAST("state_update_host", py_state_update_host), FAST("forward", py_forward),
                          FAST("backward", py_backward), FAST("scan", py_scan), FAST("mixer", py_mixer),
                          FAST("conv1d_forward", py_conv_forward), FAST("conv1d_backward", py_conv_backward),
-                         FAST("rmsnorm_forward", py_norm_forward), FAST("rmsnorm_backward", py_norm_backward), {nullptr, nullptr, 0, nullptr}};
+                         FAST("rmsnorm_forward", py_norm_forward), FAST("rmsnorm_backward", py_norm_backward),
+                         FAST("selscan_forward", py_sel_forward), FAST("selscan_backward", py_sel_backward), FAST("selscan", py_sel_scan),
+                         FAST("selscan_step", py_sel_step), FAST("carry_forward", py_carry_forward), FAST("carry_backward", py_carry_backward),
+                         FAST("carry", py_carry), FAST("conv1d_step", py_conv_step), FAST("linear_forward", py_linear_forward),
+                         FAST("linear_backward", py_linear_backward), FAST("linear", py_linear), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ssd_host", "native host path of the SSD entry points", -1, methods};
 
 }  // namespace

@@ -7,6 +7,7 @@
 //
 // The step-size activation softplus(dt + dt_bias) and the gate y*silu(z) need no kernel here: they are
 // evaluated inside the scan's own kernels.
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.cuh"
@@ -947,6 +948,255 @@ __global__ void __launch_bounds__(32 * RED_GROUPS) k_norm_reduce(int nblk, int w
   if (threadIdx.y == 0 && i < width) dweight[i] = a;
 }
 
+// ---------------------------------------------------------------------------------------------
+// The convolution with a carried history.  With ext = history (K-1 rows, zeros if absent) followed by the input,
+//     pre[t] = bias + sum_k w[k] ext[t+k],   out = act(pre),   new_history = ext[len .. len+K-2];
+// rows at or past a sequence's length are not read.
+struct Carry {
+  const void* history;     // [B, K-1, C] dense, or null
+  const int* lengths;      // [B], or null
+  int tiles;               // per sequence
+};
+__device__ __forceinline__ int carry_len(const SsdConvDims& d, const Carry& q, int b) {
+  return q.lengths ? min(max(q.lengths[b], 0), d.seqlen) : d.seqlen;
+}
+// row `e` of ext (e >= K-1: input row e-K+1, read when it is before the length), or zeros
+template <typename T, int K, int NC>
+__device__ __forceinline__ void load_ext(const T* in, const T* hist, long long stride_l, int channels, int e, int len, RawN<T, NC>& r) {
+  if (e >= K - 1) {
+    if (e - (K - 1) < len) { load_raw(in + (long long)(e - (K - 1)) * stride_l, r); return; }
+  } else if (e >= 0 && hist) {
+    load_raw(hist + (long long)e * channels, r);
+    return;
+  }
+  r = RawN<T, NC>{};
+}
+
+constexpr int CARRY_TL = 32;
+// Work item = (sequence, tile of 32 tokens, 16 bytes of channels), channels fastest; the thread walks its tile with the last K-1
+// rows in registers, eight rows requested at a time.  The items of a sequence's first tile also write the new history.
+template <typename T, int K>
+__global__ void __launch_bounds__(CONV_THREADS) k_carry_fwd(SsdConvDims d, Carry q, const T* __restrict__ in, const float* __restrict__ weight,
+                                                            const float* __restrict__ bias, T* __restrict__ out, T* __restrict__ nh) {
+  pdl_wait();
+  constexpr int NC = 16 / (int)sizeof(T), CH = 8;
+  const int CV = d.channels / NC;
+  const long long item = (long long)blockIdx.x * CONV_THREADS + threadIdx.x;
+  if (item >= (long long)d.batch * q.tiles * CV) return;
+  const int c0 = (int)(item % CV) * NC;
+  const long long bt = item / CV;
+  const int b = (int)(bt / q.tiles), tile = (int)(bt % q.tiles), t0 = tile * CARRY_TL, t1 = min(t0 + CARRY_TL, d.seqlen);
+  const int len = carry_len(d, q, b);
+  const T* ip = in + (long long)b * d.in_stride_b + c0;
+  const T* hp = q.history ? (const T*)q.history + (long long)b * (K - 1) * d.channels + c0 : nullptr;
+  T* op = out + (long long)b * d.out_stride_b + c0;
+  if (tile == 0 && nh) {
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) {
+      RawN<T, NC> r;
+      float v[NC];
+      load_ext<T, K, NC>(ip, hp, d.in_stride_l, d.channels, len + j, len, r);
+      unpack_raw(r, v);
+      store_n(nh + ((long long)b * (K - 1) + j) * d.channels + c0, v);
+    }
+  }
+  float w[NC][K], bs[NC], win[K][NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[j][k] = __ldg(weight + (size_t)(c0 + j) * K + k);
+    bs[j] = bias ? __ldg(bias + c0 + j) : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) {
+    RawN<T, NC> r;
+    load_ext<T, K, NC>(ip, hp, d.in_stride_l, d.channels, t0 + k, len, r);
+    unpack_raw(r, win[k]);
+  }
+  for (int tc = t0; tc < t1; tc += CH) {
+    RawN<T, NC> raw[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) load_ext<T, K, NC>(ip, hp, d.in_stride_l, d.channels, tc + i + K - 1, min(len, t1), raw[i]);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      unpack_raw(raw[i], win[K - 1]);
+      float o[NC];
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        float a = bs[j];
+#pragma unroll
+        for (int k = 0; k < K; ++k) a = fmaf(w[j][k], win[k][j], a);
+        o[j] = tc + i < len ? (d.activation ? a * sig_<T>(a) : a) : 0.f;
+      }
+      if (tc + i < t1) store_n(op + (long long)(tc + i) * d.out_stride_l, o);
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+        for (int j = 0; j < NC; ++j) win[k][j] = win[k + 1][j];
+    }
+  }
+}
+
+// Backward over the rows e of ext: dext[e] = sum_k w[k] dpre[e-k] (+ the gradient of the new history on its rows), which is
+// complete at step t = e of a walk forward in time.  Thread = (row of items, 8 bytes of channels); a row walks (sequence, tile of 64
+// ext rows) pairs, counts dpre of its own rows into dweight and dbias (tile sums first, then their sum) and leaves one partial row.
+// The sigmoid is exp and a division here in both storage types: dweight and dbias are fp32.
+constexpr int CARRY_TLB = 64, CARRY_ROWS = 1024;
+struct CarryBwd {
+  const void *dout, *dnew;
+  long long dout_sb, dout_sl;
+  void *din, *dhist;
+  int rows, tiles;
+};
+template <typename T, int K>
+__global__ void __launch_bounds__(CONV_THREADS) k_carry_bwd(SsdConvDims d, Carry q, CarryBwd g, const T* __restrict__ in,
+                                                            const float* __restrict__ weight, const float* __restrict__ bias,
+                                                            float* __restrict__ partial) {
+  pdl_wait();
+  constexpr int NC = 4, CH = 4;
+  const int CV = d.channels / NC;
+  const long long item = (long long)blockIdx.x * CONV_THREADS + threadIdx.x;
+  if (item >= (long long)g.rows * CV) return;
+  const int c0 = (int)(item % CV) * NC, row = (int)(item / CV);
+  float w[NC][K], bs[NC], dw[NC][K], db[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) { w[j][k] = __ldg(weight + (size_t)(c0 + j) * K + k); dw[j][k] = 0.f; }
+    bs[j] = bias ? __ldg(bias + c0 + j) : 0.f;
+    db[j] = 0.f;
+  }
+  const long long pairs = (long long)d.batch * g.tiles;
+  for (long long pair = row; pair < pairs; pair += g.rows) {
+    const int b = (int)(pair / g.tiles), e0 = (int)(pair - (long long)b * g.tiles) * CARRY_TLB, e1 = min(e0 + CARRY_TLB, d.seqlen + K - 1);
+    const int len = carry_len(d, q, b);
+    const T* ip = in + (long long)b * d.in_stride_b + c0;
+    const T* hp = q.history ? (const T*)q.history + (long long)b * (K - 1) * d.channels + c0 : nullptr;
+    const T* gp = (const T*)g.dout + (long long)b * g.dout_sb + c0;
+    const T* np = g.dnew ? (const T*)g.dnew + (long long)b * (K - 1) * d.channels + c0 : nullptr;
+    float win[K][NC], dpw[K][NC], tw[NC][K], tb[NC];   // win[k] = ext[t+k], dpw[k] = dpre[t-K+1+k]
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      tb[j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) { tw[j][k] = 0.f; dpw[k][j] = 0.f; }
+    }
+    const int tb0 = e0 - (K - 1);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+      RawN<T, NC> r;
+      load_ext<T, K, NC>(ip, hp, d.in_stride_l, d.channels, tb0 + k, len, r);
+      unpack_raw(r, win[k + 1]);
+    }
+    for (int tc = tb0; tc < e1; tc += CH) {
+      RawN<T, NC> rin[CH], rgo[CH];
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int t = tc + i;
+        load_ext<T, K, NC>(ip, hp, d.in_stride_l, d.channels, t + K - 1, t < e1 ? len : 0, rin[i]);
+        if (t >= 0 && t < len && t < e1) load_raw(gp + (long long)t * g.dout_sl, rgo[i]); else rgo[i] = RawN<T, NC>{};
+      }
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int t = tc + i;
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+          for (int j = 0; j < NC; ++j) { win[k][j] = win[k + 1][j]; dpw[k][j] = dpw[k + 1][j]; }
+        unpack_raw(rin[i], win[K - 1]);
+        float go[NC];
+        unpack_raw(rgo[i], go);
+        const bool own = t >= e0 && t < e1;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          float v = go[j];
+          if (d.activation) {
+            float a = bs[j];
+#pragma unroll
+            for (int k = 0; k < K; ++k) a = fmaf(w[j][k], win[k][j], a);
+            const float sg = sig_<float>(a);
+            v *= sg * (1.f + a * (1.f - sg));
+          }
+          dpw[K - 1][j] = v;
+          if (own) {
+            tb[j] += v;
+#pragma unroll
+            for (int k = 0; k < K; ++k) tw[j][k] = fmaf(v, win[k][j], tw[j][k]);
+          }
+        }
+        if (own) {
+          float o[NC];
+          const int hr = t - len;
+          if (np && hr >= 0 && hr < K - 1) {
+            RawN<T, NC> r;
+            load_raw(np + (long long)hr * d.channels, r);
+            unpack_raw(r, o);
+          } else {
+#pragma unroll
+            for (int j = 0; j < NC; ++j) o[j] = 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int k = 0; k < K; ++k) o[j] = fmaf(w[j][k], dpw[K - 1 - k][j], o[j]);
+          if (t >= K - 1) store_n((T*)g.din + ((long long)b * d.seqlen + t - (K - 1)) * d.channels + c0, o);
+          else if (g.dhist) store_n((T*)g.dhist + ((long long)b * (K - 1) + t) * d.channels + c0, o);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      db[j] += tb[j];
+#pragma unroll
+      for (int k = 0; k < K; ++k) dw[j][k] += tw[j][k];
+    }
+  }
+  float* pp = partial + ((size_t)row * d.channels + c0) * (K + 1);
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) pp[j * (K + 1) + k] = dw[j][k];
+    pp[j * (K + 1) + K] = db[j];
+  }
+}
+
+// One token per stream; the history moves up by a row in place.  Thread = (stream, 16 bytes of channels).
+template <typename T, int K>
+__global__ void __launch_bounds__(256) k_conv_step(SsdConvDims d, const T* __restrict__ in, const float* __restrict__ weight,
+                                                   const float* __restrict__ bias, T* __restrict__ history, T* __restrict__ out) {
+  pdl_wait();
+  constexpr int NC = 16 / (int)sizeof(T);
+  const int CV = d.channels / NC;
+  const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (item >= (long long)d.batch * CV) return;
+  const int c0 = (int)(item % CV) * NC;
+  const long long b = item / CV;
+  T* hp = history + b * (K - 1) * d.channels + c0;
+  RawN<T, NC> r[K];
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) r[k] = *reinterpret_cast<const RawN<T, NC>*>(hp + (long long)k * d.channels);
+  load_raw(in + b * d.in_stride_b + c0, r[K - 1]);
+  float o[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) o[j] = bias ? __ldg(bias + c0 + j) : 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    float v[NC];
+    unpack_raw(r[k], v);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) o[j] = fmaf(__ldg(weight + (size_t)(c0 + j) * K + k), v[j], o[j]);
+    if (k > 0) *reinterpret_cast<RawN<T, NC>*>(hp + (long long)(k - 1) * d.channels) = r[k];
+  }
+#pragma unroll
+  for (int j = 0; j < NC; ++j) if (d.activation) o[j] *= sig_<T>(o[j]);
+  store_n(out + b * d.out_stride_b + c0, o);
+}
+int carry_bwd_tiles(const SsdConvDims* d) { return (d->seqlen + d->width - 1 + CARRY_TLB - 1) / CARRY_TLB; }
+int carry_rows(const SsdConvDims* d) {
+  const long long pairs = (long long)d->batch * carry_bwd_tiles(d);
+  return (int)(pairs < CARRY_ROWS ? pairs : CARRY_ROWS);
+}
+
 int conv_rows(const SsdConvDims* d) {   // thread rows of the backward kernel = partial sums to add
   const int ntile = (d->seqlen + CONV_TLB - 1) / CONV_TLB;
   const long long pairs = (long long)d->batch * ntile;
@@ -1120,6 +1370,106 @@ int32_t ssd_conv1d_backward(const SsdConvDims* dims, const void* in, const float
   SSD_CUDA_CHECK_LAUNCH("conv1d_reduce");
   return SSD_OK;
 }
+
+#define CARRY_BY_TYPE(F) do { \
+    if (dims->dtype == SSD_BF16) { if (dims->width == 4) F(__nv_bfloat16, 4); else if (dims->width == 3) F(__nv_bfloat16, 3); else F(__nv_bfloat16, 2); } \
+    else { if (dims->width == 4) F(float, 4); else if (dims->width == 3) F(float, 3); else F(float, 2); } } while (0)
+
+static int check_carry(const char* what, const SsdConvDims* d, std::initializer_list<const void*> required, std::initializer_list<const void*> others) {
+  int rc = check_conv(d);
+  if (rc) return rc;
+  for (const void* p : required) if (!p) { set_error("%s: a required pointer is NULL", what); return SSD_ERR_NULL_POINTER; }
+  for (auto list : {required, others})
+    for (const void* p : list) if (!aligned16(p)) { set_error("%s: pointers must be 16-byte aligned", what); return SSD_ERR_BAD_ALIGNMENT; }
+  if (d->device >= 0) {
+    int cur = -1;
+    if (cudaGetDevice(&cur) != cudaSuccess || cur != d->device) {
+      set_error("%s: current CUDA device is %d but dims.device is %d (the library never switches devices)", what, cur, d->device);
+      return SSD_ERR_CUDA;
+    }
+  }
+  return SSD_OK;
+}
+static bool overlap(const void* a, const void* b, size_t n) {
+  const char *x = (const char*)a, *y = (const char*)b;
+  return x && y && x < y + n && y < x + n;
+}
+
+int32_t ssd_conv1d_carry_forward(const SsdConvDims* dims, const void* in, const float* weight, const float* bias, const void* history,
+                                 const int32_t* lengths, void* out, void* new_history, void* cuda_stream) {
+  clear_error();
+  const int rc = check_carry("conv1d carry", dims, {in, out}, {history, new_history});
+  if (rc) return rc;
+  if (!weight) { set_error("conv1d carry: weight is NULL"); return SSD_ERR_NULL_POINTER; }
+  const int es = dims->dtype == SSD_BF16 ? 2 : 4;
+  if (overlap(history, new_history, (size_t)dims->batch * (dims->width - 1) * dims->channels * es)) {
+    set_error("conv1d carry: history and new_history overlap");
+    return SSD_ERR_BAD_SHAPE;
+  }
+  cudaStream_t s = (cudaStream_t)cuda_stream;
+  const Carry q{history, lengths, (dims->seqlen + CARRY_TL - 1) / CARRY_TL};
+  const long long blocks = ((long long)dims->batch * q.tiles * (dims->channels * es / 16) + CONV_THREADS - 1) / CONV_THREADS;
+  if (blocks > 0x7fffffffLL) { set_error("conv1d carry: too many blocks for one grid (%lld)", blocks); return SSD_ERR_UNSUPPORTED; }
+#define CARRY_RUN(T, K) launch<k_carry_fwd<T, K>>((unsigned)blocks, CONV_THREADS, 0, s, *dims, q, (const T*)in, weight, bias, (T*)out, (T*)new_history)
+  CARRY_BY_TYPE(CARRY_RUN);
+#undef CARRY_RUN
+  SSD_CUDA_CHECK_LAUNCH("conv1d_carry_fwd");
+  return SSD_OK;
+}
+
+size_t ssd_conv1d_carry_workspace_bytes(const SsdConvDims* dims) {
+  clear_error();
+  if (check_conv(dims)) return 0;
+  return (size_t)carry_rows(dims) * dims->channels * (dims->width + 1) * sizeof(float);
+}
+
+int32_t ssd_conv1d_carry_backward(const SsdConvDims* dims, const void* in, const float* weight, const float* bias, const void* history,
+                                  const int32_t* lengths, const void* dout, int64_t dout_stride_b, int64_t dout_stride_l,
+                                  const void* dnew_history, void* din, void* dhistory, float* dweight, float* dbias, void* workspace,
+                                  size_t workspace_bytes, void* cuda_stream) {
+  clear_error();
+  int rc = check_carry("conv1d carry backward", dims, {in, dout, din, workspace}, {history, dnew_history, dhistory});
+  if (rc) return rc;
+  if (!weight || !dweight) { set_error("conv1d carry backward: a required pointer is NULL"); return SSD_ERR_NULL_POINTER; }
+  const int es = dims->dtype == SSD_BF16 ? 2 : 4;
+  if (dout_stride_l < dims->channels || (dout_stride_b * es) % 16 || (dout_stride_l * es) % 16) {
+    set_error("conv1d carry backward: dout rows must cover the channels, strides multiples of 16 bytes");
+    return SSD_ERR_BAD_ALIGNMENT;
+  }
+  const size_t need = (size_t)carry_rows(dims) * dims->channels * (dims->width + 1) * sizeof(float);
+  if (workspace_bytes < need) { set_error("conv1d carry backward: workspace too small: %zu < %zu", workspace_bytes, need); return SSD_ERR_WORKSPACE_TOO_SMALL; }
+  cudaStream_t s = (cudaStream_t)cuda_stream;
+  const Carry q{history, lengths, 0};
+  const CarryBwd g{dout, dnew_history, dout_stride_b, dout_stride_l, din, dhistory, carry_rows(dims), carry_bwd_tiles(dims)};
+  const unsigned grid = (unsigned)(((long long)g.rows * (dims->channels / 4) + CONV_THREADS - 1) / CONV_THREADS);
+#define CARRY_RUN(T, K) launch<k_carry_bwd<T, K>>(grid, CONV_THREADS, 0, s, *dims, q, g, (const T*)in, weight, bias, (float*)workspace)
+  CARRY_BY_TYPE(CARRY_RUN);
+#undef CARRY_RUN
+  SSD_CUDA_CHECK_LAUNCH("conv1d_carry_bwd");
+  const int n = dims->channels * (dims->width + 1);
+  launch<k_conv_reduce>((n + 31) / 32, dim3(32, RED_GROUPS), 0, s, g.rows, dims->channels, dims->width, (const float*)workspace, dweight, dbias);
+  SSD_CUDA_CHECK_LAUNCH("conv1d_carry_reduce");
+  return SSD_OK;
+}
+
+int32_t ssd_conv1d_step(const SsdConvDims* dims, const void* in, const float* weight, const float* bias, void* history, void* out,
+                        void* cuda_stream) {
+  clear_error();
+  if (dims && dims->seqlen != 1) { set_error("conv1d step: seqlen must be 1 (got %d)", dims->seqlen); return SSD_ERR_BAD_SHAPE; }
+  const int rc = check_carry("conv1d step", dims, {in, history, out}, {});
+  if (rc) return rc;
+  if (!weight) { set_error("conv1d step: weight is NULL"); return SSD_ERR_NULL_POINTER; }
+  const int es = dims->dtype == SSD_BF16 ? 2 : 4;
+  cudaStream_t s = (cudaStream_t)cuda_stream;
+  const long long blocks = ((long long)dims->batch * (dims->channels * es / 16) + 255) / 256;
+  if (blocks > 0x7fffffffLL) { set_error("conv1d step: too many blocks for one grid (%lld)", blocks); return SSD_ERR_UNSUPPORTED; }
+#define CARRY_RUN(T, K) launch<k_conv_step<T, K>>((unsigned)blocks, 256, 0, s, *dims, (const T*)in, weight, bias, (T*)history, (T*)out)
+  CARRY_BY_TYPE(CARRY_RUN);
+#undef CARRY_RUN
+  SSD_CUDA_CHECK_LAUNCH("conv1d_step");
+  return SSD_OK;
+}
+#undef CARRY_BY_TYPE
 
 static int check_norm(const SsdNormDims* d) {
   if (!d) { set_error("dims is NULL"); return SSD_ERR_NULL_POINTER; }

@@ -28,6 +28,28 @@ def conv1d_backward(inp, weight, bias, douts: Sequence[torch.Tensor], *, activat
     return L.host().conv1d_backward(inp, weight, bias, activation, *douts)
 
 
+def conv1d_carry_forward(inp, weight, bias=None, history=None, *, lengths=None, activation=True):
+    """out, new_history: conv1d_forward over sequences that go on where another call stopped.  `history` [batch, width-1, channels]
+    holds the rows before the first (oldest first; None = zeros), `new_history` those before the next call's first.  `lengths` (int32
+    [batch] on the device): rows at or past it are not read, their output is zero and they are not in the new history."""
+    return L.host().carry_forward(inp, weight, bias, history, lengths, activation)
+
+
+def conv1d_carry_backward(inp, weight, bias, history, dout, dnew_history=None, *, lengths=None, activation=True):
+    """din, dweight, dbias, dhistory (None without a bias / history) from the gradients of both outputs."""
+    return L.host().carry_backward(inp, weight, bias, history, dout, dnew_history, lengths, activation)
+
+
+def causal_conv1d_carry(inp, weight, bias=None, history=None, *, lengths=None, activation=True):
+    """Differentiable conv1d_carry_forward: returns (out, new_history)."""
+    return L.host().carry(inp, weight, bias, history, lengths, activation)
+
+
+def conv1d_step(history, inp, weight, bias=None, *, activation=True, out=None):
+    """One token per stream, IN PLACE on `history` [streams, width-1, channels]; inp and out [streams, channels]."""
+    return L.host().conv1d_step(history, inp, weight, bias, activation, out)
+
+
 def rmsnorm_forward(inp, weight=None, *, eps=1e-5):
     """RMS norm over the last dim (all earlier dims are rows).  Returns out, rstd."""
     return L.host().rmsnorm_forward(inp, weight, eps)
