@@ -1,8 +1,12 @@
 // A layer's projection with its epilogue:  out = act(x W^T + bias) + residual, and its gradients.
 //
-// k_mm is the general form: any sizes, strides and both storage types, fp32 products and sums on the CUDA cores.
+// k_mm2: bf16 on the tensor cores, pairs of CTAs on tiles of 256 x up to 256.
+// k_mm: the general form, any sizes, strides and both storage types, fp32 products and sums on the CUDA cores.
+#include <type_traits>
+
 #include "common.cuh"
 #include "ssd_internal.h"
+#include "umma.cuh"
 
 namespace ssd {
 namespace {
@@ -79,44 +83,494 @@ __global__ void __launch_bounds__(256) k_mm(MmArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// out[m][n] = epilogue(sum_k P(m,k) Q(n,k)) for bf16 operands that a tensor map can describe.
+//
+// A pair of CTAs computes tiles of 256 x bn: every CTA loads 128 rows of P and bn/2 rows of Q per block of 64 k (32 KB at bn = 256),
+// where a CTA on its own would load 48 KB for the same work per SM: at the tensor cores' rate that is 13 instead of 19 TB/s out
+// of the L2.  Warp 0 of each CTA issues the loads (six stages), warp 1 of the leader the MMAs, eight warps per CTA read the
+// accumulators (two of them in TMEM, so that a tile's epilogue runs beside the next tile's products).  Pairs walk the units
+// (split of k, tile row, tile column) with a fixed stride; with splits > 1 a unit leaves fp32 sums in the workspace and k_mm2_join adds
+// them in order.  Every wait is bounded: when one runs out a code goes to the status word and the outputs become NaN.
+namespace u = umma;
+constexpr int MM_STAGES = 5, MM_BM = 256, MM_EPI = 8, MM_THREADS = 32 * (4 + MM_EPI);
+constexpr int MM_STAGE = 32768;                    // 16 KB of P, 16 KB of Q
+constexpr int MM_SLOT = 4096;                      // output staging of a warp: two boxes of 32 x 32 bf16, or one of fp32
+constexpr int MM_ROWS = 8;                         // tile rows walked side by side: the pairs at work share operands in the L2
+constexpr size_t MM_SMEM = (size_t)MM_STAGES * MM_STAGE + MM_EPI * MM_SLOT + 1024;
+
+struct Mm2 {
+  long long M, N;                                  // of the tiles: rows of P, rows of Q
+  int kb, kper, splits, bn, rt, ct, units;         // blocks of 64 k, per split; tile rows and columns
+  int trans;                                       // the tiles' rows are the output's columns (few tokens: the weights are P)
+  int act, vec;                                    // vec: tensor maps fit out, pre and residual (with splits: the sums)
+  long long os, rs;
+  const __nv_bfloat16 *bias, *residual;
+  __nv_bfloat16 *out, *pre;
+  float* part;                                     // [splits][out rows][out columns]
+  int* status;
+};
+
+// unit -> split, tile row, tile column; columns of a group of MM_ROWS tile rows one after the other
+__device__ __forceinline__ void unit_at(const Mm2& a, int un, int& sp, int& r, int& c) {
+  const int tiles = a.rt * a.ct;
+  sp = un / tiles;
+  const int t = un - sp * tiles, g = t / (MM_ROWS * a.ct), r0 = g * MM_ROWS, n = min(MM_ROWS, a.rt - r0), w = t - g * MM_ROWS * a.ct;
+  c = w / n; r = r0 + w - c * n;
+}
+// One value of the result at output row m and column n.
+__device__ __forceinline__ void finish_one(const Mm2& a, long long cols, long long m, long long n, float v) {
+  if (a.bias) v += __bfloat162float(a.bias[n]);
+  if (a.pre) a.pre[m * cols + n] = __float2bfloat16_rn(v);
+  v = act_of(v, a.act);
+  if (a.residual) v += __bfloat162float(a.residual[m * a.rs + n]);
+  a.out[m * a.os + n] = __float2bfloat16_rn(v);
+}
+
+// Output through shared memory and TMA stores (a thread holds a row: stored from registers, the lanes of a warp write 16 or 32 bytes
+// each at the rows' distance, 2.3 times the tensor cores' time at 16384 x 768 x 3352).
+__device__ __forceinline__ void stage_bf16(uint32_t box, int lane, const float (&v)[32]) {   // 64-byte rows, 64-byte swizzle
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    u::st_shared_v4(box + lane * 64 + ((i ^ (lane >> 1)) & 3) * 16, u::pack_bf16(v[8 * i], v[8 * i + 1]), u::pack_bf16(v[8 * i + 2], v[8 * i + 3]),
+                    u::pack_bf16(v[8 * i + 4], v[8 * i + 5]), u::pack_bf16(v[8 * i + 6], v[8 * i + 7]));
+}
+__device__ __forceinline__ void stage_f32(uint32_t box, int lane, const float (&v)[32]) {    // 128-byte rows, 128-byte swizzle
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    u::st_shared_v4(box + lane * 128 + ((i ^ lane) & 7) * 16, __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                    __float_as_uint(v[4 * i + 3]));
+}
+
+template <bool PMN, bool QMN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MM_THREADS, 1)
+k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tout,
+      const __grid_constant__ CUtensorMap tpre, const __grid_constant__ Mm2 a) {
+  extern __shared__ unsigned char mm_raw[];
+  __shared__ __align__(8) uint64_t full[MM_STAGES], empty[MM_STAGES], tfull[2], tempty[2];
+  __shared__ uint32_t slot;
+  __shared__ int dead;
+  __shared__ __align__(16) float s_bias[2][256];
+  unsigned char* st = mm_raw + (1024 - (u::smem_u32(mm_raw) & 1023)) % 1024;   // the same offset in both CTAs
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = u::cluster_rank();
+  if (tid == 0) {
+    dead = 0;
+    for (int i = 0; i < MM_STAGES; ++i) { u::mbar_init(&full[i], 1); u::mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { u::mbar_init(&tfull[i], 1); u::mbar_init(&tempty[i], 2 * MM_EPI); }
+    u::mbar_fence_init();
+  }
+  if (warp == 2) u::tmem_alloc_pair(&slot, 512);
+  u::tc_fence_before();
+  __syncthreads();
+  u::cluster_sync();
+  u::tc_fence_after();
+  const uint32_t tmem = slot;
+  pdl_wait();
+  if (blockIdx.x == 0 && tid == 0) *a.status = 0;
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  volatile int* is_dead = &dead;
+  auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+    if (*is_dead) return false;
+    if (u::mbar_wait(bar, parity)) return true;
+    *is_dead = 1;
+    *a.status = code;
+    return false;
+  };
+  const int half = a.bn / 2;
+  if (warp == 0) {
+    if (lane == 0) {
+      const int qbox = QMN ? (half + 63) / 64 : 1;
+      const uint32_t bytes = 2u * (16384u + (QMN ? qbox * 8192u : half * 128u));
+      int s = 0;
+      uint32_t ph = 1;
+      bool ok = true;
+      for (int un = pair; un < a.units && ok; un += npairs) {
+        int sp, r, c;
+        unit_at(a, un, sp, r, c);
+        const int k0 = sp * a.kper, k1 = min(k0 + a.kper, a.kb);
+        const int prow = r * MM_BM + (int)rank * 128, qrow = c * a.bn + (int)rank * half;
+        for (int k = k0; k < k1; ++k) {
+          if (!(ok = wait(&empty[s], ph, 201))) break;
+          unsigned char* sa = st + s * MM_STAGE;
+          unsigned char* sb = sa + 16384;
+          if (rank == 0) u::mbar_expect_tx(&full[s], bytes);
+          const uint32_t bar = u::map_rank(&full[s], 0);
+          if (PMN) {
+            u::tma_load_2d_pair(sa, &tp, prow, k * 64, bar);
+            u::tma_load_2d_pair(sa + 8192, &tp, prow + 64, k * 64, bar);
+          } else {
+            u::tma_load_2d_pair(sa, &tp, k * 64, prow, bar);
+          }
+          if (QMN) {
+            for (int j = 0; j < qbox; ++j) u::tma_load_2d_pair(sb + j * 8192, &tq, qrow + j * 64, k * 64, bar);
+          } else {
+            u::tma_load_2d_pair(sb, &tq, k * 64, qrow, bar);
+          }
+          if (++s == MM_STAGES) { s = 0; ph ^= 1; }
+        }
+      }
+      if (!ok) {   // let copies in flight land before the shared memory goes back
+        const long long t0 = clock64();
+        while (clock64() - t0 < 4000000) {}
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      const uint32_t idesc = u::make_idesc(256, a.bn, PMN, QMN);
+      int s = 0, buf = 0;
+      uint32_t ph = 0, tph = 1;
+      bool ok = true;
+      for (int un = pair; un < a.units && ok; un += npairs) {
+        const int sp = un / (a.ct * a.rt);
+        const int k0 = sp * a.kper, k1 = min(k0 + a.kper, a.kb);
+        if (!(ok = wait(&tempty[buf], tph, 202))) break;
+        u::tc_fence_after();
+        for (int k = k0; k < k1; ++k) {
+          if (!(ok = wait(&full[s], ph, 203))) break;
+          u::tc_fence_after();
+          const uint32_t sa = u::smem_u32(st + s * MM_STAGE), sb = sa + 16384;
+          const uint64_t ad = PMN ? u::desc_sw128_mn(sa, 0, 0, 8192) : u::desc_sw128_k(sa, 0);
+          const uint64_t bd = QMN ? u::desc_sw128_mn(sb, 0, 0, 8192) : u::desc_sw128_k(sb, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            u::mma_bf16_pair(tmem + buf * 256, u::desc_adv(ad, i * (PMN ? 2048 : 32)), u::desc_adv(bd, i * (QMN ? 2048 : 32)), idesc, k > k0 || i > 0);
+          u::mma_commit_pair(&empty[s]);
+          if (++s == MM_STAGES) { s = 0; ph ^= 1; }
+        }
+        if (!ok) break;
+        u::mma_commit_pair(&tfull[buf]);
+        buf ^= 1;
+        if (!buf) tph ^= 1;
+      }
+    }
+  } else if (warp >= 4) {
+    const int e = warp - 4, quad = warp & 3, grp = e >> 2;
+    const uint32_t release = u::map_rank(&tempty[0], 0);    // (the second is 8 bytes on)
+    unsigned char* const slot_p = st + MM_STAGES * MM_STAGE + e * MM_SLOT;
+    const uint32_t slot_a = u::smem_u32(slot_p);
+    int buf = 0, box = 0;
+    uint32_t tph = 0;
+    bool ok = true;
+    for (int un = pair; un < a.units; un += npairs) {
+      int sp, r, c;
+      unit_at(a, un, sp, r, c);
+      const int row0 = r * MM_BM + (int)rank * 128 + quad * 32;
+      const long long row = row0 + lane, n0 = (long long)c * a.bn;
+      const int ncol = (int)min((long long)a.bn, a.N - n0);
+      const bool live = row < a.M, direct = !a.trans && a.splits == 1;
+      uint4 q[4];
+      auto ask = [&](int j) {                        // residual of the columns j .. j+31, asked for a chunk ahead
+        const __nv_bfloat16* p = a.residual + row * a.rs + n0 + j;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = live && j + 8 * i < ncol ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+      };
+      const bool res = direct && a.vec && a.residual;
+      if (res) ask(grp * 32);
+      if (direct) {
+        for (int i = tid - 128; i < 256; i += 32 * MM_EPI) s_bias[buf][i] = a.bias && i < ncol ? __bfloat162float(a.bias[n0 + i]) : 0.f;
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * MM_EPI) : "memory");
+      }
+      ok = ok && wait(&tfull[buf], tph, 204);
+      u::tc_fence_after();
+      for (int j = grp * 32; j < ncol; j += 64) {
+        float v[32];
+        u::tmem_ld32(u::tmem_addr(tmem + buf * 256, quad * 32, j), v);
+        const int nv = min(32, ncol - j);
+        if (!ok)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fc00000);
+        if (a.splits > 1) {
+          if (a.vec) {
+            if (lane == 0) u::bulk_wait_read0();
+            __syncwarp();
+            stage_f32(slot_a, lane, v);
+            u::fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < a.M) { u::tma_store_3d(&tout, slot_p, (int)n0 + j, row0, sp); u::bulk_commit(); }
+          } else if (live && a.trans) {
+            float* p = a.part + ((long long)sp * a.N + n0 + j) * a.M + row;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) if (i < nv) p[i * a.M] = v[i];
+          } else if (live) {
+            float* p = a.part + ((long long)sp * a.M + row) * a.N + n0 + j;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) if (i < nv) p[i] = v[i];
+          }
+          continue;
+        }
+        if (a.trans || !a.vec) {
+          if (live)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < nv) { if (a.trans) finish_one(a, a.M, n0 + j + i, row, v[i]); else finish_one(a, a.N, row, n0 + j + i, v[i]); }
+          continue;
+        }
+        const uint4 h[4] = {q[0], q[1], q[2], q[3]};
+        if (res && j + 64 < ncol) ask(j + 64);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 b = *reinterpret_cast<const float4*>(&s_bias[buf][j + 4 * i]);
+          v[4 * i] += b.x; v[4 * i + 1] += b.y; v[4 * i + 2] += b.z; v[4 * i + 3] += b.w;
+        }
+        auto put = [&](const CUtensorMap* map) {     // two boxes in turn: the older store has read its box
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          __syncwarp();
+          stage_bf16(slot_a + box * 2048, lane, v);
+          u::fence_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < a.M) { u::tma_store_3d(map, slot_p + box * 2048, (int)n0 + j, row0, 0); u::bulk_commit(); }
+          box ^= 1;
+        };
+        if (a.pre) put(&tpre);
+        if (a.act == SSD_ACT_SILU) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = act_of(v[i], SSD_ACT_SILU);
+        } else if (a.act == SSD_ACT_SOFTPLUS) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = act_of(v[i], SSD_ACT_SOFTPLUS);
+        } else if (a.act == SSD_ACT_RELU2) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = act_of(v[i], SSD_ACT_RELU2);
+        }
+        if (res) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t w[4] = {h[i].x, h[i].y, h[i].z, h[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = u::unpack_bf16(w[k]);
+              v[8 * i + 2 * k] += f.x; v[8 * i + 2 * k + 1] += f.y;
+            }
+          }
+        }
+        put(&tout);
+      }
+      u::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) u::mbar_arrive_remote(release + buf * 8);
+      buf ^= 1;
+      if (!buf) tph ^= 1;
+    }
+    if (lane == 0) u::bulk_wait0();
+  }
+  __syncwarp();
+  __syncthreads();
+  u::cluster_sync();
+  u::tc_fence_after();
+  if (warp == 2) u::tmem_dealloc_pair(tmem, 512);
+}
+
+// The splits' sums in order, then the epilogue.  Thread = one value; neighbouring threads neighbouring columns.
+__global__ void __launch_bounds__(256) k_mm2_join(Mm2 a, long long rows, long long cols) {
+  pdl_wait();
+  const long long n = rows * cols;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    float v = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) v += a.part[s * n + i];
+    const long long m = i / cols;
+    finish_one(a, cols, m, i - m * cols, v);
+  }
+}
+
 // dpre = dout act'(pre), rounded to the storage type (what the two products read), and the column sums of the unrounded dpre over a
-// part of the rows.  Block = 32 columns x 8 rows at a time; `parts` parts of the rows on the y axis.
-template <typename T>
+// part of the rows (`parts` of them on the y axis).  Thread = V neighbouring columns, block = 32 V columns x 8 rows at a time, four
+// rows of a thread requested together.  V = 16 bytes where all rows start on 16 bytes, else one value.
+template <typename T> __device__ __forceinline__ void values_of(const T& r, float (&v)[1]) { v[0] = (float)r; }
+__device__ __forceinline__ void values_of(const uint4& r, float (&v)[4]) {
+  v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+}
+__device__ __forceinline__ void values_of(const uint4& r, float (&v)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { const float2 f = umma::unpack_bf16(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+}
+template <typename T> __device__ __forceinline__ void put_values(T* p, const float (&v)[1]) { stf(p, v[0]); }
+__device__ __forceinline__ void put_values(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void put_values(__nv_bfloat16* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(umma::pack_bf16(v[0], v[1]), umma::pack_bf16(v[2], v[3]), umma::pack_bf16(v[4], v[5]), umma::pack_bf16(v[6], v[7]));
+}
+template <typename T, int V>
 __global__ void __launch_bounds__(256) k_dpre(long long M, int N, int act, const T* __restrict__ dout, long long dos, const T* __restrict__ pre,
                                               T* __restrict__ dpre, float* __restrict__ partial) {
-  __shared__ float s[8][32];
+  __shared__ float s[8][32 * V];
   pdl_wait();
-  const int n = blockIdx.x * 32 + threadIdx.x;
+  typedef typename std::conditional<V == 1, T, uint4>::type Raw;   // V values as they lie in memory
+  constexpr int R = 4;
+  const int n = (blockIdx.x * 32 + threadIdx.x) * V;
   const long long per = (M + gridDim.y - 1) / gridDim.y, lo = per * blockIdx.y, hi = min(lo + per, M);
-  float a = 0.f;
+  float a[V] = {};
   if (n < N) {
-    float t = 0.f;
-    int c = 0;
-    for (long long m = lo + threadIdx.y; m < hi; m += 8) {
-      float g = ldf(dout + m * dos + n);
-      if (act) g *= dact_of(ldf(pre + m * N + n), act);
-      if (dpre) stf(dpre + m * N + n, g);
-      t += g;
-      if (++c == 16) { a += t; t = 0.f; c = 0; }
+    for (long long m = lo + threadIdx.y; m < hi; m += 8 * R) {
+      Raw g[R], p[R];
+      float t[V] = {};
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (m + 8 * r < hi) {
+          g[r] = *reinterpret_cast<const Raw*>(dout + (m + 8 * r) * dos + n);
+          if (act) p[r] = *reinterpret_cast<const Raw*>(pre + (m + 8 * r) * N + n);
+        }
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (m + 8 * r < hi) {
+          float x[V], q[V];
+          values_of(g[r], x);
+          if (act) {
+            values_of(p[r], q);
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] *= dact_of(q[j], act);
+          }
+#pragma unroll
+          for (int j = 0; j < V; ++j) t[j] += x[j];
+          if (dpre) put_values(dpre + (m + 8 * r) * N + n, x);
+        }
+#pragma unroll
+      for (int j = 0; j < V; ++j) a[j] += t[j];
     }
-    a += t;
   }
   if (!partial) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[threadIdx.y][threadIdx.x * V + j] = a[j];
+  __syncthreads();
+  for (int i = threadIdx.y * 32 + threadIdx.x; i < 32 * V; i += 256) {
+    const int col = blockIdx.x * 32 * V + i;
+    if (col >= N) break;
+    float b = s[0][i];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) b += s[k][i];
+    partial[(long long)blockIdx.y * N + col] = b;
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(1024) k_dbias(int N, int parts, const float* __restrict__ partial, T* __restrict__ dbias) {
+  __shared__ float s[32][33];
+  pdl_wait();
+  const int n = blockIdx.x * 32 + threadIdx.x;
+  float a = 0.f;
+  if (n < N)
+    for (int p = threadIdx.y; p < parts; p += 32) a += partial[(long long)p * N + n];
   s[threadIdx.y][threadIdx.x] = a;
   __syncthreads();
   if (threadIdx.y || n >= N) return;
 #pragma unroll
-  for (int k = 1; k < 8; ++k) a += s[k][threadIdx.x];
-  partial[(long long)blockIdx.y * N + n] = a;
-}
-template <typename T>
-__global__ void __launch_bounds__(256) k_dbias(int N, int parts, const float* __restrict__ partial, T* __restrict__ dbias) {
-  pdl_wait();
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
-  float a = 0.f;
-  for (int p = 0; p < parts; ++p) a += partial[(long long)p * N + n];
+  for (int k = 1; k < 32; ++k) a += s[k][threadIdx.x];
   stf(dbias + n, a);
+}
+
+// ---- tensor-core products: shape of the tiles and the launch ------------------------------------------------------------
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn get_encode() {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess
+               ? (EncodeFn)p : nullptr;
+  }();
+  return fn;
+}
+// [rows, cols] bf16, rows `stride` elements apart; box = 64 columns x `box` rows, 128-byte swizzle
+int make_map2(CUtensorMap* m, const void* p, long long rows, long long cols, long long stride, int box, const char* what) {
+  EncodeFn enc = get_encode();
+  if (!enc) { set_error("cuTensorMapEncodeTiled is not available from the driver"); return SSD_ERR_CUDA; }
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * 2};
+  const cuuint32_t b[2] = {64, (cuuint32_t)box}, es[2] = {1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dims, strides, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled(%s) failed with CUresult %d", what, (int)r); return SSD_ERR_CUDA; }
+  return SSD_OK;
+}
+// output boxes of 32 x 32: [rows, cols] bf16, or the splits' sums [splits, rows, cols] fp32
+int make_out_map(CUtensorMap* m, const void* p, bool f32, long long splits, long long rows, long long cols, long long stride, const char* what) {
+  EncodeFn enc = get_encode();
+  if (!enc) { set_error("cuTensorMapEncodeTiled is not available from the driver"); return SSD_ERR_CUDA; }
+  const int es = f32 ? 4 : 2;
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)splits};
+  const cuuint64_t strides[2] = {(cuuint64_t)stride * es, (cuuint64_t)stride * rows * es};
+  const cuuint32_t b[3] = {32, 32, 1}, one[3] = {1, 1, 1};
+  const CUresult r = enc(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, b, one,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled(%s, output) failed with CUresult %d", what, (int)r); return SSD_ERR_CUDA; }
+  return SSD_OK;
+}
+bool map_fits(const void* p, long long rows, long long stride) {
+  return ((uintptr_t)p & 15) == 0 && stride % 8 == 0 && rows <= 0x7fffffffLL && stride < (1LL << 38);
+}
+
+// Shape of the tiles for an M x N product over K, estimated in SM clocks: a pair's block of 64 k takes 2 bn on the tensor cores and
+// 256 + bn for its loads; 2500 to fill the pipeline and empty the last accumulator; split sums are written and read at DRAM speed and
+// cost a launch.  With `may_trans` the weights may be the tiles' rows (few tokens).
+struct TileShape { int trans, bn, splits, kper; long long rt, ct; double cost; };
+TileShape find_tiles(long long M, long long N, long long K, bool may_trans) {
+  const int pairs = 74, kb = (int)((K + 63) / 64);
+  TileShape best{0, 0, 0, 0, 0, 0, 1e30};
+  for (int trans = 0; trans <= (may_trans && M <= 128 ? 1 : 0); ++trans) {   // (beyond that its stores, a value at a time, show)
+    const long long R = trans ? N : M, C = trans ? M : N;
+    const long long rt = (R + MM_BM - 1) / MM_BM;
+    for (int bn = 32; bn <= 256; bn += 32) {     // what an MMA of a pair takes
+      if (bn > 32 && bn - 32 >= C) break;
+      const long long ct = (C + bn - 1) / bn;
+      const double tk = 2.0 * bn > 256 + bn ? 2.0 * bn : 256 + bn;
+      for (int s = 1; s <= 32 && s <= kb; ++s) {
+        const int kper = (kb + s - 1) / s;
+        if ((kb + kper - 1) / kper != s) continue;
+        const double units = (double)rt * ct * s, waves = (double)(long long)((units + pairs - 1) / pairs);
+        const double cost = waves * (kper * tk + 200.0) + 2500.0 + (s > 1 ? 4000.0 + 8.0 * s * M * N / 3400.0 : 0.0);
+        if (cost < best.cost) best = TileShape{trans, bn, s, kper, rt, ct, cost};
+      }
+    }
+  }
+  return best;
+}
+// The same for a size that this thread met before (the search takes some microseconds on the host).
+TileShape choose_tiles(long long M, long long N, long long K, bool may_trans) {
+  struct Entry { long long M, N, K; bool may_trans; TileShape t; };
+  static thread_local Entry memo[64] = {};
+  Entry& e = memo[(size_t)(M * 31 + N * 7 + K * 3 + may_trans) % 64];
+  if (e.M != M || e.N != N || e.K != K || e.may_trans != may_trans) e = Entry{M, N, K, may_trans, find_tiles(M, N, K, may_trans)};
+  return e.t;
+}
+size_t part_bytes(const TileShape& t, long long M, long long N) { return t.splits > 1 ? (size_t)t.splits * M * N * sizeof(float) : 0; }
+
+// out [M,N] of P (rows M) and Q (rows N): pointer, whether its k runs along memory, and the stride of its memory rows.
+struct Operand { const void* p; bool kmajor; long long stride; };
+struct Result { __nv_bfloat16 *out, *pre; const __nv_bfloat16 *bias, *residual; long long os, rs; int act; };
+int run_mm2(const char* what, const TileShape& t, Operand P, Operand Q, long long M, long long N, long long K, const Result& o, float* part,
+            int* status, cudaStream_t s) {
+  Mm2 a;
+  if (t.trans) { const Operand x = P; P = Q; Q = x; }
+  a.M = t.trans ? N : M; a.N = t.trans ? M : N;
+  a.kb = (int)((K + 63) / 64); a.kper = t.kper; a.splits = t.splits; a.bn = t.bn; a.rt = (int)t.rt; a.ct = (int)t.ct;
+  a.units = (int)(t.rt * t.ct * t.splits); a.trans = t.trans; a.act = o.act;
+  a.os = o.os; a.rs = o.rs; a.bias = o.bias; a.residual = o.residual; a.out = o.out; a.pre = o.pre; a.part = part; a.status = status;
+  if (t.splits > 1) a.vec = !t.trans && N % 4 == 0 && N < (1LL << 36) / M;
+  else a.vec = !t.trans && N % 8 == 0 && (((uintptr_t)o.out | (uintptr_t)o.pre | (uintptr_t)o.residual) & 15) == 0 && o.os % 8 == 0 &&
+               (!o.residual || o.rs % 8 == 0) && o.os < (1LL << 36) / M;
+  CUtensorMap tp, tq, tout, tpre;
+  int rc = P.kmajor ? make_map2(&tp, P.p, a.M, K, P.stride, 128, what) : make_map2(&tp, P.p, K, a.M, P.stride, 64, what);
+  if (rc) return rc;
+  rc = Q.kmajor ? make_map2(&tq, Q.p, a.N, K, Q.stride, t.bn / 2, what) : make_map2(&tq, Q.p, K, a.N, Q.stride, 64, what);
+  if (rc) return rc;
+  tout = tpre = tp;
+  if (a.vec) {
+    rc = t.splits > 1 ? make_out_map(&tout, part, true, t.splits, M, N, N, what) : make_out_map(&tout, o.out, false, 1, M, N, o.os, what);
+    if (!rc && t.splits == 1 && o.pre) rc = make_out_map(&tpre, o.pre, false, 1, M, N, N, what);
+    if (rc) return rc;
+  }
+  const int pairs = a.units < 74 ? a.units : 74;
+#define MM2_RUN(A, B) launch<k_mm2<A, B>>(2 * pairs, MM_THREADS, MM_SMEM, s, tp, tq, tout, tpre, a)
+  if (P.kmajor) { if (Q.kmajor) MM2_RUN(false, false); else MM2_RUN(false, true); }
+  else { if (Q.kmajor) MM2_RUN(true, false); else MM2_RUN(true, true); }
+#undef MM2_RUN
+  SSD_CUDA_CHECK_LAUNCH(what);
+  if (t.splits > 1) {
+    const long long n = (M * N + 255) / 256, most = (long long)sm_count() * 8;
+    launch<k_mm2_join>((unsigned)(n < most ? n : most), 256, 0, s, a, M, N);
+    SSD_CUDA_CHECK_LAUNCH("linear_join");
+  }
+  return SSD_OK;
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
@@ -124,9 +578,11 @@ size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 struct LinPlan {
   long long M, xs, os, rs;
   int K, N, act, es, parts;
-  size_t dpre, partial, fwd_bytes, bwd_bytes;
+  bool tc;                                          // bf16: products on the tensor cores where the operands' rows allow it
+  TileShape fwd, tdx, tdw;
+  size_t part_fwd, dpre, partial, part_bwd, fwd_bytes, bwd_bytes;   // a status word comes first in both workspaces
 };
-int make_lin_plan(const SsdLinearDims* d, LinPlan* o) {
+int make_lin_plan(const SsdLinearDims* d, int pass, LinPlan* o) {
   if (!d) { set_error("linear: dims is NULL"); return SSD_ERR_NULL_POINTER; }
   if (d->rows <= 0 || d->in_features <= 0 || d->out_features <= 0) {
     set_error("linear: rows, in_features and out_features must be positive (got %lld %d %d)", (long long)d->rows, d->in_features, d->out_features);
@@ -139,14 +595,29 @@ int make_lin_plan(const SsdLinearDims* d, LinPlan* o) {
   o->os = d->out_stride_row ? d->out_stride_row : o->N;
   o->rs = d->residual_stride_row ? d->residual_stride_row : o->N;
   if (o->xs < o->K || o->os < o->N || o->rs < o->N) { set_error("linear: row strides must be at least the row size"); return SSD_ERR_BAD_SHAPE; }
-  if (((o->M + 63) / 64) * ((o->N + 63) / 64) > 0x7fffffffLL) { set_error("linear: too many output tiles for one grid"); return SSD_ERR_UNSUPPORTED; }
-  const long long cols = (o->N + 31) / 32, want = (4 * 148 + cols - 1) / cols, most = (o->M + 63) / 64;
+  if (((o->M + 63) / 64) * (((o->N > o->K ? o->N : o->K) + 63LL) / 64) > 0x7fffffffLL) { set_error("linear: too many output tiles for one grid"); return SSD_ERR_UNSUPPORTED; }
+  const long long cols = (o->N + 255) / 256, want = (8 * 148 + cols - 1) / cols, most = (o->M + 63) / 64;
   o->parts = (int)(want < most ? want : most);
   size_t at = 0;
   auto take = [&](size_t n) { const size_t r = at; at += up256(n); return r; };
-  o->fwd_bytes = 256;
+  take(256);
+  o->tc = d->dtype == SSD_BF16 && o->M <= 0x7fffff00LL;
+  size_t join = 0;
+  if (o->tc) {
+    if (pass == SSD_PASS_FWD) {
+      o->fwd = choose_tiles(o->M, o->N, o->K, true);
+    } else {
+      o->tdx = choose_tiles(o->M, o->K, o->N, true);
+      o->tdw = choose_tiles(o->N, o->K, o->M, false);
+      const size_t x = part_bytes(o->tdx, o->M, o->K), w = part_bytes(o->tdw, o->N, o->K);
+      join = x > w ? x : w;
+    }
+  }
+  o->part_fwd = at;
+  o->fwd_bytes = at + (o->tc && pass == SSD_PASS_FWD ? up256(part_bytes(o->fwd, o->M, o->N)) : 0) + 256;
   o->dpre = take(o->act ? (size_t)o->M * o->N * o->es : 0);
   o->partial = take((size_t)o->parts * o->N * sizeof(float));
+  o->part_bwd = take(join);
   o->bwd_bytes = at + 256;
   return SSD_OK;
 }
@@ -177,15 +648,30 @@ int linear_backward(const LinPlan& p, const void* x, const void* w, const void* 
   if (need_dpre || db) {
     T* dpre = need_dpre ? (T*)(ws + p.dpre) : nullptr;
     float* partial = db ? (float*)(ws + p.partial) : nullptr;
-    launch<k_dpre<T>>(dim3((p.N + 31) / 32, p.parts), dim3(32, 8), 0, s, p.M, p.N, p.act, (const T*)dout, dos, (const T*)pre, dpre, partial);
+    constexpr int V = 16 / (int)sizeof(T);
+    if (p.N % V == 0 && dos % V == 0 && (((uintptr_t)dout | (p.act ? (uintptr_t)pre : 0)) & 15) == 0)
+      launch<k_dpre<T, V>>(dim3((p.N + 32 * V - 1) / (32 * V), p.parts), dim3(32, 8), 0, s, p.M, p.N, p.act, (const T*)dout, dos, (const T*)pre, dpre, partial);
+    else
+      launch<k_dpre<T, 1>>(dim3((p.N + 31) / 32, p.parts), dim3(32, 8), 0, s, p.M, p.N, p.act, (const T*)dout, dos, (const T*)pre, dpre, partial);
     SSD_CUDA_CHECK_LAUNCH("linear_dpre");
     if (db) {
-      launch<k_dbias<T>>((p.N + 255) / 256, 256, 0, s, p.N, p.parts, (const float*)partial, (T*)db);
+      launch<k_dbias<T>>((p.N + 31) / 32, dim3(32, 32), 0, s, p.N, p.parts, (const float*)partial, (T*)db);
       SSD_CUDA_CHECK_LAUNCH("linear_dbias");
     }
     if (need_dpre) { g = dpre; gs = p.N; }
   }
   int rc = SSD_OK;
+  if (std::is_same<T, __nv_bfloat16>::value && p.tc && map_fits(g, p.M, gs) && map_fits(w, p.N, p.K)) {
+    typedef __nv_bfloat16 bf;
+    int* status = (int*)ws;
+    float* part = (float*)(ws + p.part_bwd);
+    if (dx && (rc = run_mm2("linear_dx", p.tdx, {g, true, gs}, {w, false, p.K}, p.M, p.K, p.N, {(bf*)dx, nullptr, nullptr, nullptr, p.K, 0, 0}, part, status, s)))
+      return rc;
+    if (!dw) return rc;
+    if (map_fits(x, p.M, p.xs))
+      return run_mm2("linear_dw", p.tdw, {g, false, gs}, {x, false, p.xs}, p.N, p.K, p.M, {(bf*)dw, nullptr, nullptr, nullptr, p.K, 0, 0}, part, status, s);
+    dx = nullptr;
+  }
   if (dx && (rc = run_mm<T>("linear_dx", MmArgs{g, w, nullptr, nullptr, dx, nullptr, p.M, p.K, p.N, gs, 1, 1, p.K, p.K, 0, 0}, s))) return rc;
   if (dw && (rc = run_mm<T>("linear_dw", MmArgs{g, x, nullptr, nullptr, dw, nullptr, p.N, p.K, p.M, 1, gs, 1, p.xs, p.K, 0, 0}, s))) return rc;
   return rc;
@@ -201,7 +687,7 @@ extern "C" {
 size_t ssd_linear_workspace_bytes(const SsdLinearDims* dims, int32_t pass) {
   clear_error();
   LinPlan p;
-  if (make_lin_plan(dims, &p)) return 0;
+  if (make_lin_plan(dims, pass, &p)) return 0;
   return pass == SSD_PASS_BWD ? p.bwd_bytes : p.fwd_bytes;
 }
 
@@ -209,11 +695,17 @@ int32_t ssd_linear_forward(const SsdLinearDims* dims, const void* x, const void*
                            void* pre, void* workspace, size_t workspace_bytes, void* cuda_stream) {
   clear_error();
   LinPlan p;
-  int rc = make_lin_plan(dims, &p);
+  int rc = make_lin_plan(dims, SSD_PASS_FWD, &p);
   if (rc || (rc = check_device(dims))) return rc;
   if (!x || !weight || !out || !workspace) { set_error("linear: x, weight, out and workspace must be non-NULL"); return SSD_ERR_NULL_POINTER; }
   if (workspace_bytes < p.fwd_bytes) { set_error("linear: workspace too small: %zu < %zu", workspace_bytes, p.fwd_bytes); return SSD_ERR_WORKSPACE_TOO_SMALL; }
   cudaStream_t s = (cudaStream_t)cuda_stream;
+  if (p.tc && map_fits(x, p.M, p.xs) && map_fits(weight, p.N, p.K)) {
+    char* ws = aligned_base(workspace);
+    typedef __nv_bfloat16 bf;
+    return run_mm2("linear_fwd", p.fwd, {x, true, p.xs}, {weight, true, p.K}, p.M, p.N, p.K,
+                   {(bf*)out, (bf*)pre, (const bf*)bias, (const bf*)residual, p.os, p.rs, p.act}, (float*)(ws + p.part_fwd), (int*)ws, s);
+  }
   const MmArgs a{x, weight, bias, residual, out, pre, p.M, p.N, p.K, p.xs, 1, p.K, 1, p.os, p.rs, p.act};
   return dims->dtype == SSD_BF16 ? run_mm<__nv_bfloat16>("linear_fwd", a, s) : run_mm<float>("linear_fwd", a, s);
 }
@@ -223,7 +715,7 @@ int32_t ssd_linear_backward(const SsdLinearDims* dims, const void* x, const void
                             void* cuda_stream) {
   clear_error();
   LinPlan p;
-  int rc = make_lin_plan(dims, &p);
+  int rc = make_lin_plan(dims, SSD_PASS_BWD, &p);
   if (rc || (rc = check_device(dims))) return rc;
   if (!x || !weight || !dout || !workspace) { set_error("linear backward: x, weight, dout and workspace must be non-NULL"); return SSD_ERR_NULL_POINTER; }
   if (p.act && !pre) { set_error("linear backward: an activation needs the forward's pre"); return SSD_ERR_NULL_POINTER; }
