@@ -24,62 +24,160 @@ __device__ __forceinline__ float dact_of(float v, int act) {
   return 1.f;
 }
 
+// Values of a 16-byte piece (or a single one) as it lies in memory.
+template <typename T> __device__ __forceinline__ void values_of(const T& r, float (&v)[1]) { v[0] = (float)r; }
+__device__ __forceinline__ void values_of(const uint4& r, float (&v)[4]) {
+  v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+}
+__device__ __forceinline__ void values_of(const uint4& r, float (&v)[8]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { const float2 f = umma::unpack_bf16(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+}
+template <typename T> __device__ __forceinline__ void put_values(T* p, const float (&v)[1]) { stf(p, v[0]); }
+__device__ __forceinline__ void put_values(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void put_values(__nv_bfloat16* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(umma::pack_bf16(v[0], v[1]), umma::pack_bf16(v[2], v[3]), umma::pack_bf16(v[4], v[5]), umma::pack_bf16(v[6], v[7]));
+}
+
 // out[m][n] = epilogue(sum_k P(m,k) Q(n,k)); element strides of P and Q along both dims.
 struct MmArgs {
   const void *P, *Q, *bias, *residual;
   void *out, *pre;
   long long M, N, K, psm, psk, qsn, qsk, os, rs;
-  int act;
+  int act, splits;
+  long long kper;
+  float* part;                                      // splits > 1: [splits][M][N] sums, finished by k_join
 };
+template <typename T> __device__ __forceinline__ void finish(const MmArgs& a, long long m, long long n, float v) {
+  if (a.bias) v += ldf((const T*)a.bias + n);
+  if (a.pre) stf((T*)a.pre + m * a.N + n, v);
+  v = act_of(v, a.act);
+  if (a.residual) v += ldf((const T*)a.residual + m * a.rs + n);
+  stf((T*)a.out + m * a.os + n, v);
+}
 
-template <typename T>
+// Block = 16 TM x 16 TM outputs, thread = TM x TM of them as packed pairs; 32 k at a time through shared memory, the next 32 in
+// registers meanwhile.  Eight k by four rows per warp and request where k runs along memory: whole sectors, and no two lanes of a
+// store on one bank.
+template <typename T, int TM>
 __global__ void __launch_bounds__(256) k_mm(MmArgs a) {
-  constexpr int BM = 64, BN = 64, BK = 16;
-  __shared__ float sp[BK][BM + 1], sq[BK][BN + 1];
+  constexpr int BM = 16 * TM, BK = 32, LD = BM + 4, IT = BM * BK / 256;
+  __shared__ __align__(16) float sp[BK][LD], sq[BK][LD];
   pdl_wait();
-  const int tid = threadIdx.x;
-  const long long nn = (a.N + BN - 1) / BN, m0 = (long long)(blockIdx.x / nn) * BM, n0 = (long long)(blockIdx.x % nn) * BN;
-  const int tm = tid / 16, tn = tid % 16;
+  const int tid = threadIdx.x, tm = tid / 16, tn = tid % 16;
+  const long long nn = (a.N + BM - 1) / BM, nm = (a.M + BM - 1) / BM;
+  const long long tile = blockIdx.x % (nn * nm), sp_i = blockIdx.x / (nn * nm);
+  const long long m0 = tile / nn * BM, n0 = tile % nn * BM, kb = sp_i * a.kper, ke = min(kb + a.kper, a.K);
   const T *P = (const T*)a.P, *Q = (const T*)a.Q;
-  float acc[4][4] = {};
-  const bool pk = a.psk == 1, qk = a.qsk == 1;      // which index runs along memory: neighbouring threads follow it
-  for (long long k0 = 0; k0 < a.K; k0 += BK) {
+  auto where = [&](bool along_k, int i, int& k, int& r) {
+    const int e = tid + i * 256;
+    if (along_k) { const int w = e >> 5, l = e & 31; k = (w & 3) * 8 + (l & 7); r = (w >> 2) * 4 + (l >> 3); }
+    else { k = e / BM; r = e % BM; }
+  };
+  const bool pk = a.psk == 1, qk = a.qsk == 1;
+  float rp[IT], rq[IT];
+  auto request = [&](long long k0) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      int k, r;
+      where(pk, i, k, r);
+      rp[i] = m0 + r < a.M && k0 + k < ke ? ldf(P + (m0 + r) * a.psm + (k0 + k) * a.psk) : 0.f;
+      where(qk, i, k, r);
+      rq[i] = n0 + r < a.N && k0 + k < ke ? ldf(Q + (n0 + r) * a.qsn + (k0 + k) * a.qsk) : 0.f;
+    }
+  };
+  f32x2 acc[TM][TM / 2] = {};
+  request(kb);
+  for (long long k0 = kb; k0 < ke; k0 += BK) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < BM * BK / 256; ++i) {
-      const int e = tid + i * 256;
-      const int k = pk ? e % BK : e / BM, m = pk ? e / BK : e % BM;
-      sp[k][m] = m0 + m < a.M && k0 + k < a.K ? ldf(P + (m0 + m) * a.psm + (k0 + k) * a.psk) : 0.f;
-      const int kq = qk ? e % BK : e / BN, n = qk ? e / BK : e % BN;
-      sq[kq][n] = n0 + n < a.N && k0 + kq < a.K ? ldf(Q + (n0 + n) * a.qsn + (k0 + kq) * a.qsk) : 0.f;
+    for (int i = 0; i < IT; ++i) {
+      int k, r;
+      where(pk, i, k, r); sp[k][r] = rp[i];
+      where(qk, i, k, r); sq[k][r] = rq[i];
     }
     __syncthreads();
-#pragma unroll
+    if (k0 + BK < ke) request(k0 + BK);
+#pragma unroll 8
     for (int k = 0; k < BK; ++k) {
-      float x[4], y[4];
+      float x[TM];
+      f32x2 y[TM / 2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { x[i] = sp[k][tm + 16 * i]; y[i] = sq[k][tn + 16 * i]; }
+      for (int h = 0; h < TM / 4; ++h) {
+        const float4 v = *reinterpret_cast<const float4*>(&sp[k][h * 64 + tm * 4]), w = *reinterpret_cast<const float4*>(&sq[k][h * 64 + tn * 4]);
+        x[4 * h] = v.x; x[4 * h + 1] = v.y; x[4 * h + 2] = v.z; x[4 * h + 3] = v.w;
+        y[2 * h] = pack2(w.x, w.y); y[2 * h + 1] = pack2(w.z, w.w);
+      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < TM; ++i) {
+        const f32x2 xx = pack2(x[i], x[i]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+        for (int j = 0; j < TM / 2; ++j) acc[i][j] = fma2(xx, y[j], acc[i][j]);
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long m = m0 + tm + 16 * i;
+  for (int i = 0; i < TM; ++i) {
+    const long long m = m0 + (i / 4) * 64 + tm * 4 + i % 4;
     if (m >= a.M) continue;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const long long n = n0 + tn + 16 * j;
+    for (int j = 0; j < TM; ++j) {
+      const long long n = n0 + (j / 4) * 64 + tn * 4 + j % 4;
       if (n >= a.N) continue;
-      float v = acc[i][j];
-      if (a.bias) v += ldf((const T*)a.bias + n);
-      if (a.pre) stf((T*)a.pre + m * a.N + n, v);
-      v = act_of(v, a.act);
-      if (a.residual) v += ldf((const T*)a.residual + m * a.rs + n);
-      stf((T*)a.out + m * a.os + n, v);
+      float lo, hi;
+      unpack2(acc[i][j / 2], lo, hi);
+      const float v = j % 2 ? hi : lo;
+      if (a.splits > 1) a.part[(sp_i * a.M + m) * a.N + n] = v;
+      else finish<T>(a, m, n, v);
     }
+  }
+}
+// The splits' sums in order, then the epilogue.  Thread = one value; neighbouring threads neighbouring columns.
+template <typename T>
+__global__ void __launch_bounds__(256) k_join(MmArgs a) {
+  pdl_wait();
+  const long long n = a.M * a.N;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    float v = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) v += a.part[s * n + i];
+    const long long m = i / a.N;
+    finish<T>(a, m, i - m * a.N, v);
+  }
+}
+
+// Few rows (up to eight tokens): bound by one reading of the weights and, below some megabytes, by latency, so one launch and every
+// load of a weight row in flight at once.  Warp = F output features and all tokens, lane = 16 bytes of k at a time; x comes out of
+// the L1, F features share a reading of it.
+template <typename T, int RM, int F>
+__global__ void __launch_bounds__(256) k_mm_few(MmArgs a) {
+  constexpr int V = 16 / (int)sizeof(T);
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long n0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * F;
+  if (n0 >= a.N) return;
+  const T *P = (const T*)a.P, *Q = (const T*)a.Q;
+  float acc[F][RM] = {};
+#pragma unroll (RM * F > 8 ? 2 : 4)
+  for (long long k = lane * V; k < a.K; k += 32 * V) {
+    float w[F][V], x[V];
+#pragma unroll
+    for (int f = 0; f < F; ++f) values_of(__ldg(reinterpret_cast<const uint4*>(Q + min(n0 + f, a.N - 1) * a.qsn + k)), w[f]);
+#pragma unroll
+    for (int m = 0; m < RM; ++m) {
+      values_of(__ldg(reinterpret_cast<const uint4*>(P + min((long long)m, a.M - 1) * a.psm + k)), x);
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[f][m] = fmaf(x[v], w[f][v], acc[f][m]);
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    int m;
+    const float v = fold_rows<32, RM>(acc[f], lane, m);
+    if ((lane & (32 / RM - 1)) == 0 && m < a.M && n0 + f < a.N) finish<T>(a, m, n0 + f, v);
   }
 }
 
@@ -377,20 +475,6 @@ __global__ void __launch_bounds__(256) k_mm2_join(Mm2 a, long long rows, long lo
 // dpre = dout act'(pre), rounded to the storage type (what the two products read), and the column sums of the unrounded dpre over a
 // part of the rows (`parts` of them on the y axis).  Thread = V neighbouring columns, block = 32 V columns x 8 rows at a time, four
 // rows of a thread requested together.  V = 16 bytes where all rows start on 16 bytes, else one value.
-template <typename T> __device__ __forceinline__ void values_of(const T& r, float (&v)[1]) { v[0] = (float)r; }
-__device__ __forceinline__ void values_of(const uint4& r, float (&v)[4]) {
-  v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
-}
-__device__ __forceinline__ void values_of(const uint4& r, float (&v)[8]) {
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { const float2 f = umma::unpack_bf16(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
-}
-template <typename T> __device__ __forceinline__ void put_values(T* p, const float (&v)[1]) { stf(p, v[0]); }
-__device__ __forceinline__ void put_values(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-__device__ __forceinline__ void put_values(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(umma::pack_bf16(v[0], v[1]), umma::pack_bf16(v[2], v[3]), umma::pack_bf16(v[4], v[5]), umma::pack_bf16(v[6], v[7]));
-}
 template <typename T, int V>
 __global__ void __launch_bounds__(256) k_dpre(long long M, int N, int act, const T* __restrict__ dout, long long dos, const T* __restrict__ pre,
                                               T* __restrict__ dpre, float* __restrict__ partial) {
@@ -573,6 +657,24 @@ int run_mm2(const char* what, const TileShape& t, Operand P, Operand Q, long lon
   return SSD_OK;
 }
 
+// ---- CUDA-core products: tiles of 128 where they fill the SMs, else of 64, and splits of K (64 at least) where those do not either
+struct CoreShape { bool big; long long tiles, kper; int splits; };
+CoreShape core_shape(long long M, long long N, long long K) {
+  CoreShape c;
+  const long long big = ((M + 127) / 128) * ((N + 127) / 128);
+  c.big = big >= 148;
+  c.tiles = c.big ? big : ((M + 63) / 64) * ((N + 63) / 64);
+  const long long want = c.tiles < 148 ? (2 * 148 + c.tiles - 1) / c.tiles : 1, most = (K + 63) / 64;
+  const long long s = want < most ? want : most;
+  c.kper = ((K + s - 1) / s + 31) / 32 * 32;
+  c.splits = (int)((K + c.kper - 1) / c.kper);
+  return c;
+}
+size_t core_bytes(long long M, long long N, long long K) {
+  const CoreShape c = core_shape(M, N, K);
+  return c.splits > 1 ? (size_t)c.splits * M * N * sizeof(float) : 0;
+}
+
 // ---- host --------------------------------------------------------------------------------------------------------------
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 struct LinPlan {
@@ -601,20 +703,25 @@ int make_lin_plan(const SsdLinearDims* d, int pass, LinPlan* o) {
   size_t at = 0;
   auto take = [&](size_t n) { const size_t r = at; at += up256(n); return r; };
   take(256);
+  // split sums: the largest that any kernel of the pass may leave (operands decide on the kernel, the workspace is sized before)
   o->tc = d->dtype == SSD_BF16 && o->M <= 0x7fffff00LL;
   size_t join = 0;
-  if (o->tc) {
-    if (pass == SSD_PASS_FWD) {
-      o->fwd = choose_tiles(o->M, o->N, o->K, true);
-    } else {
+  auto keep = [&](size_t v) { if (v > join) join = v; };
+  if (pass == SSD_PASS_FWD) {
+    keep(core_bytes(o->M, o->N, o->K));
+    if (o->tc) { o->fwd = choose_tiles(o->M, o->N, o->K, true); keep(part_bytes(o->fwd, o->M, o->N)); }
+  } else {
+    keep(core_bytes(o->M, o->K, o->N));
+    keep(core_bytes(o->N, o->K, o->M));
+    if (o->tc) {
       o->tdx = choose_tiles(o->M, o->K, o->N, true);
       o->tdw = choose_tiles(o->N, o->K, o->M, false);
-      const size_t x = part_bytes(o->tdx, o->M, o->K), w = part_bytes(o->tdw, o->N, o->K);
-      join = x > w ? x : w;
+      keep(part_bytes(o->tdx, o->M, o->K));
+      keep(part_bytes(o->tdw, o->N, o->K));
     }
   }
   o->part_fwd = at;
-  o->fwd_bytes = at + (o->tc && pass == SSD_PASS_FWD ? up256(part_bytes(o->fwd, o->M, o->N)) : 0) + 256;
+  o->fwd_bytes = at + up256(join) + 256;
   o->dpre = take(o->act ? (size_t)o->M * o->N * o->es : 0);
   o->partial = take((size_t)o->parts * o->N * sizeof(float));
   o->part_bwd = take(join);
@@ -633,9 +740,28 @@ int check_device(const SsdLinearDims* d) {
 char* aligned_base(void* ws) { return (char*)(((uintptr_t)ws + 255) & ~(uintptr_t)255); }
 
 template <typename T> int run_mm(const char* what, const MmArgs& a, cudaStream_t s) {
-  const long long blocks = ((a.M + 63) / 64) * ((a.N + 63) / 64);
-  launch<k_mm<T>>((unsigned)blocks, 256, 0, s, a);
+  const CoreShape c = core_shape(a.M, a.N, a.K);
+  MmArgs b = a;
+  b.splits = c.splits; b.kper = c.kper;
+  if (c.big) launch<k_mm<T, 8>>((unsigned)(c.tiles * c.splits), 256, 0, s, b);
+  else launch<k_mm<T, 4>>((unsigned)(c.tiles * c.splits), 256, 0, s, b);
   SSD_CUDA_CHECK_LAUNCH(what);
+  if (c.splits > 1) {
+    const long long n = (a.M * a.N + 255) / 256, most = (long long)sm_count() * 8;
+    launch<k_join<T>>((unsigned)(n < most ? n : most), 256, 0, s, b);
+    SSD_CUDA_CHECK_LAUNCH("linear_join");
+  }
+  return SSD_OK;
+}
+constexpr int FEW = 8;
+template <typename T> int run_few(const MmArgs& a, cudaStream_t s) {
+  const int rm = a.M <= 1 ? 1 : a.M <= 2 ? 2 : a.M <= 4 ? 4 : 8;
+  const bool two = a.N >= 8192;   // enough warps for the SMs with two features each
+  const unsigned grid = (unsigned)((a.N + (two ? 16 : 8) - 1) / (two ? 16 : 8));
+#define FEW_RUN(RM) do { if (two) launch<k_mm_few<T, RM, 2>>(grid, 256, 0, s, a); else launch<k_mm_few<T, RM, 1>>(grid, 256, 0, s, a); } while (0)
+  if (rm == 1) FEW_RUN(1); else if (rm == 2) FEW_RUN(2); else if (rm == 4) FEW_RUN(4); else FEW_RUN(8);
+#undef FEW_RUN
+  SSD_CUDA_CHECK_LAUNCH("linear_few");
   return SSD_OK;
 }
 
@@ -672,8 +798,8 @@ int linear_backward(const LinPlan& p, const void* x, const void* w, const void* 
       return run_mm2("linear_dw", p.tdw, {g, false, gs}, {x, false, p.xs}, p.N, p.K, p.M, {(bf*)dw, nullptr, nullptr, nullptr, p.K, 0, 0}, part, status, s);
     dx = nullptr;
   }
-  if (dx && (rc = run_mm<T>("linear_dx", MmArgs{g, w, nullptr, nullptr, dx, nullptr, p.M, p.K, p.N, gs, 1, 1, p.K, p.K, 0, 0}, s))) return rc;
-  if (dw && (rc = run_mm<T>("linear_dw", MmArgs{g, x, nullptr, nullptr, dw, nullptr, p.N, p.K, p.M, 1, gs, 1, p.xs, p.K, 0, 0}, s))) return rc;
+  if (dx && (rc = run_mm<T>("linear_dx", MmArgs{g, w, nullptr, nullptr, dx, nullptr, p.M, p.K, p.N, gs, 1, 1, p.K, p.K, 0, 0, 1, 0, (float*)(ws + p.part_bwd)}, s))) return rc;
+  if (dw && (rc = run_mm<T>("linear_dw", MmArgs{g, x, nullptr, nullptr, dw, nullptr, p.N, p.K, p.M, 1, gs, 1, p.xs, p.K, 0, 0, 1, 0, (float*)(ws + p.part_bwd)}, s))) return rc;
   return rc;
 }
 
@@ -700,14 +826,16 @@ int32_t ssd_linear_forward(const SsdLinearDims* dims, const void* x, const void*
   if (!x || !weight || !out || !workspace) { set_error("linear: x, weight, out and workspace must be non-NULL"); return SSD_ERR_NULL_POINTER; }
   if (workspace_bytes < p.fwd_bytes) { set_error("linear: workspace too small: %zu < %zu", workspace_bytes, p.fwd_bytes); return SSD_ERR_WORKSPACE_TOO_SMALL; }
   cudaStream_t s = (cudaStream_t)cuda_stream;
+  char* ws = aligned_base(workspace);
+  const MmArgs a{x, weight, bias, residual, out, pre, p.M, p.N, p.K, p.xs, 1, p.K, 1, p.os, p.rs, p.act, 1, 0, (float*)(ws + p.part_fwd)};
+  const bool bf16 = dims->dtype == SSD_BF16, vectors = (((uintptr_t)x | (uintptr_t)weight) & 15) == 0 && p.K % (16 / p.es) == 0 && (p.M == 1 || p.xs % (16 / p.es) == 0);
+  if (p.M <= FEW && vectors) return bf16 ? run_few<__nv_bfloat16>(a, s) : run_few<float>(a, s);
   if (p.tc && map_fits(x, p.M, p.xs) && map_fits(weight, p.N, p.K)) {
-    char* ws = aligned_base(workspace);
     typedef __nv_bfloat16 bf;
     return run_mm2("linear_fwd", p.fwd, {x, true, p.xs}, {weight, true, p.K}, p.M, p.N, p.K,
                    {(bf*)out, (bf*)pre, (const bf*)bias, (const bf*)residual, p.os, p.rs, p.act}, (float*)(ws + p.part_fwd), (int*)ws, s);
   }
-  const MmArgs a{x, weight, bias, residual, out, pre, p.M, p.N, p.K, p.xs, 1, p.K, 1, p.os, p.rs, p.act};
-  return dims->dtype == SSD_BF16 ? run_mm<__nv_bfloat16>("linear_fwd", a, s) : run_mm<float>("linear_fwd", a, s);
+  return bf16 ? run_mm<__nv_bfloat16>("linear_fwd", a, s) : run_mm<float>("linear_fwd", a, s);
 }
 
 int32_t ssd_linear_backward(const SsdLinearDims* dims, const void* x, const void* weight, const void* pre, const void* dout,

@@ -207,10 +207,22 @@ struct PairWalk {
   }
 };
 
-template <typename T, int K>
+// What the convolution with a carried history adds to its operands: with ext = history (K-1 rows, zeros if absent) followed by
+// the input, pre[t] = bias + sum_k w[k] ext[t+k], new_history = ext[len .. len+K-2]; rows at or past a length are not read.
+struct Carry {
+  const void* history;     // [B, K-1, C] dense, or null
+  const int* lengths;      // [B], or null
+  int tiles;               // per sequence
+};
+__device__ __forceinline__ int carry_len(const SsdConvDims& d, const Carry& q, int b) {
+  return q.lengths ? min(max(__ldg(q.lengths + b), 0), d.seqlen) : d.seqlen;
+}
+
+// CARRY: rows before the sequence's first come from the history, and the CTAs of a sequence's first tile write the new one.
+template <typename T, int K, bool CARRY>
 __global__ void __launch_bounds__(CONVS_THREADS, CONVS_CTAS_PER_SM)
 k_conv_fwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__ weight, const float* __restrict__ bias,
-              T* __restrict__ out, int ntt) {
+              T* __restrict__ out, int ntt, Carry q, T* __restrict__ nh) {
   pdl_wait();
   constexpr int NC = 16 / (int)sizeof(T);            // channels per 16-byte copy piece
   constexpr int NP = 8 / (int)sizeof(T);             // channels per thread in the arithmetic (8 bytes: half the weights in
@@ -234,11 +246,14 @@ k_conv_fwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__
       const T* src = ibase + (long long)pw.b * d.in_stride_b + (long long)(t0 - (K - 1) + seg) * d.in_stride_l;
       unsigned char* sp = conv_smem + stage * STAGE_BYTES + cv * 16 + seg * CONVS_ROWB;
       int t = t0 - (K - 1) + seg;
+      const int len = CARRY ? carry_len(d, q, pw.b) : d.seqlen;
 #pragma unroll
       for (int j = 0; j < (ROWS + 15) / 16; ++j) {
         if (seg + 16 * j < ROWS) {
-          const bool ok = cok && t >= 0 && t < d.seqlen;
-          cp_async16(sp, ok ? (const void*)src : (const void*)in, ok);
+          const bool old = CARRY && t < 0 && q.history;
+          const bool ok = cok && (old || (t >= 0 && t < len));
+          const T* from = old ? (const T*)q.history + ((long long)pw.b * (K - 1) + t + K - 1) * d.channels + c0 : src;
+          cp_async16(sp, ok ? (const void*)from : (const void*)in, ok);
         }
         sp += 16 * CONVS_ROWB; src += 16 * d.in_stride_l; t += 16;
       }
@@ -269,6 +284,14 @@ k_conv_fwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__
     const int t0 = cur.tt * CONVS_TT + rs * TPT;
     const unsigned char* sp = conv_smem + stage * STAGE_BYTES + hv * 8 + rs * TPT * CONVS_ROWB;
     T* op = out + (long long)cur.b * d.out_stride_b + (long long)t0 * d.out_stride_l + c1;
+    const int len = CARRY ? carry_len(d, q, cur.b) : d.seqlen;
+    if (CARRY && nh && cur.tt == 0 && seg < K - 1 && cok) {
+      const int e = len + seg;                        // row of ext
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (e >= K - 1) v = __ldg(reinterpret_cast<const uint4*>(ibase + (long long)cur.b * d.in_stride_b + (long long)(e - (K - 1)) * d.in_stride_l));
+      else if (q.history) v = __ldg(reinterpret_cast<const uint4*>((const T*)q.history + ((long long)cur.b * (K - 1) + e) * d.channels + c0));
+      *reinterpret_cast<uint4*>(nh + ((long long)cur.b * (K - 1) + seg) * d.channels + c0) = v;
+    }
     cur.next();
     stage = stage + 1 == CONVS_STAGES ? 0 : stage + 1;
     if (!live) continue;
@@ -290,6 +313,7 @@ k_conv_fwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__
         unpack2(a2, a, b);
         o[2 * j] = d.activation ? a * sig_<T>(a) : a;
         o[2 * j + 1] = d.activation ? b * sig_<T>(b) : b;
+        if (CARRY && t0 + i >= len) o[2 * j] = o[2 * j + 1] = 0.f;
       }
       if (t0 + i < d.seqlen) store_n(op, o);
       op += d.out_stride_l;
@@ -949,17 +973,7 @@ __global__ void __launch_bounds__(32 * RED_GROUPS) k_norm_reduce(int nblk, int w
 }
 
 // ---------------------------------------------------------------------------------------------
-// The convolution with a carried history.  With ext = history (K-1 rows, zeros if absent) followed by the input,
-//     pre[t] = bias + sum_k w[k] ext[t+k],   out = act(pre),   new_history = ext[len .. len+K-2];
-// rows at or past a sequence's length are not read.
-struct Carry {
-  const void* history;     // [B, K-1, C] dense, or null
-  const int* lengths;      // [B], or null
-  int tiles;               // per sequence
-};
-__device__ __forceinline__ int carry_len(const SsdConvDims& d, const Carry& q, int b) {
-  return q.lengths ? min(max(q.lengths[b], 0), d.seqlen) : d.seqlen;
-}
+// The convolution with a carried history, where a row is too short for the staged kernel, its backward, and its single step.
 // row `e` of ext (e >= K-1: input row e-K+1, read when it is before the length), or zeros
 template <typename T, int K, int NC>
 __device__ __forceinline__ void load_ext(const T* in, const T* hist, long long stride_l, int channels, int e, int len, RawN<T, NC>& r) {
@@ -1160,36 +1174,58 @@ __global__ void __launch_bounds__(CONV_THREADS) k_carry_bwd(SsdConvDims d, Carry
   }
 }
 
-// One token per stream; the history moves up by a row in place.  Thread = (stream, 16 bytes of channels).
-template <typename T, int K>
+// One token per stream; the history moves up by a row in place.  Thread = 16 bytes of channels, whose weights it keeps, of SPT
+// streams: with one, a thread's 32 weights are 512 bytes of requests beside 80 bytes of stream.
+template <typename T, int K, int SPT>
 __global__ void __launch_bounds__(256) k_conv_step(SsdConvDims d, const T* __restrict__ in, const float* __restrict__ weight,
                                                    const float* __restrict__ bias, T* __restrict__ history, T* __restrict__ out) {
   pdl_wait();
   constexpr int NC = 16 / (int)sizeof(T);
-  const int CV = d.channels / NC;
+  typedef RawN<T, NC> Raw;
+  const int CV = d.channels / NC, groups = (d.batch + SPT - 1) / SPT;
   const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (item >= (long long)d.batch * CV) return;
+  if (item >= (long long)groups * CV) return;
   const int c0 = (int)(item % CV) * NC;
-  const long long b = item / CV;
-  T* hp = history + b * (K - 1) * d.channels + c0;
-  RawN<T, NC> r[K];
+  const long long b0 = item / CV;                    // streams b0, b0 + groups, ..
+  const long long C = d.channels;
+  Raw r[SPT][K];
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) r[k] = *reinterpret_cast<const RawN<T, NC>*>(hp + (long long)k * d.channels);
-  load_raw(in + b * d.in_stride_b + c0, r[K - 1]);
-  float o[NC];
+  for (int i = 0; i < SPT; ++i) {
+    const long long b = min(b0 + (long long)i * groups, (long long)d.batch - 1);
 #pragma unroll
-  for (int j = 0; j < NC; ++j) o[j] = bias ? __ldg(bias + c0 + j) : 0.f;
+    for (int k = 0; k < K - 1; ++k) r[i][k] = *reinterpret_cast<const Raw*>(history + (b * (K - 1) + k) * C + c0);
+    load_raw(in + b * d.in_stride_b + c0, r[i][K - 1]);
+  }
+  float w[NC * K], bs[NC];                           // w[j * K + k]
+  const float* wp = weight + (size_t)c0 * K;
+  if ((reinterpret_cast<uintptr_t>(weight) & 15) == 0) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    float v[NC];
-    unpack_raw(r[k], v);
+    for (int i = 0; i < NC * K / 4; ++i) *reinterpret_cast<float4*>(w + 4 * i) = __ldg(reinterpret_cast<const float4*>(wp) + i);
+  } else {
 #pragma unroll
-    for (int j = 0; j < NC; ++j) o[j] = fmaf(__ldg(weight + (size_t)(c0 + j) * K + k), v[j], o[j]);
-    if (k > 0) *reinterpret_cast<RawN<T, NC>*>(hp + (long long)(k - 1) * d.channels) = r[k];
+    for (int i = 0; i < NC * K; ++i) w[i] = __ldg(wp + i);
   }
 #pragma unroll
-  for (int j = 0; j < NC; ++j) if (d.activation) o[j] *= sig_<T>(o[j]);
-  store_n(out + b * d.out_stride_b + c0, o);
+  for (int j = 0; j < NC; ++j) bs[j] = bias ? __ldg(bias + c0 + j) : 0.f;
+#pragma unroll
+  for (int i = 0; i < SPT; ++i) {
+    const long long b = b0 + (long long)i * groups;
+    if (b >= d.batch) break;
+    float o[NC];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) o[j] = bs[j];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float v[NC];
+      unpack_raw(r[i][k], v);
+#pragma unroll
+      for (int j = 0; j < NC; ++j) o[j] = fmaf(w[j * K + k], v[j], o[j]);
+      if (k > 0) *reinterpret_cast<Raw*>(history + (b * (K - 1) + k - 1) * C + c0) = r[i][k];
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j) if (d.activation) o[j] *= sig_<T>(o[j]);
+    store_n(out + b * d.out_stride_b + c0, o);
+  }
 }
 int carry_bwd_tiles(const SsdConvDims* d) { return (d->seqlen + d->width - 1 + CARRY_TLB - 1) / CARRY_TLB; }
 int carry_rows(const SsdConvDims* d) {
@@ -1271,7 +1307,7 @@ int32_t ssd_conv1d_forward(const SsdConvDims* dims, const void* in, const float*
     const dim3 grid((unsigned)gx, (unsigned)ncb);
 #define CONV_FWD_SM(T, K) do { \
       constexpr int smem = (CONVS_TT + K - 1) * CONVS_ROWB * CONVS_STAGES; \
-      launch<k_conv_fwd_sm<T, K>>(grid, CONVS_THREADS, smem, s, *dims, (const T*)in, weight, bias, (T*)out, ntt); } while (0)
+      launch<k_conv_fwd_sm<T, K, false>>(grid, CONVS_THREADS, smem, s, *dims, (const T*)in, weight, bias, (T*)out, ntt, Carry{}, (T*)nullptr); } while (0)
     if (dims->dtype == SSD_BF16) {
       if (dims->width == 4) CONV_FWD_SM(__nv_bfloat16, 4); else if (dims->width == 3) CONV_FWD_SM(__nv_bfloat16, 3); else CONV_FWD_SM(__nv_bfloat16, 2);
     } else {
@@ -1407,6 +1443,21 @@ int32_t ssd_conv1d_carry_forward(const SsdConvDims* dims, const void* in, const 
     return SSD_ERR_BAD_SHAPE;
   }
   cudaStream_t s = (cudaStream_t)cuda_stream;
+  if ((long long)dims->channels * es >= CONVS_ROWB / 2) {   // as in ssd_conv1d_forward
+    const int ntt = (dims->seqlen + CONVS_TT - 1) / CONVS_TT, ncb = (dims->channels * es + CONVS_ROWB - 1) / CONVS_ROWB;
+    const long long pairs = (long long)dims->batch * ntt;
+    if (pairs > 0x7fffffffLL || ncb > 65535) { set_error("conv1d carry: too many token tiles or channels"); return SSD_ERR_UNSUPPORTED; }
+    long long gx = (long long)sm_count() * CONVS_CTAS_PER_SM / ncb;
+    if (gx > pairs) gx = pairs;
+    if (gx < 1) gx = 1;
+    const Carry q{history, lengths, ntt};
+#define CARRY_RUN(T, K) launch<k_conv_fwd_sm<T, K, true>>(dim3((unsigned)gx, (unsigned)ncb), CONVS_THREADS, (CONVS_TT + K - 1) * CONVS_ROWB * CONVS_STAGES, s, \
+                                                          *dims, (const T*)in, weight, bias, (T*)out, ntt, q, (T*)new_history)
+    CARRY_BY_TYPE(CARRY_RUN);
+#undef CARRY_RUN
+    SSD_CUDA_CHECK_LAUNCH("conv1d_carry_fwd");
+    return SSD_OK;
+  }
   const Carry q{history, lengths, (dims->seqlen + CARRY_TL - 1) / CARRY_TL};
   const long long blocks = ((long long)dims->batch * q.tiles * (dims->channels * es / 16) + CONV_THREADS - 1) / CONV_THREADS;
   if (blocks > 0x7fffffffLL) { set_error("conv1d carry: too many blocks for one grid (%lld)", blocks); return SSD_ERR_UNSUPPORTED; }
@@ -1461,9 +1512,13 @@ int32_t ssd_conv1d_step(const SsdConvDims* dims, const void* in, const float* we
   if (!weight) { set_error("conv1d step: weight is NULL"); return SSD_ERR_NULL_POINTER; }
   const int es = dims->dtype == SSD_BF16 ? 2 : 4;
   cudaStream_t s = (cudaStream_t)cuda_stream;
-  const long long blocks = ((long long)dims->batch * (dims->channels * es / 16) + 255) / 256;
+  const long long vecs = dims->channels * es / 16;
+  const bool four = dims->batch * vecs >= 4LL * sm_count() * 512;   // a thread of four streams still leaves 16 warps to an SM
+  const long long blocks = ((four ? (dims->batch + 3LL) / 4 : dims->batch) * vecs + 255) / 256;
   if (blocks > 0x7fffffffLL) { set_error("conv1d step: too many blocks for one grid (%lld)", blocks); return SSD_ERR_UNSUPPORTED; }
-#define CARRY_RUN(T, K) launch<k_conv_step<T, K>>((unsigned)blocks, 256, 0, s, *dims, (const T*)in, weight, bias, (T*)history, (T*)out)
+#define CARRY_RUN(T, K) do { \
+    if (four) launch<k_conv_step<T, K, 4>>((unsigned)blocks, 256, 0, s, *dims, (const T*)in, weight, bias, (T*)history, (T*)out); \
+    else launch<k_conv_step<T, K, 1>>((unsigned)blocks, 256, 0, s, *dims, (const T*)in, weight, bias, (T*)history, (T*)out); } while (0)
   CARRY_BY_TYPE(CARRY_RUN);
 #undef CARRY_RUN
   SSD_CUDA_CHECK_LAUNCH("conv1d_step");

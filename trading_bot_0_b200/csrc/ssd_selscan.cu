@@ -72,6 +72,10 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
 __device__ __forceinline__ float hsum(f32x2 v) { float a, b; unpack2(v, a, b); return a + b; }
 __device__ __forceinline__ f32x2 dup2(float v) { return pack2(v, v); }
 __device__ __forceinline__ f32x2 ex2_2(f32x2 v) { float a, b; unpack2(v, a, b); return pack2(ex2(a), ex2(b)); }
+// exp(s A) for a pair of decays (A2 = A log2 e).  ex2.approx is 2e-8 low on average over the arguments that decays have (1.7e-8 to
+// 2.6e-8 in every interval measured between -0.75 and -0.001; rms 4e-8); a state is a product of hundreds of them, where an offset
+// adds up and scatter does not, so the argument is raised by 2e-8 log2 e.
+__device__ __forceinline__ f32x2 decay2(f32x2 A2, f32x2 s2) { return ex2_2(fma2(A2, s2, pack2(2.9e-8f, 2.9e-8f))); }
 
 struct Place { int b, seg, g, d, c; bool live; };    // batch row, part, group, channel (of all), channel of the block
 template <int LPC> __device__ __forceinline__ Place place(const SelGeo& q, int c) {
@@ -140,8 +144,8 @@ __global__ void __launch_bounds__(Sh<LPC>::TH) k_sel_fwd(SelGeo q, SelFwd p) {
       const long long at = ((long long)me.b * q.segs + s) * q.D + me.d;
       const float4 v = *reinterpret_cast<const float4*>(p.segst + at * NP + nl * 4);
       const f32x2 d2 = dup2(p.segdt[at]);
-      h01 = fma2(ex2_2(mul2(A01, d2)), h01, pack2(v.x, v.y));
-      h23 = fma2(ex2_2(mul2(A23, d2)), h23, pack2(v.z, v.w));
+      h01 = fma2(decay2(A01, d2), h01, pack2(v.x, v.y));
+      h23 = fma2(decay2(A23, d2), h23, pack2(v.z, v.w));
     }
   }
 
@@ -209,8 +213,8 @@ __global__ void __launch_bounds__(Sh<LPC>::TH) k_sel_fwd(SelGeo q, SelFwd p) {
           const float2 sd = s_dt[buf][u + i][c];
           const float4 b4 = *reinterpret_cast<const float4*>(&s_B[buf][u + i][nl * 4]);
           const f32x2 s2 = dup2(sd.x), x2 = dup2(sd.y);
-          h01 = fma2(ex2_2(mul2(A01, s2)), h01, mul2(pack2(b4.x, b4.y), x2));
-          h23 = fma2(ex2_2(mul2(A23, s2)), h23, mul2(pack2(b4.z, b4.w), x2));
+          h01 = fma2(decay2(A01, s2), h01, mul2(pack2(b4.x, b4.y), x2));
+          h23 = fma2(decay2(A23, s2), h23, mul2(pack2(b4.z, b4.w), x2));
           if (MODE == 1) dtsum += sd.x;
           if (MODE == 0) {
             const float4 c4 = *reinterpret_cast<const float4*>(&s_C[buf][u + i][nl * 4]);
@@ -319,8 +323,8 @@ __global__ void __launch_bounds__(Sh<LPC>::TH) k_sel_bwd_part(SelGeo q, SelBwd p
       const float2 sd = s_dt[r][c];
       const float4 c4 = *reinterpret_cast<const float4*>(&s_C[r][nl * 4]);
       const f32x2 s2 = dup2(sd.x), y2 = dup2(sd.y);
-      g01 = mul2(ex2_2(mul2(A01, s2)), fma2(pack2(c4.x, c4.y), y2, g01));
-      g23 = mul2(ex2_2(mul2(A23, s2)), fma2(pack2(c4.z, c4.w), y2, g23));
+      g01 = mul2(decay2(A01, s2), fma2(pack2(c4.x, c4.y), y2, g01));
+      g23 = mul2(decay2(A23, s2), fma2(pack2(c4.z, c4.w), y2, g23));
       dtsum += sd.x;
     }
   }
@@ -391,8 +395,8 @@ __global__ void __launch_bounds__(Sh<LPC>::TH) k_sel_bwd(SelGeo q, SelBwd p) {
     const long long at = ((long long)me.b * q.segs + s) * q.D + me.d;
     const float4 v = *reinterpret_cast<const float4*>(p.segst + at * NP + nl * 4);
     const f32x2 d2 = dup2(p.segdt[at]);
-    g01 = fma2(ex2_2(mul2(A01, d2)), g01, pack2(v.x, v.y));
-    g23 = fma2(ex2_2(mul2(A23, d2)), g23, pack2(v.z, v.w));
+    g01 = fma2(decay2(A01, d2), g01, pack2(v.x, v.y));
+    g23 = fma2(decay2(A23, d2), g23, pack2(v.z, v.w));
   }
   f32x2 dA01 = 0ull, dA23 = 0ull;
   float dD = 0.f, dbias = 0.f;
@@ -448,7 +452,7 @@ __global__ void __launch_bounds__(Sh<LPC>::TH) k_sel_bwd(SelGeo q, SelBwd p) {
       const float4 v = s_v[r][c];
       const float4 b4 = *reinterpret_cast<const float4*>(&s_B[r][nl * 4]);
       const f32x2 s2 = dup2(v.x), x2 = dup2(v.y);
-      a01[r] = ex2_2(mul2(A01, s2)); a23[r] = ex2_2(mul2(A23, s2));
+      a01[r] = decay2(A01, s2); a23[r] = decay2(A23, s2);
       h01[r + 1] = fma2(a01[r], h01[r], mul2(pack2(b4.x, b4.y), x2));
       h23[r + 1] = fma2(a23[r], h23[r], mul2(pack2(b4.z, b4.w), x2));
     }
