@@ -451,7 +451,7 @@ SSD_API int32_t ssd_conv1d_step(const SsdConvDims* dims, const void* in, const f
 /*
  * A layer's projection: out = act(x W^T + bias) + residual, x [rows, in_features], W [out_features, in_features] dense, all of one
  * storage dtype; products are added in fp32 and the result is rounded once.  bf16 operands whose rows are 16-byte aligned run on
- * the tensor cores; all other sizes, strides and fp32 on the CUDA cores in fp32.  `pre` (optional, dense, storage dtype) receives
+ * the tensor cores; all other sizes, strides and fp32 on the CUDA cores in fp32.  `pre` (optional, dense, fp32) receives
  * x W^T + bias for the backward, which needs it where act is not NONE.  Backward: dpre = dout * act'(pre), dx = dpre W,
  * dweight = dpre^T x, dbias = sum of dpre over the rows; each of the three is optional.
  */

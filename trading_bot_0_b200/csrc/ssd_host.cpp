@@ -641,7 +641,7 @@ void linear_fwd(const Tensor& x, const Tensor& w, const Tensor* bias, const Tens
   } else {
     out = like_rows(x, N, x.scalar_type());
   }
-  if (for_backward && act) pre = like_rows(x, N, x.scalar_type());
+  if (for_backward && act) pre = like_rows(x, N, at::kFloat);
   Tensor ws = bytes_on(api.linear_workspace_bytes(&d, SSD_PASS_FWD), dev);
   check_rc(api.linear_forward(&d, ptr(&xr), ptr(&w), ptr(bias), ptr(&rr), ptr(&out), ptr(&pre), ws.data_ptr(), (size_t)ws.numel(), stream_of(dev)));
 }
@@ -653,14 +653,14 @@ LinGrads linear_bwd(const Tensor& dout, const Tensor& x, const Tensor& w, const 
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor xr = as_rows("x", x, d.in_features);
   d.rows = xr.size(0); d.x_stride_row = apart(xr, 0);
-  auto check = [&](const char* name, const Tensor& t) {
-    if (t.scalar_type() != x.scalar_type() || t.device() != dev || t.dim() < 1 || t.size(-1) != N || t.numel() != d.rows * N)
-      fail("linear: ", name, ": expected x's leading dims with ", N, " values in the last, ", x.scalar_type(), " on ", dev, ", got ", t.sizes(), " ",
+  auto check = [&](const char* name, const Tensor& t, at::ScalarType st) {
+    if (t.scalar_type() != st || t.device() != dev || t.dim() < 1 || t.size(-1) != N || t.numel() != d.rows * N)
+      fail("linear: ", name, ": expected x's leading dims with ", N, " values in the last, ", st, " on ", dev, ", got ", t.sizes(), " ",
            t.scalar_type(), " on ", t.device());
   };
-  check("dout", dout);
+  check("dout", dout, x.scalar_type());
   if (act && !pre) fail("linear: an activation needs the pre that the forward returned with for_backward");
-  if (pre) { check("pre", *pre); if (!pre->is_contiguous()) fail("linear: pre must be contiguous"); }
+  if (pre) { check("pre", *pre, at::kFloat); if (!pre->is_contiguous()) fail("linear: pre must be contiguous"); }
   const Tensor gr = as_rows("dout", dout, N);
   LinGrads g;
   if (want_dx) g.dx = empty(x.sizes(), x.scalar_type(), dev);

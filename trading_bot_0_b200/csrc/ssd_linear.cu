@@ -34,6 +34,11 @@ __device__ __forceinline__ void values_of(const uint4& r, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) { const float2 f = umma::unpack_bf16(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
 }
+template <int V> __device__ __forceinline__ void load_floats(const float* p, float (&v)[V]) {
+  if (V == 1) { v[0] = *p; return; }
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i) *reinterpret_cast<float4*>(v + 4 * i) = *reinterpret_cast<const float4*>(p + 4 * i);
+}
 template <typename T> __device__ __forceinline__ void put_values(T* p, const float (&v)[1]) { stf(p, v[0]); }
 __device__ __forceinline__ void put_values(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ void put_values(__nv_bfloat16* p, const float (&v)[8]) {
@@ -43,7 +48,8 @@ __device__ __forceinline__ void put_values(__nv_bfloat16* p, const float (&v)[8]
 // out[m][n] = epilogue(sum_k P(m,k) Q(n,k)); element strides of P and Q along both dims.
 struct MmArgs {
   const void *P, *Q, *bias, *residual;
-  void *out, *pre;
+  void* out;
+  float* pre;
   long long M, N, K, psm, psk, qsn, qsk, os, rs;
   int act, splits;
   long long kper;
@@ -51,7 +57,7 @@ struct MmArgs {
 };
 template <typename T> __device__ __forceinline__ void finish(const MmArgs& a, long long m, long long n, float v) {
   if (a.bias) v += ldf((const T*)a.bias + n);
-  if (a.pre) stf((T*)a.pre + m * a.N + n, v);
+  if (a.pre) a.pre[m * a.N + n] = v;
   v = act_of(v, a.act);
   if (a.residual) v += ldf((const T*)a.residual + m * a.rs + n);
   stf((T*)a.out + m * a.os + n, v);
@@ -193,7 +199,7 @@ __global__ void __launch_bounds__(256) k_mm_few(MmArgs a) {
 namespace u = umma;
 constexpr int MM_STAGES = 5, MM_BM = 256, MM_EPI = 8, MM_THREADS = 32 * (4 + MM_EPI);
 constexpr int MM_STAGE = 32768;                    // 16 KB of P, 16 KB of Q
-constexpr int MM_SLOT = 4096;                      // output staging of a warp: two boxes of 32 x 32 bf16, or one of fp32
+constexpr int MM_SLOT = 6144;                      // output staging of a warp: a box of 32 x 32 fp32 and one of bf16, or two of bf16
 constexpr int MM_ROWS = 8;                         // tile rows walked side by side: the pairs at work share operands in the L2
 constexpr size_t MM_SMEM = (size_t)MM_STAGES * MM_STAGE + MM_EPI * MM_SLOT + 1024;
 
@@ -204,8 +210,8 @@ struct Mm2 {
   int act, vec;                                    // vec: tensor maps fit out, pre and residual (with splits: the sums)
   long long os, rs;
   const __nv_bfloat16 *bias, *residual;
-  __nv_bfloat16 *out, *pre;
-  float* part;                                     // [splits][out rows][out columns]
+  __nv_bfloat16* out;
+  float *pre, *part;                                     // [splits][out rows][out columns]
   int* status;
 };
 
@@ -219,7 +225,7 @@ __device__ __forceinline__ void unit_at(const Mm2& a, int un, int& sp, int& r, i
 // One value of the result at output row m and column n.
 __device__ __forceinline__ void finish_one(const Mm2& a, long long cols, long long m, long long n, float v) {
   if (a.bias) v += __bfloat162float(a.bias[n]);
-  if (a.pre) a.pre[m * cols + n] = __float2bfloat16_rn(v);
+  if (a.pre) a.pre[m * cols + n] = v;
   v = act_of(v, a.act);
   if (a.residual) v += __bfloat162float(a.residual[m * a.rs + n]);
   a.out[m * a.os + n] = __float2bfloat16_rn(v);
@@ -411,16 +417,15 @@ k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMa
           const float4 b = *reinterpret_cast<const float4*>(&s_bias[buf][j + 4 * i]);
           v[4 * i] += b.x; v[4 * i + 1] += b.y; v[4 * i + 2] += b.z; v[4 * i + 3] += b.w;
         }
-        auto put = [&](const CUtensorMap* map) {     // two boxes in turn: the older store has read its box
+        auto put = [&](const CUtensorMap* map, int at, bool f32) {   // two boxes in turn: the older store has read its box
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
           __syncwarp();
-          stage_bf16(slot_a + box * 2048, lane, v);
+          if (f32) stage_f32(slot_a + at, lane, v); else stage_bf16(slot_a + at, lane, v);
           u::fence_async_smem();
           __syncwarp();
-          if (lane == 0 && row0 < a.M) { u::tma_store_3d(map, slot_p + box * 2048, (int)n0 + j, row0, 0); u::bulk_commit(); }
-          box ^= 1;
+          if (lane == 0 && row0 < a.M) { u::tma_store_3d(map, slot_p + at, (int)n0 + j, row0, 0); u::bulk_commit(); }
         };
-        if (a.pre) put(&tpre);
+        if (a.pre) put(&tpre, 0, true);
         if (a.act == SSD_ACT_SILU) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = act_of(v[i], SSD_ACT_SILU);
@@ -442,7 +447,8 @@ k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMa
             }
           }
         }
-        put(&tout);
+        put(&tout, a.pre ? 4096 : box * 2048, false);
+        box ^= 1;
       }
       u::tc_fence_before();
       __syncwarp();
@@ -476,7 +482,7 @@ __global__ void __launch_bounds__(256) k_mm2_join(Mm2 a, long long rows, long lo
 // part of the rows (`parts` of them on the y axis).  Thread = V neighbouring columns, block = 32 V columns x 8 rows at a time, four
 // rows of a thread requested together.  V = 16 bytes where all rows start on 16 bytes, else one value.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) k_dpre(long long M, int N, int act, const T* __restrict__ dout, long long dos, const T* __restrict__ pre,
+__global__ void __launch_bounds__(256) k_dpre(long long M, int N, int act, const T* __restrict__ dout, long long dos, const float* __restrict__ pre,
                                               T* __restrict__ dpre, float* __restrict__ partial) {
   __shared__ float s[8][32 * V];
   pdl_wait();
@@ -487,24 +493,22 @@ __global__ void __launch_bounds__(256) k_dpre(long long M, int N, int act, const
   float a[V] = {};
   if (n < N) {
     for (long long m = lo + threadIdx.y; m < hi; m += 8 * R) {
-      Raw g[R], p[R];
-      float t[V] = {};
+      Raw g[R];
+      float q[R][V], t[V] = {};
 #pragma unroll
       for (int r = 0; r < R; ++r)
         if (m + 8 * r < hi) {
           g[r] = *reinterpret_cast<const Raw*>(dout + (m + 8 * r) * dos + n);
-          if (act) p[r] = *reinterpret_cast<const Raw*>(pre + (m + 8 * r) * N + n);
+          if (act) load_floats(pre + (m + 8 * r) * N + n, q[r]);
         }
 #pragma unroll
       for (int r = 0; r < R; ++r)
         if (m + 8 * r < hi) {
-          float x[V], q[V];
+          float x[V];
           values_of(g[r], x);
-          if (act) {
-            values_of(p[r], q);
+          if (act)
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[j] *= dact_of(q[j], act);
-          }
+            for (int j = 0; j < V; ++j) x[j] *= dact_of(q[r][j], act);
 #pragma unroll
           for (int j = 0; j < V; ++j) t[j] += x[j];
           if (dpre) put_values(dpre + (m + 8 * r) * N + n, x);
@@ -620,7 +624,7 @@ size_t part_bytes(const TileShape& t, long long M, long long N) { return t.split
 
 // out [M,N] of P (rows M) and Q (rows N): pointer, whether its k runs along memory, and the stride of its memory rows.
 struct Operand { const void* p; bool kmajor; long long stride; };
-struct Result { __nv_bfloat16 *out, *pre; const __nv_bfloat16 *bias, *residual; long long os, rs; int act; };
+struct Result { __nv_bfloat16* out; float* pre; const __nv_bfloat16 *bias, *residual; long long os, rs; int act; };
 int run_mm2(const char* what, const TileShape& t, Operand P, Operand Q, long long M, long long N, long long K, const Result& o, float* part,
             int* status, cudaStream_t s) {
   Mm2 a;
@@ -640,7 +644,7 @@ int run_mm2(const char* what, const TileShape& t, Operand P, Operand Q, long lon
   tout = tpre = tp;
   if (a.vec) {
     rc = t.splits > 1 ? make_out_map(&tout, part, true, t.splits, M, N, N, what) : make_out_map(&tout, o.out, false, 1, M, N, o.os, what);
-    if (!rc && t.splits == 1 && o.pre) rc = make_out_map(&tpre, o.pre, false, 1, M, N, N, what);
+    if (!rc && t.splits == 1 && o.pre) rc = make_out_map(&tpre, o.pre, true, 1, M, N, N, what);
     if (rc) return rc;
   }
   const int pairs = a.units < 74 ? a.units : 74;
@@ -776,9 +780,9 @@ int linear_backward(const LinPlan& p, const void* x, const void* w, const void* 
     float* partial = db ? (float*)(ws + p.partial) : nullptr;
     constexpr int V = 16 / (int)sizeof(T);
     if (p.N % V == 0 && dos % V == 0 && (((uintptr_t)dout | (p.act ? (uintptr_t)pre : 0)) & 15) == 0)
-      launch<k_dpre<T, V>>(dim3((p.N + 32 * V - 1) / (32 * V), p.parts), dim3(32, 8), 0, s, p.M, p.N, p.act, (const T*)dout, dos, (const T*)pre, dpre, partial);
+      launch<k_dpre<T, V>>(dim3((p.N + 32 * V - 1) / (32 * V), p.parts), dim3(32, 8), 0, s, p.M, p.N, p.act, (const T*)dout, dos, (const float*)pre, dpre, partial);
     else
-      launch<k_dpre<T, 1>>(dim3((p.N + 31) / 32, p.parts), dim3(32, 8), 0, s, p.M, p.N, p.act, (const T*)dout, dos, (const T*)pre, dpre, partial);
+      launch<k_dpre<T, 1>>(dim3((p.N + 31) / 32, p.parts), dim3(32, 8), 0, s, p.M, p.N, p.act, (const T*)dout, dos, (const float*)pre, dpre, partial);
     SSD_CUDA_CHECK_LAUNCH("linear_dpre");
     if (db) {
       launch<k_dbias<T>>((p.N + 31) / 32, dim3(32, 32), 0, s, p.N, p.parts, (const float*)partial, (T*)db);
@@ -827,13 +831,13 @@ int32_t ssd_linear_forward(const SsdLinearDims* dims, const void* x, const void*
   if (workspace_bytes < p.fwd_bytes) { set_error("linear: workspace too small: %zu < %zu", workspace_bytes, p.fwd_bytes); return SSD_ERR_WORKSPACE_TOO_SMALL; }
   cudaStream_t s = (cudaStream_t)cuda_stream;
   char* ws = aligned_base(workspace);
-  const MmArgs a{x, weight, bias, residual, out, pre, p.M, p.N, p.K, p.xs, 1, p.K, 1, p.os, p.rs, p.act, 1, 0, (float*)(ws + p.part_fwd)};
+  const MmArgs a{x, weight, bias, residual, out, (float*)pre, p.M, p.N, p.K, p.xs, 1, p.K, 1, p.os, p.rs, p.act, 1, 0, (float*)(ws + p.part_fwd)};
   const bool bf16 = dims->dtype == SSD_BF16, vectors = (((uintptr_t)x | (uintptr_t)weight) & 15) == 0 && p.K % (16 / p.es) == 0 && (p.M == 1 || p.xs % (16 / p.es) == 0);
   if (p.M <= FEW && vectors) return bf16 ? run_few<__nv_bfloat16>(a, s) : run_few<float>(a, s);
   if (p.tc && map_fits(x, p.M, p.xs) && map_fits(weight, p.N, p.K)) {
     typedef __nv_bfloat16 bf;
     return run_mm2("linear_fwd", p.fwd, {x, true, p.xs}, {weight, true, p.K}, p.M, p.N, p.K,
-                   {(bf*)out, (bf*)pre, (const bf*)bias, (const bf*)residual, p.os, p.rs, p.act}, (float*)(ws + p.part_fwd), (int*)ws, s);
+                   {(bf*)out, (float*)pre, (const bf*)bias, (const bf*)residual, p.os, p.rs, p.act}, (float*)(ws + p.part_fwd), (int*)ws, s);
   }
   return bf16 ? run_mm<__nv_bfloat16>("linear_fwd", a, s) : run_mm<float>("linear_fwd", a, s);
 }

@@ -8,6 +8,8 @@
 // (one bf16 token-channel is 8 bytes moved against dstate exponentials).  A thread holds four states of one channel in registers
 // and walks the tokens; dstate / 4 neighbouring lanes make up a channel.  What is needed once per token and channel (softplus, s x,
 // the gate) is computed once by one thread of the block, a tile of 16 tokens ahead, and handed over in shared memory.
+#include <initializer_list>
+
 #include "common.cuh"
 #include "ssd_internal.h"
 #include "umma.cuh"
@@ -17,27 +19,34 @@ namespace {
 
 using umma::ex2;
 
-constexpr int SEL_T = 16;             // tokens per tile, and between the states kept for the backward pass
+constexpr int SEL_T = 16;             // tokens per tile
+constexpr int SEL_C = 8;              // tokens between the states kept for the backward pass
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct SelGeo {
   int B, L, D, N, G, Dg, nb;          // nb = channel blocks per group
   int segs, seg_len;                  // the tokens in `segs` parts of seg_len (a multiple of SEL_T)
-  int softplus, nt;                   // nt = tiles of the whole sequence
+  int softplus, nc;                   // nc = states kept per channel and sequence
+  int wide;                           // four channels of a row may be moved at once
   int par_row;                        // a block's sums of dA, dD and ddt_bias: D*NP + 2*D floats, up to a multiple of four
   long long xsb, xsl, dtsb, dtsl, bsb, bsl, csb, csl, zsb, zsl, ysb, ysl;
 };
 
-// Lanes per channel -> block shape.
-template <int LPC> struct Sh {
-  static constexpr int NP = 4 * LPC;                 // states per channel, padded
-  static constexpr int CHB = LPC <= 8 ? 32 : 16;     // channels per block
+// Block shape for LPC lanes per channel with KS states each.  Two roles: the scan (thread = KS states of a channel), and tasks of a
+// token and four neighbouring channels, in which everything that a token needs once per channel is loaded, computed and stored.
+template <int KS_, int LPC_, int CHB_> struct Sh {
+  static constexpr int KS = KS_, LPC = LPC_, CHB = CHB_;
+  static constexpr int KP = KS / 2;                  // pairs of states
+  static constexpr int NP = KS * LPC;                // states per channel, padded
   static constexpr int TH = CHB * LPC;               // threads
-  static constexpr int IT = SEL_T * CHB / TH;        // (token, channel) items per thread
-  static constexpr int RS = TH / CHB;                // tokens between a thread's items
-  static constexpr int BI = SEL_T * NP / TH;         // values of B (and of C) per thread
   static constexpr int W = TH / 32;
-  static constexpr int BWD_SMEM = SEL_T * CHB * 16 + W * SEL_T * 2 * NP * 4;   // backward: a tile's values per channel, the warps' shares of dB and dC
+  static constexpr int CPW = 32 / LPC;               // channels per warp
+  static constexpr int QR = CHB / 4;                 // tasks per token
+  static constexpr int RS = TH / QR < SEL_T ? TH / QR : SEL_T;   // tokens between a thread's tasks
+  static constexpr int IT = SEL_T / RS;              // tasks per thread
+  static constexpr int BI = (SEL_T * NP + TH - 1) / TH;          // values of B (and of C) per thread
+  static constexpr int COPIES = CPW < KS ? CPW : KS; // backward: orders of the states among a warp's lanes (see ChannelSum)
+  static constexpr int BWD_SMEM = (SEL_T * CHB * 4 + 2 * COPIES * SEL_T * NP + W * SEL_T * 2 * NP + 3 * SEL_T * CHB) * 4;
 };
 
 // log(1 + e) for e in [0, 1]: e P(e) with P the least-maximum fit of log1p(e) / e of degree 8 (relative error 3e-8, 1.7e-7 as
@@ -54,14 +63,23 @@ __device__ __forceinline__ float log1p01(float e) {
   p = fmaf(p, e, 0.99999997f);
   return p * e;
 }
+// exp(-|v|), the rounding of the argument made good
+__device__ __forceinline__ float exp_neg(float v) {
+  const float x = -fabsf(v), t = x * LOG2E, r = fmaf(x, LOG2E, -t), e = ex2(t);
+  return fmaf(e, r * LN2, e);
+}
 // softplus(v) = max(v, 0) + log(1 + exp(-|v|))
 __device__ __forceinline__ float sel_step(float raw, float bias, int softplus) {
   const float v = raw + bias;
-  return softplus ? fmaxf(v, 0.f) + log1p01(expf(-fabsf(v))) : v;
+  return softplus ? fmaxf(v, 0.f) + log1p01(exp_neg(v)) : v;
 }
-// d step / d raw
-__device__ __forceinline__ float sel_dstep(float raw, float bias, int softplus) {
-  return softplus ? 1.f / (1.f + __expf(-(raw + bias))) : 1.f;
+// the same, and its derivative 1 / (1 + exp(-v)) from the same exponential
+__device__ __forceinline__ float sel_step_d(float raw, float bias, int softplus, float& d) {
+  const float v = raw + bias;
+  if (!softplus) { d = 1.f; return v; }
+  const float e = exp_neg(v);
+  d = __fdividef(v >= 0.f ? 1.f : e, 1.f + e);
+  return fmaxf(v, 0.f) + log1p01(e);
 }
 __device__ __forceinline__ float sig(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
 __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
@@ -77,26 +95,115 @@ __device__ __forceinline__ f32x2 ex2_2(f32x2 v) { float a, b; unpack2(v, a, b); 
 // adds up and scatter does not, so the argument is raised by 2e-8 log2 e.
 __device__ __forceinline__ f32x2 decay2(f32x2 A2, f32x2 s2) { return ex2_2(fma2(A2, s2, pack2(2.9e-8f, 2.9e-8f))); }
 
-struct Place { int b, seg, g, d, c; bool live; };    // batch row, part, group, channel (of all), channel of the block
-template <int LPC> __device__ __forceinline__ Place place(const SelGeo& q, int c) {
+// The same once more (a value that the compiler does not keep from the first time).
+__device__ __forceinline__ f32x2 decay2_again(f32x2 A2, f32x2 s2) {
+  float a, b;
+  unpack2(fma2(A2, s2, pack2(2.9e-8f, 2.9e-8f)), a, b);
+  asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+  return pack2(a, b);
+}
+
+// Four neighbouring values of a row as they lie in memory.
+template <typename T> struct Raw4;
+template <> struct Raw4<float> { float4 v; };
+template <> struct Raw4<__nv_bfloat16> { uint2 v; };
+__device__ __forceinline__ void zero4(Raw4<float>& r) { r.v = make_float4(0.f, 0.f, 0.f, 0.f); }
+__device__ __forceinline__ void zero4(Raw4<__nv_bfloat16>& r) { r.v = make_uint2(0, 0); }
+__device__ __forceinline__ void load4(const float* p, bool wide, int n, Raw4<float>& r) {   // n = 1..4 values are there
+  if (wide) { r.v = *reinterpret_cast<const float4*>(p); return; }
+  r.v = make_float4(p[0], n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, bool wide, int n, Raw4<__nv_bfloat16>& r) {
+  if (wide) { r.v = *reinterpret_cast<const uint2*>(p); return; }
+  const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+  r.v.x = q[0] | (n > 1 ? (uint32_t)q[1] << 16 : 0u);
+  r.v.y = (n > 2 ? q[2] : 0u) | (n > 3 ? (uint32_t)q[3] << 16 : 0u);
+}
+__device__ __forceinline__ void values4(const Raw4<float>& r, float (&v)[4]) { v[0] = r.v.x; v[1] = r.v.y; v[2] = r.v.z; v[3] = r.v.w; }
+__device__ __forceinline__ void values4(const Raw4<__nv_bfloat16>& r, float (&v)[4]) {
+  v[0] = __uint_as_float(r.v.x << 16); v[1] = __uint_as_float(r.v.x & 0xffff0000u);
+  v[2] = __uint_as_float(r.v.y << 16); v[3] = __uint_as_float(r.v.y & 0xffff0000u);
+}
+__device__ __forceinline__ void put4(float* p, bool wide, int n, const float (&v)[4]) {
+  if (wide) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); return; }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) if (i < n) p[i] = v[i];
+}
+__device__ __forceinline__ void put4(__nv_bfloat16* p, bool wide, int n, const float (&v)[4]) {
+  if (wide) { *reinterpret_cast<uint2*>(p) = make_uint2(umma::pack_bf16(v[0], v[1]), umma::pack_bf16(v[2], v[3])); return; }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) if (i < n) p[i] = __float2bfloat16_rn(v[i]);
+}
+
+struct Place { int b, seg, g, d, n; };               // batch row, part, group, first channel (of all), channels from there on (<= 0: none)
+template <class S> __device__ __forceinline__ Place place(const SelGeo& q, int c) {
   const int nblk = q.G * q.nb;
   Place p;
   const int blk = blockIdx.x % nblk, rest = blockIdx.x / nblk;
   p.seg = rest % q.segs; p.b = rest / q.segs;
   p.g = blk / q.nb;
-  const int cg = (blk - p.g * q.nb) * Sh<LPC>::CHB + c;
-  p.c = c; p.live = cg < q.Dg; p.d = p.g * q.Dg + (p.live ? cg : 0);
+  const int cg = (blk - p.g * q.nb) * S::CHB + c;
+  p.n = q.Dg - cg; p.d = p.g * q.Dg + (p.n > 0 ? cg : 0);
   return p;
 }
 
-// Four states of a [.., D, N] fp32 array (N not padded).
-template <int LPC> __device__ __forceinline__ void load_state(const float* p, int N, int nl, bool live, float (&v)[4]) {
+// KS states of a [.., D, N] fp32 array (N not padded) at `p`, in the order (j ^ m).
+template <class S> __device__ __forceinline__ void load_state(const float* p, int N, int nl, bool live, int m, f32x2 (&v)[S::KP]) {
+  float f[S::KS];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = live && p && nl * 4 + j < N ? p[nl * 4 + j] : 0.f;
+  for (int j = 0; j < S::KS; ++j) {
+    const int n = nl * S::KS + (j ^ m);
+    f[j] = live && p && n < N ? p[n] : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < S::KP; ++k) v[k] = pack2(f[2 * k], f[2 * k + 1]);
 }
-template <int LPC> __device__ __forceinline__ void store_state(float* p, int N, int nl, bool live, const float (&v)[4]) {
+template <class S> __device__ __forceinline__ void store_state(float* p, int N, int nl, bool live, int m, const f32x2 (&v)[S::KP]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) if (live && nl * 4 + j < N) p[nl * 4 + j] = v[j];
+  for (int k = 0; k < S::KP; ++k) {
+    float f[2];
+    unpack2(v[k], f[0], f[1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int n = nl * S::KS + ((2 * k + i) ^ m);
+      if (live && n < N) p[n] = f[i];
+    }
+  }
+}
+// KS states of a padded array of our own, natural order
+template <class S> __device__ __forceinline__ void load_padded(const float* p, f32x2 (&v)[S::KP]) {
+#pragma unroll
+  for (int k = 0; k < S::KS / 4; ++k) {
+    const float4 f = *reinterpret_cast<const float4*>(p + 4 * k);
+    v[2 * k] = pack2(f.x, f.y); v[2 * k + 1] = pack2(f.z, f.w);
+  }
+}
+template <class S> __device__ __forceinline__ void store_padded(float* p, const f32x2 (&v)[S::KP]) {
+#pragma unroll
+  for (int k = 0; k < S::KS / 4; ++k) {
+    float4 f;
+    unpack2(v[2 * k], f.x, f.y); unpack2(v[2 * k + 1], f.z, f.w);
+    *reinterpret_cast<float4*>(p + 4 * k) = f;
+  }
+}
+// natural order -> order (j ^ m), m uniform over nothing: one exchange of halves per bit
+template <class S> __device__ __forceinline__ void permute(f32x2 (&v)[S::KP], int m) {
+  float f[S::KS];
+#pragma unroll
+  for (int k = 0; k < S::KP; ++k) unpack2(v[k], f[2 * k], f[2 * k + 1]);
+#pragma unroll
+  for (int bit = 1; bit < S::KS; bit <<= 1) {
+    const bool swap = m & bit;
+#pragma unroll
+    for (int j = 0; j < S::KS; ++j)
+      if (!(j & bit)) {
+        const float a = f[j], b = f[j | bit];
+        f[j] = swap ? b : a; f[j | bit] = swap ? a : b;
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < S::KP; ++k) v[k] = pack2(f[2 * k], f[2 * k + 1]);
 }
 
 struct SelFwd {
@@ -104,157 +211,169 @@ struct SelFwd {
   const float *A, *D, *bias, *init;
   const int* lengths;
   void* y;
-  float *fin, *ckpt;                  // ckpt [B][nt][D][NP]: the state entering every tile
+  float *fin, *ckpt;                  // ckpt [B][nc][D][NP]: the state before every SEL_C-th token
   float *segst, *segdt;               // [B][segs][D][NP] states of the parts from zero, [B][segs][D] their summed steps
 };
 
 // MODE 0: outputs (and the states kept for the backward); MODE 1: a part's own state from zero and its summed steps.
-template <typename T, int LPC, int MODE>
-__global__ void __launch_bounds__(Sh<LPC>::TH) k_sel_fwd(SelGeo q, SelFwd p) {
-  using S = Sh<LPC>;
-  constexpr int NP = S::NP, CHB = S::CHB, TH = S::TH, IT = S::IT, BI = S::BI;
-  __shared__ float2 s_dt[2][SEL_T][CHB];             // step, step * x
-  __shared__ __align__(16) float s_B[2][SEL_T][NP], s_C[2][SEL_T][NP];
-  __shared__ float s_y[SEL_T][CHB];
+template <typename T, class S, int MODE>
+__global__ void __launch_bounds__(S::TH, S::TH == 128 ? 4 : 1) k_sel_fwd(SelGeo q, SelFwd p) {
+  constexpr int KS = S::KS, LPC = S::LPC, KP = S::KP, NP = S::NP, CHB = S::CHB, TH = S::TH, IT = S::IT, BI = S::BI;
+  __shared__ __align__(16) float2 s_dt[SEL_T][CHB];  // step, step * x
+  __shared__ __align__(16) float s_B[SEL_T][NP], s_C[SEL_T][NP], s_y[SEL_T][CHB];
   pdl_wait();
-  const int tid = threadIdx.x, c = tid / LPC, nl = tid % LPC;
-  const Place me = place<LPC>(q, c), it = place<LPC>(q, tid % CHB);   // roles: states of a channel; (token, channel) items
+  const int tid = threadIdx.x, c = tid / LPC, nl = tid % LPC, qc = tid % S::QR * 4, r0 = tid / S::QR;
+  const bool tasks = r0 < SEL_T;
+  const Place me = place<S>(q, c), it = place<S>(q, qc);
   if (MODE == 1 && me.seg == q.segs - 1) return;
+  const bool live = me.n > 0, wide = q.wide;
   const int len = p.lengths ? min(max(p.lengths[me.b], 0), q.L) : q.L;
-  const int t_begin = me.seg * q.seg_len, t_end = min(t_begin + q.seg_len, q.L);
-  const int r0 = tid / CHB;
+  const int t_begin = me.seg * q.seg_len, t_end = min(t_begin + q.seg_len, q.L), t_live = min(t_end, len);
   const T* xp = (const T*)p.x + (long long)it.b * q.xsb + it.d;
   const T* dtp = (const T*)p.dt + (long long)it.b * q.dtsb + it.d;
   const T* zp = (const T*)p.z + (long long)it.b * q.zsb + it.d;
   const T* bp = (const T*)p.Bm + (long long)it.b * q.bsb + (long long)it.g * q.N;
   const T* cp = (const T*)p.Cm + (long long)it.b * q.csb + (long long)it.g * q.N;
   T* yp = (T*)p.y + (long long)it.b * q.ysb + it.d;
-  const float bias = p.bias ? p.bias[it.d] : 0.f, Dv = p.D ? p.D[it.d] : 0.f;
-  const bool want_y = MODE == 0 && p.y;
+  const bool want_y = MODE == 0 && p.y, gated = want_y && p.z;
+  float bias[4], Dv[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    bias[k] = p.bias && k < it.n ? p.bias[it.d + k] : 0.f;
+    Dv[k] = p.D && k < it.n ? p.D[it.d + k] : 0.f;
+  }
 
-  float A4[4], h4[4];
-  load_state<LPC>(p.A + (long long)me.d * q.N, q.N, nl, me.live, A4);
-  const f32x2 A01 = pack2(A4[0] * LOG2E, A4[1] * LOG2E), A23 = pack2(A4[2] * LOG2E, A4[3] * LOG2E);
-  f32x2 h01 = 0ull, h23 = 0ull;
+  f32x2 A[KP], h[KP];
+  load_state<S>(p.A + (long long)me.d * q.N, q.N, nl, live, 0, A);
+#pragma unroll
+  for (int k = 0; k < KP; ++k) { A[k] = mul2(A[k], dup2(LOG2E)); h[k] = 0ull; }
   float dtsum = 0.f;
   if (MODE == 0) {
-    load_state<LPC>(p.init ? p.init + ((long long)me.b * q.D + me.d) * q.N : nullptr, q.N, nl, me.live, h4);
-    h01 = pack2(h4[0], h4[1]); h23 = pack2(h4[2], h4[3]);
+    load_state<S>(p.init ? p.init + ((long long)me.b * q.D + me.d) * q.N : nullptr, q.N, nl, live, 0, h);
     for (int s = 0; s < me.seg; ++s) {
       const long long at = ((long long)me.b * q.segs + s) * q.D + me.d;
-      const float4 v = *reinterpret_cast<const float4*>(p.segst + at * NP + nl * 4);
+      f32x2 v[KP];
+      load_padded<S>(p.segst + at * NP + nl * KS, v);
       const f32x2 d2 = dup2(p.segdt[at]);
-      h01 = fma2(decay2(A01, d2), h01, pack2(v.x, v.y));
-      h23 = fma2(decay2(A23, d2), h23, pack2(v.z, v.w));
+#pragma unroll
+      for (int k = 0; k < KP; ++k) h[k] = fma2(decay2(A[k], d2), h[k], v[k]);
     }
   }
 
-  T rx[IT], rd[IT], rz[IT], rb[BI], rc[BI];
+  Raw4<T> rx[IT], rd[IT], rz[IT];
+  T rb[BI], rc[BI];
   auto request = [&](int t0) {                       // values of a tile into registers; nothing past the end is read
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int t = t0 + r0 + i * S::RS;
-      const bool ok = it.live && t < len && t < t_end;
-      rx[i] = rd[i] = rz[i] = T(0.f);
-      if (ok) {
-        rx[i] = xp[(long long)t * q.xsl]; rd[i] = dtp[(long long)t * q.dtsl];
-        if (want_y && p.z) rz[i] = zp[(long long)t * q.zsl];
+      zero4(rx[i]); zero4(rd[i]); zero4(rz[i]);
+      if (tasks && it.n > 0 && t < t_live) {
+        load4(xp + (long long)t * q.xsl, wide, it.n, rx[i]);
+        load4(dtp + (long long)t * q.dtsl, wide, it.n, rd[i]);
+        if (gated) load4(zp + (long long)t * q.zsl, wide, it.n, rz[i]);
       }
     }
 #pragma unroll
     for (int i = 0; i < BI; ++i) {
       const int e = tid + i * TH, n = e % NP, t = t0 + e / NP;
-      const bool ok = n < q.N && t < len && t < t_end;
       rb[i] = rc[i] = T(0.f);
-      if (ok) {
+      if (n < q.N && t < t_live && e < SEL_T * NP) {
         rb[i] = bp[(long long)t * q.bsl + n];
         if (want_y) rc[i] = cp[(long long)t * q.csl + n];
       }
     }
   };
-  float kx[IT], kz[IT];
-  auto hand_over = [&](int t0, int buf) {
+  request(t_begin);
+  for (int t0 = t_begin; t0 < t_end; t0 += SEL_T) {
+    float x[IT][4];
+    Raw4<T> kz[IT];
+    // hand over: step sizes, B and C of this tile
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int t = t0 + r0 + i * S::RS;
-      kx[i] = (float)rx[i]; kz[i] = (float)rz[i];
-      const float s = it.live && t < len && t < t_end ? sel_step((float)rd[i], bias, q.softplus) : 0.f;
-      s_dt[buf][r0 + i * S::RS][tid % CHB] = make_float2(s, s * kx[i]);
+      const int r = r0 + i * S::RS, t = t0 + r;
+      float d[4], s[4];
+      values4(rx[i], x[i]); values4(rd[i], d);
+      kz[i] = rz[i];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k] = t < t_live ? sel_step(d[k], bias[k], q.softplus) : 0.f;
+      if (tasks) {
+        float4* w = reinterpret_cast<float4*>(&s_dt[r][qc]);
+        w[0] = make_float4(s[0], s[0] * x[i][0], s[1], s[1] * x[i][1]);
+        w[1] = make_float4(s[2], s[2] * x[i][2], s[3], s[3] * x[i][3]);
+      }
     }
 #pragma unroll
     for (int i = 0; i < BI; ++i) {
       const int e = tid + i * TH;
-      s_B[buf][e / NP][e % NP] = (float)rb[i];
-      if (want_y) s_C[buf][e / NP][e % NP] = (float)rc[i];
-    }
-  };
-
-  request(t_begin);
-  hand_over(t_begin, 0);
-  __syncthreads();
-  int buf = 0;
-  for (int t0 = t_begin; t0 < t_end; t0 += SEL_T, buf ^= 1) {
-    const bool more = t0 + SEL_T < t_end;
-    float ex[IT], ez[IT];
-#pragma unroll
-    for (int i = 0; i < IT; ++i) { ex[i] = kx[i]; ez[i] = kz[i]; }
-    if (more) request(t0 + SEL_T);
-    if (MODE == 0 && p.ckpt && me.live) {
-      float4 v;
-      unpack2(h01, v.x, v.y); unpack2(h23, v.z, v.w);
-      *reinterpret_cast<float4*>(p.ckpt + (((long long)me.b * q.nt + t0 / SEL_T) * q.D + me.d) * NP + nl * 4) = v;
-    }
-    if (t0 < len) {
-#pragma unroll
-      for (int u = 0; u < SEL_T; u += LPC) {
-        float v[LPC];
-#pragma unroll
-        for (int i = 0; i < LPC; ++i) {
-          const float2 sd = s_dt[buf][u + i][c];
-          const float4 b4 = *reinterpret_cast<const float4*>(&s_B[buf][u + i][nl * 4]);
-          const f32x2 s2 = dup2(sd.x), x2 = dup2(sd.y);
-          h01 = fma2(decay2(A01, s2), h01, mul2(pack2(b4.x, b4.y), x2));
-          h23 = fma2(decay2(A23, s2), h23, mul2(pack2(b4.z, b4.w), x2));
-          if (MODE == 1) dtsum += sd.x;
-          if (MODE == 0) {
-            const float4 c4 = *reinterpret_cast<const float4*>(&s_C[buf][u + i][nl * 4]);
-            v[i] = hsum(fma2(pack2(c4.z, c4.w), h23, mul2(pack2(c4.x, c4.y), h01)));
-          }
-        }
-        if (MODE == 0 && want_y) {
-          int k;
-          const float sum = fold_rows<LPC, LPC>(v, nl, k);
-          s_y[u + k][c] = sum;
-        }
+      if (e < SEL_T * NP) {
+        s_B[e / NP][e % NP] = (float)rb[i];
+        if (want_y) s_C[e / NP][e % NP] = (float)rc[i];
       }
     }
     __syncthreads();
-    if (want_y && it.live) {
+    if (t0 + SEL_T < t_end) request(t0 + SEL_T);
+    const bool work = t0 < len;
+#pragma unroll
+    for (int u = 0; u < SEL_T; u += LPC) {
+      if (MODE == 0 && u % SEL_C == 0 && p.ckpt && live && t0 + u < t_end)
+        store_padded<S>(p.ckpt + (((long long)me.b * q.nc + (t0 + u) / SEL_C) * q.D + me.d) * NP + nl * KS, h);
+      if (!work) continue;
+      float v[LPC];
+#pragma unroll
+      for (int i = 0; i < LPC; ++i) {
+        const float2 sd = s_dt[u + i][c];
+        const f32x2 s2 = dup2(sd.x), x2 = dup2(sd.y);
+        f32x2 acc = 0ull;
+#pragma unroll
+        for (int k = 0; k < KP; k += 2) {
+          const float4 b4 = *reinterpret_cast<const float4*>(&s_B[u + i][nl * KS + 2 * k]);
+          h[k] = fma2(decay2(A[k], s2), h[k], mul2(pack2(b4.x, b4.y), x2));
+          h[k + 1] = fma2(decay2(A[k + 1], s2), h[k + 1], mul2(pack2(b4.z, b4.w), x2));
+          if (MODE == 0) {
+            const float4 c4 = *reinterpret_cast<const float4*>(&s_C[u + i][nl * KS + 2 * k]);
+            acc = k ? fma2(pack2(c4.x, c4.y), h[k], acc) : mul2(pack2(c4.x, c4.y), h[k]);
+            acc = fma2(pack2(c4.z, c4.w), h[k + 1], acc);
+          }
+        }
+        if (MODE == 1) dtsum += sd.x;
+        v[i] = hsum(acc);
+      }
+      if (want_y) {
+        int k;
+        const float sum = fold_rows<LPC, LPC>(v, nl, k);
+        s_y[u + k][c] = sum;
+      }
+    }
+    __syncthreads();
+    if (want_y && tasks && it.n > 0) {
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
         const int r = r0 + i * S::RS, t = t0 + r;
-        if (t < t_end) {
-          float o = 0.f;
-          if (t < len) {
-            o = fmaf(Dv, ex[i], s_y[r][tid % CHB]);
-            if (p.z) o *= ez[i] * sig(ez[i]);
+        if (t >= t_end) continue;
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+        if (t < len) {
+          const float4 y4 = *reinterpret_cast<const float4*>(&s_y[r][qc]);
+          o[0] = fmaf(Dv[0], x[i][0], y4.x); o[1] = fmaf(Dv[1], x[i][1], y4.y);
+          o[2] = fmaf(Dv[2], x[i][2], y4.z); o[3] = fmaf(Dv[3], x[i][3], y4.w);
+          if (gated) {
+            float z[4];
+            values4(kz[i], z);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] *= z[k] * sig(z[k]);
           }
-          stf(yp + (long long)t * q.ysl, o);
         }
+        put4(yp + (long long)t * q.ysl, wide, it.n, o);
       }
     }
-    if (more) hand_over(t0 + SEL_T, buf ^ 1);
-    __syncthreads();
   }
-  unpack2(h01, h4[0], h4[1]); unpack2(h23, h4[2], h4[3]);
   if (MODE == 1) {
     const long long at = ((long long)me.b * q.segs + me.seg) * q.D + me.d;
-    if (me.live) {
-      *reinterpret_cast<float4*>(p.segst + at * NP + nl * 4) = make_float4(h4[0], h4[1], h4[2], h4[3]);
+    if (live) {
+      store_padded<S>(p.segst + at * NP + nl * KS, h);
       if (nl == 0) p.segdt[at] = dtsum;
     }
   } else if (p.fin && me.seg == q.segs - 1) {
-    store_state<LPC>(p.fin + ((long long)me.b * q.D + me.d) * q.N, q.N, nl, me.live, h4);
+    store_state<S>(p.fin + ((long long)me.b * q.D + me.d) * q.N, q.N, nl, live, 0, h);
   }
 }
 
@@ -262,10 +381,10 @@ __global__ void __launch_bounds__(Sh<LPC>::TH) k_sel_fwd(SelGeo q, SelFwd p) {
 // Backward, with g_t = dL/dh_t = C_t dy'_t + a_{t+1} g_{t+1} and dy' = dy silu(z):
 //     dB_t = sum_d g_t s x,   dC_t = sum_d dy' h_t,   dx = s (g.B) + D dy',   ds = x (g.B) + sum_n g_t a_t h_{t-1} A,
 //     dA = sum_t g_t a_t h_{t-1} s.
-// Per tile of 16 tokens the states and decays are computed again from the state kept at the tile's start and stay in registers
-// (so an exponential is computed once here, as in the forward), then the tile is walked backwards.  Sums over the states go over the
-// lanes of a channel, sums over the channels over the lanes and warps of a block; blocks leave partial sums of dB and dC which a
-// second kernel adds in order.
+// Eight tokens at a time the states and decays are computed again from the state kept before them and stay in registers (an
+// exponential is computed once here, as in the forward), then the eight are walked backwards.  Sums over the states go over the lanes
+// of a channel, sums over the channels over the lanes and warps of a block; blocks leave partial sums of dB and dC which a second
+// kernel adds in order.
 struct SelBwd {
   const void *x, *dt, *Bm, *Cm, *z, *dy;
   const float *A, *D, *bias, *dfin, *ckpt;
@@ -276,106 +395,155 @@ struct SelBwd {
 };
 
 // A part's own gradient of the state before it, from zero.
-template <typename T, int LPC>
-__global__ void __launch_bounds__(Sh<LPC>::TH) k_sel_bwd_part(SelGeo q, SelBwd p) {
-  using S = Sh<LPC>;
-  constexpr int NP = S::NP, CHB = S::CHB, TH = S::TH, IT = S::IT, BI = S::BI;
-  __shared__ float2 s_dt[SEL_T][CHB];                // step, dy'
+template <typename T, class S>
+__global__ void __launch_bounds__(S::TH) k_sel_bwd_part(SelGeo q, SelBwd p) {
+  constexpr int KS = S::KS, LPC = S::LPC, KP = S::KP, NP = S::NP, CHB = S::CHB, TH = S::TH, IT = S::IT, BI = S::BI;
+  __shared__ __align__(16) float2 s_dt[SEL_T][CHB];  // step, dy'
   __shared__ __align__(16) float s_C[SEL_T][NP];
   pdl_wait();
-  const int tid = threadIdx.x, c = tid / LPC, nl = tid % LPC;
-  const Place me = place<LPC>(q, c), it = place<LPC>(q, tid % CHB);
+  const int tid = threadIdx.x, c = tid / LPC, nl = tid % LPC, qc = tid % S::QR * 4, r0 = tid / S::QR;
+  const bool tasks = r0 < SEL_T;
+  const Place me = place<S>(q, c), it = place<S>(q, qc);
   if (me.seg == 0) return;
+  const bool live = me.n > 0, wide = q.wide;
   const int len = p.lengths ? min(max(p.lengths[me.b], 0), q.L) : q.L;
-  const int t_begin = me.seg * q.seg_len, t_end = min(t_begin + q.seg_len, q.L);
-  const int r0 = tid / CHB;
+  const int t_begin = me.seg * q.seg_len, t_end = min(t_begin + q.seg_len, q.L), t_live = min(t_end, len);
   const T* dtp = (const T*)p.dt + (long long)it.b * q.dtsb + it.d;
   const T* zp = (const T*)p.z + (long long)it.b * q.zsb + it.d;
   const T* dyp = (const T*)p.dy + (long long)it.b * q.ysb + it.d;
   const T* cp = (const T*)p.Cm + (long long)it.b * q.csb + (long long)it.g * q.N;
-  const float bias = p.bias ? p.bias[it.d] : 0.f;
-  float A4[4];
-  load_state<LPC>(p.A + (long long)me.d * q.N, q.N, nl, me.live, A4);
-  const f32x2 A01 = pack2(A4[0] * LOG2E, A4[1] * LOG2E), A23 = pack2(A4[2] * LOG2E, A4[3] * LOG2E);
-  f32x2 g01 = 0ull, g23 = 0ull;
+  float bias[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) bias[k] = p.bias && k < it.n ? p.bias[it.d + k] : 0.f;
+  f32x2 A[KP], g[KP];
+  load_state<S>(p.A + (long long)me.d * q.N, q.N, nl, live, 0, A);
+#pragma unroll
+  for (int k = 0; k < KP; ++k) { A[k] = mul2(A[k], dup2(LOG2E)); g[k] = 0ull; }
   float dtsum = 0.f;
-  for (int t0 = t_begin + (t_end - t_begin - 1) / SEL_T * SEL_T; t0 >= t_begin; t0 -= SEL_T) {
-    __syncthreads();
+  Raw4<T> rd[IT], ry[IT], rz[IT];
+  T rc[BI];
+  auto request = [&](int t0) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int r = r0 + i * S::RS, t = t0 + r;
-      float s = 0.f, g = 0.f;
-      if (it.live && t < len && t < t_end) {
-        s = sel_step((float)dtp[(long long)t * q.dtsl], bias, q.softplus);
-        g = (float)dyp[(long long)t * q.ysl];
-        if (p.z) { const float z = (float)zp[(long long)t * q.zsl]; g *= z * sig(z); }
+      const int t = t0 + r0 + i * S::RS;
+      zero4(rd[i]); zero4(ry[i]); zero4(rz[i]);
+      if (tasks && it.n > 0 && t < t_live) {
+        load4(dtp + (long long)t * q.dtsl, wide, it.n, rd[i]);
+        load4(dyp + (long long)t * q.ysl, wide, it.n, ry[i]);
+        if (p.z) load4(zp + (long long)t * q.zsl, wide, it.n, rz[i]);
       }
-      s_dt[r][tid % CHB] = make_float2(s, g);
     }
 #pragma unroll
     for (int i = 0; i < BI; ++i) {
       const int e = tid + i * TH, n = e % NP, t = t0 + e / NP;
-      s_C[e / NP][n] = n < q.N && t < len && t < t_end ? (float)cp[(long long)t * q.csl + n] : 0.f;
+      rc[i] = T(0.f);
+      if (n < q.N && t < t_live && e < SEL_T * NP) rc[i] = cp[(long long)t * q.csl + n];
+    }
+  };
+  const int t_last = t_begin + (t_end - t_begin - 1) / SEL_T * SEL_T;
+  request(t_last);
+  for (int t0 = t_last; t0 >= t_begin; t0 -= SEL_T) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int r = r0 + i * S::RS, t = t0 + r;
+      float d[4], y[4], z[4];
+      values4(rd[i], d); values4(ry[i], y); values4(rz[i], z);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        d[k] = t < t_live ? sel_step(d[k], bias[k], q.softplus) : 0.f;
+        if (p.z) y[k] *= z[k] * sig(z[k]);
+      }
+      if (tasks) {
+        float4* w = reinterpret_cast<float4*>(&s_dt[r][qc]);
+        w[0] = make_float4(d[0], y[0], d[1], y[1]);
+        w[1] = make_float4(d[2], y[2], d[3], y[3]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < BI; ++i) {
+      const int e = tid + i * TH;
+      if (e < SEL_T * NP) s_C[e / NP][e % NP] = (float)rc[i];
     }
     __syncthreads();
+    if (t0 > t_begin) request(t0 - SEL_T);
+    if (t0 < len) {
 #pragma unroll
-    for (int r = SEL_T - 1; r >= 0; --r) {
-      const float2 sd = s_dt[r][c];
-      const float4 c4 = *reinterpret_cast<const float4*>(&s_C[r][nl * 4]);
-      const f32x2 s2 = dup2(sd.x), y2 = dup2(sd.y);
-      g01 = mul2(decay2(A01, s2), fma2(pack2(c4.x, c4.y), y2, g01));
-      g23 = mul2(decay2(A23, s2), fma2(pack2(c4.z, c4.w), y2, g23));
-      dtsum += sd.x;
+      for (int r = SEL_T - 1; r >= 0; --r) {
+        const float2 sd = s_dt[r][c];
+        const f32x2 s2 = dup2(sd.x), y2 = dup2(sd.y);
+#pragma unroll
+        for (int k = 0; k < KP; k += 2) {
+          const float4 c4 = *reinterpret_cast<const float4*>(&s_C[r][nl * KS + 2 * k]);
+          g[k] = mul2(decay2(A[k], s2), fma2(pack2(c4.x, c4.y), y2, g[k]));
+          g[k + 1] = mul2(decay2(A[k + 1], s2), fma2(pack2(c4.z, c4.w), y2, g[k + 1]));
+        }
+        dtsum += sd.x;
+      }
     }
+    __syncthreads();
   }
   const long long at = ((long long)me.b * q.segs + me.seg) * q.D + me.d;
-  if (me.live) {
-    float4 v;
-    unpack2(g01, v.x, v.y); unpack2(g23, v.z, v.w);
-    *reinterpret_cast<float4*>(p.segst + at * NP + nl * 4) = v;
+  if (live) {
+    store_padded<S>(p.segst + at * NP + nl * KS, g);
     if (nl == 0) p.segdt[at] = dtsum;
   }
 }
 
-// Sums of R values over the CPW lane groups of a warp that hold other channels (lane = channel * LPC + nl): every exchange folds
-// two values into one; a lane ends up with the sums of `left` values, the first of them value `u`.
-template <int LPC, int R> struct ChannelFold {
-  static constexpr int CPW = 32 / LPC;
-  static constexpr int left = R > CPW ? R / CPW : 1;
-  __device__ static __forceinline__ void run(float (&v)[R], int lane, int& u) {
-    u = 0;
+// Sums over the channels of a warp (lane = channel * LPC + nl) of a token's contributions to dB and dC, KS states each.  Every
+// exchange folds two values into one: the lanes of a pair keep one half of the states each and give the other.  Which half a lane
+// keeps follows from a bit of its channel; its registers hold the states in the order (j ^ m), m the lane's bits, so that the half to
+// keep is the same registers in every lane and no selects are needed (they were a quarter of the backward's instructions).
+// A lane ends up with V values: state v ^ m of dB and of dC, or, with one value, that of `kind`.
+template <class S> struct ChannelSum {
+  static constexpr int CPW = S::CPW, KS = S::KS;
+  static constexpr int V = CPW >= KS ? 1 : KS / CPW;             // states left per kind
+  static constexpr bool ONE = CPW >= 2 * KS;                     // and one kind
+  __device__ static __forceinline__ int order(int lane) {        // m
+    int m = 0, o = 16;
+#pragma unroll
+    for (int h = KS / 2; h > 0 && o >= S::LPC; h >>= 1, o >>= 1) if (lane & o) m |= h;
+    return m;
+  }
+  // b, c: the 2 KS values; afterwards b[0..V-1], c[0..V-1] (ONE: b[0], kind returned)
+  __device__ static __forceinline__ int run(float (&b)[KS], float (&c)[KS], int lane) {
     int o = 16;
 #pragma unroll
-    for (int n = R; n > 1; n >>= 1, o >>= 1) {
-      if (o < LPC) break;
-      const bool up = lane & o;
+    for (int h = KS / 2; h > 0 && o >= S::LPC; h >>= 1, o >>= 1) {
 #pragma unroll
-      for (int i = 0; i < n / 2; ++i) {
-        const float keep = up ? v[n / 2 + i] : v[i], give = up ? v[i] : v[n / 2 + i];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      for (int j = 0; j < h; ++j) {
+        b[j] += __shfl_xor_sync(0xffffffffu, b[j + h], o);
+        c[j] += __shfl_xor_sync(0xffffffffu, c[j + h], o);
       }
-      u += up ? n / 2 : 0;
     }
+    int kind = 0;
+    if (ONE) {
+      const bool up = lane & o;
+      const float keep = up ? c[0] : b[0], give = up ? b[0] : c[0];
+      b[0] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      kind = up;
 #pragma unroll
-    for (; o >= LPC && CPW > R; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+      for (o >>= 1; o >= S::LPC; o >>= 1) b[0] += __shfl_xor_sync(0xffffffffu, b[0], o);
+    }
+    return kind;
   }
 };
 
-template <typename T, int LPC, bool GATED>
-__global__ void __launch_bounds__(Sh<LPC>::TH) k_sel_bwd(SelGeo q, SelBwd p) {
-  using S = Sh<LPC>;
-  constexpr int NP = S::NP, CHB = S::CHB, TH = S::TH, IT = S::IT, BI = S::BI, W = S::W;
-  __shared__ __align__(16) float s_B[SEL_T][NP], s_C[SEL_T][NP];
-  __shared__ float s_1[SEL_T][CHB], s_2[SEL_T][CHB], s_3[GATED ? SEL_T : 1][CHB];
-  extern __shared__ __align__(16) float4 sel_smem[];
-  float4 (*s_v)[CHB] = reinterpret_cast<float4 (*)[CHB]>(sel_smem);    // step, step * x, dy', -
-  float (*s_bc)[SEL_T][2 * NP] = reinterpret_cast<float (*)[SEL_T][2 * NP]>(sel_smem + SEL_T * CHB);
+template <typename T, class S, bool GATED>
+__global__ void __launch_bounds__(S::TH, S::TH == 128 ? 3 : 1) k_sel_bwd(SelGeo q, SelBwd p) {
+  constexpr int KS = S::KS, LPC = S::LPC, KP = S::KP, NP = S::NP, CHB = S::CHB, TH = S::TH, IT = S::IT, BI = S::BI, W = S::W, CO = S::COPIES;
+  extern __shared__ __align__(16) float sel_smem[];
+  float4 (*s_v)[CHB] = reinterpret_cast<float4 (*)[CHB]>(sel_smem);    // step, step * x, dy', d step / d raw
+  float (*s_B)[SEL_T][NP] = reinterpret_cast<float (*)[SEL_T][NP]>(sel_smem + SEL_T * CHB * 4);   // [order][token][states]
+  float (*s_C)[SEL_T][NP] = s_B + CO;
+  float (*s_bc)[SEL_T][2 * NP] = reinterpret_cast<float (*)[SEL_T][2 * NP]>(s_C + CO);            // [warp][token][dB | dC]
+  float (*s_1)[CHB] = reinterpret_cast<float (*)[CHB]>(s_bc + W), (*s_2)[CHB] = s_1 + SEL_T, (*s_3)[CHB] = s_2 + SEL_T;
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = tid / LPC, nl = tid % LPC;
-  const Place me = place<LPC>(q, c), it = place<LPC>(q, tid % CHB);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = tid / LPC, nl = tid % LPC, qc = tid % S::QR * 4, r0 = tid / S::QR;
+  const bool tasks = r0 < SEL_T;
+  const Place me = place<S>(q, c), it = place<S>(q, qc);
+  const bool live = me.n > 0, wide = q.wide;
   const int len = p.lengths ? min(max(p.lengths[me.b], 0), q.L) : q.L;
-  const int t_begin = me.seg * q.seg_len, t_end = min(t_begin + q.seg_len, q.L);
-  const int r0 = tid / CHB, ic = tid % CHB;
+  const int t_begin = me.seg * q.seg_len, t_end = min(t_begin + q.seg_len, q.L), t_live = min(t_end, len);
   const T* xp = (const T*)p.x + (long long)it.b * q.xsb + it.d;
   const T* dtp = (const T*)p.dt + (long long)it.b * q.dtsb + it.d;
   const T* zp = (const T*)p.z + (long long)it.b * q.zsb + it.d;
@@ -383,168 +551,223 @@ __global__ void __launch_bounds__(Sh<LPC>::TH) k_sel_bwd(SelGeo q, SelBwd p) {
   const T* bp = (const T*)p.Bm + (long long)it.b * q.bsb + (long long)it.g * q.N;
   const T* cp = (const T*)p.Cm + (long long)it.b * q.csb + (long long)it.g * q.N;
   const long long out0 = (long long)it.b * q.L * q.D + it.d;
-  const float bias = p.bias ? p.bias[it.d] : 0.f, Dv = p.D ? p.D[it.d] : 0.f;
-  const int blk = blockIdx.x % (q.G * q.nb);
+  float* bc0 = p.part_bc + ((long long)(blockIdx.x % (q.G * q.nb)) * q.B + me.b) * q.L * (2 * NP);
+  float bias[4], Dv[4], dD[4] = {}, dbias[4] = {};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    bias[k] = p.bias && k < it.n ? p.bias[it.d + k] : 0.f;
+    Dv[k] = p.D && k < it.n ? p.D[it.d + k] : 0.f;
+  }
+  const int m = ChannelSum<S>::order(lane);
 
-  float A4[4], g4[4];
-  load_state<LPC>(p.A + (long long)me.d * q.N, q.N, nl, me.live, A4);
-  const f32x2 A01 = pack2(A4[0] * LOG2E, A4[1] * LOG2E), A23 = pack2(A4[2] * LOG2E, A4[3] * LOG2E);
-  load_state<LPC>(p.dfin ? p.dfin + ((long long)me.b * q.D + me.d) * q.N : nullptr, q.N, nl, me.live, g4);
-  f32x2 g01 = pack2(g4[0], g4[1]), g23 = pack2(g4[2], g4[3]);    // a_{t+1} g_{t+1}
+  f32x2 A[KP], g[KP], dA[KP];                        // g: a_{t+1} g_{t+1}
+  load_state<S>(p.A + (long long)me.d * q.N, q.N, nl, live, m, A);
+  load_state<S>(p.dfin ? p.dfin + ((long long)me.b * q.D + me.d) * q.N : nullptr, q.N, nl, live, m, g);
+#pragma unroll
+  for (int k = 0; k < KP; ++k) { A[k] = mul2(A[k], dup2(LOG2E)); dA[k] = 0ull; }
   for (int s = q.segs - 1; s > me.seg; --s) {
     const long long at = ((long long)me.b * q.segs + s) * q.D + me.d;
-    const float4 v = *reinterpret_cast<const float4*>(p.segst + at * NP + nl * 4);
+    f32x2 v[KP];
+    load_padded<S>(p.segst + at * NP + nl * KS, v);
+    permute<S>(v, m);
     const f32x2 d2 = dup2(p.segdt[at]);
-    g01 = fma2(decay2(A01, d2), g01, pack2(v.x, v.y));
-    g23 = fma2(decay2(A23, d2), g23, pack2(v.z, v.w));
-  }
-  f32x2 dA01 = 0ull, dA23 = 0ull;
-  float dD = 0.f, dbias = 0.f;
-
-  for (int t0 = t_begin + (t_end - t_begin - 1) / SEL_T * SEL_T; t0 >= t_begin; t0 -= SEL_T) {
-    if (t0 >= len) {                                 // (uniform over the block) nothing here but zeros
-      if (it.live)
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
-          const int t = t0 + r0 + i * S::RS;
-          if (t < t_end) {
-            const long long o = out0 + (long long)t * q.D;
-            stf((T*)p.dx + o, 0.f); stf((T*)p.ddt + o, 0.f);
-            if (GATED) stf((T*)p.dz + o, 0.f);
-          }
-        }
-      for (int e = tid; e < SEL_T * 2 * NP; e += TH) {
-        const int t = t0 + e / (2 * NP);
-        if (t < t_end) p.part_bc[((long long)blk * q.B * q.L + (long long)me.b * q.L + t) * (2 * NP) + e % (2 * NP)] = 0.f;
-      }
-      continue;
-    }
-    float4 k4 = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (me.live) k4 = *reinterpret_cast<const float4*>(p.ckpt + (((long long)me.b * q.nt + t0 / SEL_T) * q.D + me.d) * NP + nl * 4);
-    float vx[IT], vs[IT], vd[IT], vy[IT], vz[IT];
+    for (int k = 0; k < KP; ++k) g[k] = fma2(decay2(A[k], d2), g[k], v[k]);
+  }
+
+  Raw4<T> rx[IT], rd[IT], ry[IT], rz[IT];
+  T rb[BI], rc[BI];
+  auto request = [&](int t0) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int r = r0 + i * S::RS, t = t0 + r;
-      vx[i] = vs[i] = vd[i] = vy[i] = vz[i] = 0.f;
-      float dy0 = 0.f;
-      if (it.live && t < len && t < t_end) {
-        vx[i] = (float)xp[(long long)t * q.xsl];
-        const float raw = (float)dtp[(long long)t * q.dtsl];
-        vs[i] = sel_step(raw, bias, q.softplus);
-        vd[i] = sel_dstep(raw, bias, q.softplus);
-        dy0 = vy[i] = (float)dyp[(long long)t * q.ysl];
-        if (GATED) { vz[i] = (float)zp[(long long)t * q.zsl]; dy0 *= vz[i] * sig(vz[i]); }
+      const int t = t0 + r0 + i * S::RS;
+      zero4(rx[i]); zero4(rd[i]); zero4(ry[i]); zero4(rz[i]);
+      if (tasks && it.n > 0 && t < t_live) {
+        load4(xp + (long long)t * q.xsl, wide, it.n, rx[i]);
+        load4(dtp + (long long)t * q.dtsl, wide, it.n, rd[i]);
+        load4(dyp + (long long)t * q.ysl, wide, it.n, ry[i]);
+        if (GATED) load4(zp + (long long)t * q.zsl, wide, it.n, rz[i]);
       }
-      s_v[r][ic] = make_float4(vs[i], vs[i] * vx[i], dy0, 0.f);
     }
 #pragma unroll
     for (int i = 0; i < BI; ++i) {
       const int e = tid + i * TH, n = e % NP, t = t0 + e / NP;
-      const bool ok = n < q.N && t < len && t < t_end;
-      s_B[e / NP][n] = ok ? (float)bp[(long long)t * q.bsl + n] : 0.f;
-      s_C[e / NP][n] = ok ? (float)cp[(long long)t * q.csl + n] : 0.f;
+      rb[i] = rc[i] = T(0.f);
+      if (n < q.N && t < t_live && e < SEL_T * NP) { rb[i] = bp[(long long)t * q.bsl + n]; rc[i] = cp[(long long)t * q.csl + n]; }
     }
-    __syncthreads();
-    f32x2 a01[SEL_T], a23[SEL_T], h01[SEL_T + 1], h23[SEL_T + 1];
-    h01[0] = pack2(k4.x, k4.y); h23[0] = pack2(k4.z, k4.w);
+  };
+  const float* ck0 = p.ckpt + ((long long)me.b * q.nc * q.D + me.d) * NP + nl * KS;
+  auto kept = [&](int t, f32x2 (&v)[KP]) {           // the state before token t
+    if (live && t < t_end) load_padded<S>(ck0 + (long long)(t / SEL_C) * q.D * NP, v);
+    else
 #pragma unroll
-    for (int r = 0; r < SEL_T; ++r) {
-      const float4 v = s_v[r][c];
-      const float4 b4 = *reinterpret_cast<const float4*>(&s_B[r][nl * 4]);
-      const f32x2 s2 = dup2(v.x), x2 = dup2(v.y);
-      a01[r] = decay2(A01, s2); a23[r] = decay2(A23, s2);
-      h01[r + 1] = fma2(a01[r], h01[r], mul2(pack2(b4.x, b4.y), x2));
-      h23[r + 1] = fma2(a23[r], h23[r], mul2(pack2(b4.z, b4.w), x2));
-    }
-    f32x2 tA01 = 0ull, tA23 = 0ull;                  // a tile's share of dA: sums of 16, then sums of tiles
+      for (int k = 0; k < KP; ++k) v[k] = 0ull;
+  };
+  const int t_last = t_begin + (t_end - t_begin - 1) / SEL_T * SEL_T;
+  request(t_last);
+  f32x2 first[KP];                                   // the state before the next eight tokens to be walked
+  kept(t_last + SEL_C, first);
+  for (int t0 = t_last; t0 >= t_begin; t0 -= SEL_T) {
+    Raw4<T> kx[IT], ky[IT], kz[IT];
 #pragma unroll
-    for (int u = SEL_T - LPC; u >= 0; u -= LPC) {
-      float v1[LPC], v2[LPC], v3[LPC];
+    for (int i = 0; i < IT; ++i) {
+      const int r = r0 + i * S::RS, t = t0 + r;
+      float x[4], d[4], y[4], z[4];
+      kx[i] = rx[i]; ky[i] = ry[i]; kz[i] = rz[i];
+      values4(rx[i], x); values4(rd[i], d); values4(ry[i], y); values4(rz[i], z);
 #pragma unroll
-      for (int i = LPC - 1; i >= 0; --i) {
-        const int r = u + i;
-        const float4 v = s_v[r][c];
-        const float4 b4 = *reinterpret_cast<const float4*>(&s_B[r][nl * 4]), c4 = *reinterpret_cast<const float4*>(&s_C[r][nl * 4]);
-        const f32x2 s2 = dup2(v.x), x2 = dup2(v.y), y2 = dup2(v.z);
-        const f32x2 C01 = pack2(c4.x, c4.y), C23 = pack2(c4.z, c4.w);
-        g01 = fma2(C01, y2, g01); g23 = fma2(C23, y2, g23);
-        float w[8];
-        const f32x2 e0 = mul2(g01, x2), e1 = mul2(g23, x2), e2 = mul2(h01[r + 1], y2), e3 = mul2(h23[r + 1], y2);
-        unpack2(e0, w[0], w[1]); unpack2(e1, w[2], w[3]); unpack2(e2, w[4], w[5]); unpack2(e3, w[6], w[7]);
-        v1[i] = hsum(fma2(pack2(b4.z, b4.w), g23, mul2(pack2(b4.x, b4.y), g01)));
-        if (GATED) v3[i] = hsum(fma2(C23, h23[r + 1], mul2(C01, h01[r + 1])));
-        g01 = mul2(g01, a01[r]); g23 = mul2(g23, a23[r]);
-        const f32x2 q01 = mul2(g01, h01[r]), q23 = mul2(g23, h23[r]);
-        v2[i] = hsum(fma2(A23, q23, mul2(A01, q01)));
-        tA01 = fma2(q01, s2, tA01); tA23 = fma2(q23, s2, tA23);
-        int k;
-        using F = ChannelFold<LPC, 8>;
-        F::run(w, lane, k);
-#pragma unroll
-        for (int j = 0; j < F::left; ++j) s_bc[warp][r][((k + j) >> 2) * NP + nl * 4 + ((k + j) & 3)] = w[j];
-      }
-      int k;
-      const float a = fold_rows<LPC, LPC>(v1, nl, k);
-      s_1[u + k][c] = a;
-      const float b = fold_rows<LPC, LPC>(v2, nl, k);
-      s_2[u + k][c] = b;
-      if (GATED) {
-        const float d = fold_rows<LPC, LPC>(v3, nl, k);
-        s_3[u + k][c] = d;
+      for (int k = 0; k < 4; ++k) {
+        float s = 0.f, ds = 0.f;
+        if (t < t_live) s = sel_step_d(d[k], bias[k], q.softplus, ds);
+        if (GATED) y[k] *= z[k] * sig(z[k]);
+        if (tasks) s_v[r][qc + k] = make_float4(s, s * x[k], y[k], ds);
       }
     }
-    dA01 = add2(dA01, tA01); dA23 = add2(dA23, tA23);
-    __syncthreads();
-    float tD = 0.f, tb = 0.f;
-    if (it.live)
 #pragma unroll
-      for (int i = 0; i < IT; ++i) {
-        const int r = r0 + i * S::RS, t = t0 + r;
-        if (t < t_end) {
-          const long long o = out0 + (long long)t * q.D;
-          float dx = 0.f, ddt = 0.f, dz = 0.f;
-          if (t < len) {
-            const float gB = s_1[r][ic];
-            float dy0 = vy[i];
-            if (GATED) {
-              const float sg = sig(vz[i]);
-              dz = vy[i] * fmaf(Dv, vx[i], s_3[r][ic]) * sg * fmaf(vz[i], 1.f - sg, 1.f);
-              dy0 *= vz[i] * sg;
-            }
-            dx = fmaf(vs[i], gB, Dv * dy0);
-            ddt = fmaf(vx[i], gB, s_2[r][ic] * LN2) * vd[i];
-            tD = fmaf(dy0, vx[i], tD); tb += ddt;
+    for (int i = 0; i < BI; ++i) {
+      const int e = tid + i * TH;
+      if (e < SEL_T * NP) {
+        const int r = e / NP, n = e % NP;
+#pragma unroll
+        for (int o = 0; o < CO; ++o) { const int oo = o * (KS / CO); s_B[o][r][n ^ oo] = (float)rb[i]; s_C[o][r][n ^ oo] = (float)rc[i]; }
+      }
+    }
+    f32x2 tA[KP] = {};                               // a tile's share of dA: sums of 16, then sums of tiles
+    __syncthreads();
+    if (t0 > t_begin) request(t0 - SEL_T);
+    if (t0 >= len) {
+      if (t0 > t_begin) kept(t0 - SEL_C, first);
+    } else {
+      const int co = m / (KS / CO);
+#pragma unroll 1
+      for (int half = 1; half >= 0; --half) {
+        f32x2 h[SEL_C + 1][KP];
+        permute<S>(first, m);
+#pragma unroll
+        for (int k = 0; k < KP; ++k) h[0][k] = first[k];
+        if (half) kept(t0, first);
+        else if (t0 > t_begin) kept(t0 - SEL_C, first);
+#pragma unroll
+        for (int i = 0; i < SEL_C; ++i) {
+          const int r = half * SEL_C + i;
+          const float2 v = *reinterpret_cast<const float2*>(&s_v[r][c]);
+          const f32x2 s2 = dup2(v.x), x2 = dup2(v.y);
+#pragma unroll
+          for (int k = 0; k < KP; k += 2) {
+            const float4 b4 = *reinterpret_cast<const float4*>(&s_B[co][r][nl * KS + 2 * k]);
+            h[i + 1][k] = fma2(decay2(A[k], s2), h[i][k], mul2(pack2(b4.x, b4.y), x2));
+            h[i + 1][k + 1] = fma2(decay2(A[k + 1], s2), h[i][k + 1], mul2(pack2(b4.z, b4.w), x2));
           }
-          stf((T*)p.dx + o, dx); stf((T*)p.ddt + o, ddt);
-          if (GATED) stf((T*)p.dz + o, dz);
+        }
+        constexpr int FR = LPC < SEL_C ? LPC : SEL_C;  // tokens whose sums over the states are folded together
+#pragma unroll
+        for (int u = SEL_C - FR; u >= 0; u -= FR) {
+          float v1[FR], v2[FR], v3[FR];
+#pragma unroll
+          for (int f = FR - 1; f >= 0; --f) {
+            const int i = u + f, r = half * SEL_C + i;
+            const float4 v = s_v[r][c];
+            const f32x2 s2 = dup2(v.x), x2 = dup2(v.y), y2 = dup2(v.z);
+            f32x2 a1 = 0ull, a2 = 0ull, a3 = 0ull;
+            float wb[KS], wc[KS];
+#pragma unroll
+            for (int k2 = 0; k2 < KP; k2 += 2) {
+              const float4 b4 = *reinterpret_cast<const float4*>(&s_B[co][r][nl * KS + 2 * k2]);
+              const float4 c4 = *reinterpret_cast<const float4*>(&s_C[co][r][nl * KS + 2 * k2]);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int k = k2 + e;
+                const f32x2 Bk = e ? pack2(b4.z, b4.w) : pack2(b4.x, b4.y), Ck = e ? pack2(c4.z, c4.w) : pack2(c4.x, c4.y);
+                g[k] = fma2(Ck, y2, g[k]);
+                unpack2(mul2(g[k], x2), wb[2 * k], wb[2 * k + 1]);
+                unpack2(mul2(h[i + 1][k], y2), wc[2 * k], wc[2 * k + 1]);
+                a1 = k ? fma2(Bk, g[k], a1) : mul2(Bk, g[k]);
+                if (GATED) a3 = k ? fma2(Ck, h[i + 1][k], a3) : mul2(Ck, h[i + 1][k]);
+                g[k] = mul2(g[k], decay2_again(A[k], s2));
+                const f32x2 qk = mul2(g[k], h[i][k]);
+                a2 = k ? fma2(A[k], qk, a2) : mul2(A[k], qk);
+                tA[k] = fma2(qk, s2, tA[k]);
+              }
+            }
+            v1[f] = hsum(a1); v2[f] = hsum(a2);
+            if (GATED) v3[f] = hsum(a3);
+            typedef ChannelSum<S> CS;
+            const int kind = CS::run(wb, wc, lane);
+            float* o = &s_bc[warp][r][nl * KS];
+            if (CS::ONE) o[kind * NP + m] = wb[0];
+            else
+#pragma unroll
+              for (int j = 0; j < CS::V; ++j) { o[j ^ m] = wb[j]; o[NP + (j ^ m)] = wc[j]; }
+          }
+          int k;
+          const float f1 = fold_rows<LPC, FR>(v1, nl, k);
+          const int r = half * SEL_C + u + k;
+          s_1[r][c] = f1;
+          s_2[r][c] = fold_rows<LPC, FR>(v2, nl, k);
+          if (GATED) s_3[r][c] = fold_rows<LPC, FR>(v3, nl, k);
         }
       }
-    dD += tD; dbias += tb;
-    for (int e = tid; e < SEL_T * 2 * NP; e += TH) {
-      const int r = e / (2 * NP), t = t0 + r;
-      float a = 0.f;
+    }
 #pragma unroll
-      for (int w = 0; w < W; ++w) a += s_bc[w][r][e % (2 * NP)];
-      if (t < t_end) p.part_bc[((long long)blk * q.B * q.L + (long long)me.b * q.L + t) * (2 * NP) + e % (2 * NP)] = a;
+    for (int k = 0; k < KP; ++k) dA[k] = add2(dA[k], tA[k]);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int r = r0 + i * S::RS, t = t0 + r;
+      if (!tasks || it.n <= 0 || t >= t_end) continue;
+      float dx[4] = {}, dd[4] = {}, dz[4] = {};
+      if (t < len) {
+        float x[4], y[4], z[4];
+        values4(kx[i], x); values4(ky[i], y); values4(kz[i], z);
+        const float4 f1 = *reinterpret_cast<const float4*>(&s_1[r][qc]), f2 = *reinterpret_cast<const float4*>(&s_2[r][qc]);
+        const float4 f3 = GATED ? *reinterpret_cast<const float4*>(&s_3[r][qc]) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float gB[4] = {f1.x, f1.y, f1.z, f1.w}, qA[4] = {f2.x, f2.y, f2.z, f2.w}, hC[4] = {f3.x, f3.y, f3.z, f3.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 v = s_v[r][qc + k];
+          if (GATED) {
+            const float sg = sig(z[k]);
+            dz[k] = y[k] * fmaf(Dv[k], x[k], hC[k]) * sg * fmaf(z[k], 1.f - sg, 1.f);
+          }
+          dx[k] = fmaf(v.x, gB[k], Dv[k] * v.z);
+          dd[k] = fmaf(x[k], gB[k], qA[k] * LN2) * v.w;
+          dD[k] = fmaf(v.z, x[k], dD[k]);
+          dbias[k] += dd[k];
+        }
+      }
+      const long long o = out0 + (long long)t * q.D;
+      put4((T*)p.dx + o, wide, it.n, dx); put4((T*)p.ddt + o, wide, it.n, dd);
+      if (GATED) put4((T*)p.dz + o, wide, it.n, dz);
+    }
+    for (int e = tid; e < SEL_T * 2 * NP / 4; e += TH) {
+      const int r = e / (NP / 2), n = e % (NP / 2) * 4, t = t0 + r;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (t < len)
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float4 f = *reinterpret_cast<const float4*>(&s_bc[w][r][n]);
+          v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
+        }
+      if (t < t_end) *reinterpret_cast<float4*>(bc0 + (long long)t * (2 * NP) + n) = v;
     }
     __syncthreads();
   }
-  unpack2(g01, g4[0], g4[1]); unpack2(g23, g4[2], g4[3]);
-  if (p.dinit && me.seg == 0) store_state<LPC>(p.dinit + ((long long)me.b * q.D + me.d) * q.N, q.N, nl, me.live, g4);
+  if (p.dinit && me.seg == 0) store_state<S>(p.dinit + ((long long)me.b * q.D + me.d) * q.N, q.N, nl, live, m, g);
   float* par = p.part_par + ((long long)me.b * q.segs + me.seg) * q.par_row;
-  if (me.live) {
-    float4 v;
-    unpack2(dA01, v.x, v.y); unpack2(dA23, v.z, v.w);
-    *reinterpret_cast<float4*>(par + (long long)me.d * NP + nl * 4) = v;
-  }
-  s_1[r0][ic] = dD; s_2[r0][ic] = dbias;             // the block's threads of a channel, in order
+  permute<S>(dA, m);                                 // (its own inverse)
+  if (live) store_padded<S>(par + (long long)me.d * NP + nl * KS, dA);
+  if (tasks)                                         // the threads of four channels, in order
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { s_1[r0][qc + k] = dD[k]; s_2[r0][qc + k] = dbias[k]; }
   __syncthreads();
-  if (tid < CHB && it.live) {
+  for (int e = tid; e < CHB; e += TH) {
+    const Place at = place<S>(q, e);
+    if (at.n <= 0) continue;
     float a = 0.f, b = 0.f;
 #pragma unroll
-    for (int r = 0; r < S::RS; ++r) { a += s_1[r][tid]; b += s_2[r][tid]; }
-    par[(long long)q.D * NP + it.d] = a;
-    par[(long long)q.D * (NP + 1) + it.d] = b;
+    for (int r = 0; r < S::RS; ++r) { a += s_1[r][e]; b += s_2[r][e]; }
+    par[(long long)q.D * NP + at.d] = a;
+    par[(long long)q.D * (NP + 1) + at.d] = b;
   }
 }
 
@@ -647,8 +870,22 @@ __global__ void __launch_bounds__(256) k_sel_step(SelStep q, SsdStepPtrs p) {
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
-int lanes_for(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
-int chb_for(int lpc) { return lpc <= 8 ? 32 : 16; }
+// Block shapes by the number of states (padded to 4, 8, 16, 32, 64): eight states per thread where there are as many, since what a
+// thread does per token and channel, the sums over lanes and the reads of B and C, is shared by its states.
+typedef Sh<4, 1, 64> Sh4;
+typedef Sh<8, 1, 64> Sh8;
+typedef Sh<8, 2, 64> Sh16;
+typedef Sh<8, 4, 32> Sh32;
+typedef Sh<8, 8, 16> Sh64;
+typedef Sh<4, 1, 64> Bh4;
+typedef Sh<4, 2, 64> Bh8;
+typedef Sh<4, 4, 32> Bh16;
+typedef Sh<4, 8, 16> Bh32;
+typedef Sh<8, 8, 16> Bh64;
+int block_channels_bwd(int NP) { return NP == 4 ? Bh4::CHB : NP == 8 ? Bh8::CHB : NP == 16 ? Bh16::CHB : NP == 32 ? Bh32::CHB : Bh64::CHB; }
+int padded_states(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
+int block_channels(int NP) { return NP <= 16 ? 64 : NP == 32 ? 32 : 16; }
+int lanes_for(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }   // single step: four states per thread
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 int check_common(const char* what, int channels, int dstate, int ngroups, int dtype, int device) {
@@ -671,9 +908,30 @@ int check_common(const char* what, int channels, int dstate, int ngroups, int dt
 
 struct SelPlan {
   SelGeo q;
-  int lpc, NP;
+  int NP, nb_bwd, segs_fwd, segs_bwd;
   size_t ckpt, segst, segdt, part_bc, part_par, fwd_bytes, bwd_bytes;   // offsets and totals
 };
+
+// Parts of the sequence.  n blocks walk the tokens one after the other, `fit` of them at a time on an SM; a lone block takes about half
+// as long for a tile as `fit` side by side.  More parts fill the SMs, but cost a pass of `extra` of the work for the states (or
+// gradients) that the parts begin with, and two tiles or so for a block's start and end.
+int choose_parts(long long n, int L, int fit, double extra) {
+  const int tiles = cdiv(L, SEL_T);
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 64 && s <= tiles; ++s) {
+    const int per = cdiv(tiles, s);
+    if (cdiv(tiles, per) != s) continue;
+    const long long whole = n * s / (148 * fit), rest = n * s % (148 * fit);
+    const double waves = (double)whole + (rest ? 0.5 + 0.5 * (double)((rest + 147) / 148) / fit : 0.0), cost = waves * (per + 2) * (s > 1 ? 1 + extra : 1.0);
+    if (cost < least) { least = cost; best = s; }
+  }
+  return best;
+}
+void set_parts(SelGeo& q, int segs) {
+  q.segs = segs;
+  q.seg_len = cdiv(cdiv(q.L, SEL_T), segs) * SEL_T;
+}
 
 int make_sel_plan(const SsdSelDims* d, SelPlan* o) {
   if (!d) { set_error("selscan: dims is NULL"); return SSD_ERR_NULL_POINTER; }
@@ -683,9 +941,11 @@ int make_sel_plan(const SsdSelDims* d, SelPlan* o) {
   SelGeo& q = o->q;
   q.B = d->batch; q.L = d->seqlen; q.D = d->channels; q.N = d->dstate; q.G = d->ngroups; q.Dg = q.D / q.G;
   q.softplus = d->dt_softplus != 0;
-  o->lpc = lanes_for(q.N); o->NP = 4 * o->lpc;
-  q.nb = cdiv(q.Dg, chb_for(o->lpc));
-  q.nt = cdiv(q.L, SEL_T);
+  o->NP = padded_states(q.N);
+  q.nb = cdiv(q.Dg, block_channels(o->NP));
+  o->nb_bwd = cdiv(q.Dg, block_channels_bwd(o->NP));
+  q.nc = cdiv(q.L, SEL_C);
+  q.wide = 0;
   if ((long long)q.D * (o->NP + 2) > 0x7ffffff0LL) { set_error("selscan: too many channels (%d)", q.D); return SSD_ERR_UNSUPPORTED; }
   q.par_row = (q.D * (o->NP + 2) + 3) / 4 * 4;
   const long long GN = (long long)q.G * q.N;
@@ -700,65 +960,72 @@ int make_sel_plan(const SsdSelDims* d, SelPlan* o) {
     set_error("selscan: sequence strides must be at least the dense row size");
     return SSD_ERR_BAD_SHAPE;
   }
-  // Parts of the sequence (see below): one where the channel blocks of the batch fill the SMs.
-  const long long n = (long long)q.B * q.G * q.nb;
-  const int sms = 148;
-  int segs = 1;
-  if (n < sms) {
-    segs = (int)((2LL * sms + n - 1) / n);
-    if (segs > q.nt / 4) segs = q.nt / 4;
-    if (segs < 3) segs = 1;
-  }
-  q.seg_len = cdiv(q.nt, segs) * SEL_T;
-  q.segs = cdiv(q.L, q.seg_len);
-  if (n * q.segs > 0x7fffffffLL) { set_error("selscan: too many blocks for one grid (%lld)", n * q.segs); return SSD_ERR_UNSUPPORTED; }
-  const size_t st = (size_t)q.B * q.segs * q.D * sizeof(float);
+  const long long nf = (long long)q.B * q.G * q.nb, nb = (long long)q.B * q.G * o->nb_bwd;
+  o->segs_fwd = choose_parts(nf, q.L, 4, 0.7);
+  o->segs_bwd = choose_parts(nb, q.L, 3, 0.2);
+  if (nf * o->segs_fwd > 0x7fffffffLL || nb * o->segs_bwd > 0x7fffffffLL) { set_error("selscan: too many blocks for one grid"); return SSD_ERR_UNSUPPORTED; }
+  q.segs = 1; q.seg_len = 0;
+  const int most = o->segs_fwd > o->segs_bwd ? o->segs_fwd : o->segs_bwd;
+  const size_t st = (size_t)q.B * most * q.D * sizeof(float);
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t r = at; at += up256(bytes); return r; };
   o->segst = take(st * o->NP); o->segdt = take(st);
   o->fwd_bytes = at + 256;
-  o->ckpt = take((size_t)q.B * q.nt * q.D * o->NP * sizeof(float));
-  o->part_bc = take((size_t)q.G * q.nb * q.B * q.L * 2 * o->NP * sizeof(float));
-  o->part_par = take((size_t)q.B * q.segs * q.par_row * sizeof(float));
+  o->ckpt = take((size_t)q.B * q.nc * q.D * o->NP * sizeof(float));
+  o->part_bc = take((size_t)q.G * o->nb_bwd * q.B * q.L * 2 * o->NP * sizeof(float));
+  o->part_par = take((size_t)q.B * o->segs_bwd * q.par_row * sizeof(float));
   o->bwd_bytes = at + 256;
   return SSD_OK;
 }
 int need_device(const SsdSelDims* d) { return check_common("selscan", d->channels, d->dstate, d->ngroups, d->dtype, d->device); }
 
-#define SEL_LPC(F) \
-  switch (lpc) { case 1: F(1); break; case 2: F(2); break; case 4: F(4); break; case 8: F(8); break; default: F(16); }
+#define SEL_SHAPE(F) \
+  switch (pl.NP) { case 4: F(Sh4); break; case 8: F(Sh8); break; case 16: F(Sh16); break; case 32: F(Sh32); break; default: F(Sh64); }
 
-template <typename T> int sel_forward(const SelPlan& pl, const SelFwd& p, cudaStream_t s) {
-  const SelGeo& q = pl.q;
-  const int lpc = pl.lpc;
+#define SEL_SHAPE_BWD(F) \
+  switch (pl.NP) { case 4: F(Bh4); break; case 8: F(Bh8); break; case 16: F(Bh16); break; case 32: F(Bh32); break; default: F(Bh64); }
+
+// Whether four channels of a row can be moved at once (8 bytes of bf16, 16 of fp32): every row of every tensor starts there.
+bool rows_fit(const SelGeo& q, int es, std::initializer_list<const void*> ps, std::initializer_list<long long> strides) {
+  uintptr_t low = (uintptr_t)(q.Dg * es);
+  for (const void* p : ps) low |= (uintptr_t)p;
+  for (long long v : strides) low |= (uintptr_t)(v * es);
+  return low % (4 * es) == 0;
+}
+template <typename T> int sel_forward(SelPlan pl, const SelFwd& p, cudaStream_t s) {
+  SelGeo& q = pl.q;
+  set_parts(q, pl.segs_fwd);
+  q.wide = rows_fit(q, sizeof(T), {p.x, p.dt, p.z, p.y}, {q.xsb, q.xsl, q.dtsb, q.dtsl, p.z ? q.zsb : 0, p.z ? q.zsl : 0, p.y ? q.ysb : 0, p.y ? q.ysl : 0});
   const unsigned grid = (unsigned)((long long)q.B * q.segs * q.G * q.nb);
   if (q.segs > 1) {
-#define SEL_RUN(LPC) launch<k_sel_fwd<T, LPC, 1>>(grid, Sh<LPC>::TH, 0, s, q, p)
-    SEL_LPC(SEL_RUN)
+#define SEL_RUN(S) launch<k_sel_fwd<T, S, 1>>(grid, S::TH, 0, s, q, p)
+    SEL_SHAPE(SEL_RUN)
 #undef SEL_RUN
     SSD_CUDA_CHECK_LAUNCH("selscan_parts");
   }
-#define SEL_RUN(LPC) launch<k_sel_fwd<T, LPC, 0>>(grid, Sh<LPC>::TH, 0, s, q, p)
-  SEL_LPC(SEL_RUN)
+#define SEL_RUN(S) launch<k_sel_fwd<T, S, 0>>(grid, S::TH, 0, s, q, p)
+  SEL_SHAPE(SEL_RUN)
 #undef SEL_RUN
   SSD_CUDA_CHECK_LAUNCH("selscan_fwd");
   return SSD_OK;
 }
 
-template <typename T> int sel_backward(const SelPlan& pl, const SelBwd& p, const SsdSelBwdPtrs& u, cudaStream_t s) {
-  const SelGeo& q = pl.q;
-  const int lpc = pl.lpc;
+template <typename T> int sel_backward(SelPlan pl, const SelBwd& p, const SsdSelBwdPtrs& u, cudaStream_t s) {
+  SelGeo& q = pl.q;
+  q.nb = pl.nb_bwd;
+  set_parts(q, pl.segs_bwd);
+  q.wide = rows_fit(q, sizeof(T), {p.x, p.dt, p.z, p.dy, p.dx, p.ddt, p.dz}, {q.xsb, q.xsl, q.dtsb, q.dtsl, p.z ? q.zsb : 0, p.z ? q.zsl : 0, q.ysb, q.ysl});
   const unsigned grid = (unsigned)((long long)q.B * q.segs * q.G * q.nb);
   if (q.segs > 1) {
-#define SEL_RUN(LPC) launch<k_sel_bwd_part<T, LPC>>(grid, Sh<LPC>::TH, 0, s, q, p)
-    SEL_LPC(SEL_RUN)
+#define SEL_RUN(S) launch<k_sel_bwd_part<T, S>>(grid, S::TH, 0, s, q, p)
+    SEL_SHAPE_BWD(SEL_RUN)
 #undef SEL_RUN
     SSD_CUDA_CHECK_LAUNCH("selscan_bwd_parts");
   }
-#define SEL_RUN(LPC) do { \
-    if (p.z) launch<k_sel_bwd<T, LPC, true>>(grid, Sh<LPC>::TH, Sh<LPC>::BWD_SMEM, s, q, p); \
-    else launch<k_sel_bwd<T, LPC, false>>(grid, Sh<LPC>::TH, Sh<LPC>::BWD_SMEM, s, q, p); } while (0)
-  SEL_LPC(SEL_RUN)
+#define SEL_RUN(S) do { \
+    if (p.z) launch<k_sel_bwd<T, S, true>>(grid, S::TH, S::BWD_SMEM, s, q, p); \
+    else launch<k_sel_bwd<T, S, false>>(grid, S::TH, S::BWD_SMEM, s, q, p); } while (0)
+  SEL_SHAPE_BWD(SEL_RUN)
 #undef SEL_RUN
   SSD_CUDA_CHECK_LAUNCH("selscan_bwd");
   const long long nbc = (long long)q.B * q.L * q.G * 2 * pl.NP;
@@ -864,7 +1131,7 @@ int32_t ssd_selscan_step(const SsdSelStepDims* d, const SsdStepPtrs* p, void* cu
                                 else launch<k_sel_step<__nv_bfloat16, LPC, false>>((unsigned)blocks, 256, 0, s, q, *p); } \
     else { if (vec) launch<k_sel_step<float, LPC, true>>((unsigned)blocks, 256, 0, s, q, *p); \
            else launch<k_sel_step<float, LPC, false>>((unsigned)blocks, 256, 0, s, q, *p); } } while (0)
-  SEL_LPC(SEL_RUN)
+  switch (lpc) { case 1: SEL_RUN(1); break; case 2: SEL_RUN(2); break; case 4: SEL_RUN(4); break; case 8: SEL_RUN(8); break; default: SEL_RUN(16); }
 #undef SEL_RUN
   SSD_CUDA_CHECK_LAUNCH("selscan_step");
   return SSD_OK;

@@ -18,8 +18,8 @@ def _act(name):
 
 
 def linear_forward(x, weight, bias=None, residual=None, *, activation="none", for_backward=False, out=None):
-    """out, pre.  `pre` = x W^T + bias in the storage type, kept for the backward of an activation (else None): one rounding, the one
-    that a program which keeps its pre-activations makes too."""
+    """out, pre.  `pre` = x W^T + bias in fp32, kept for the backward of an activation (else None): in bf16 its rounding would go
+    through the activation's slope into every gradient, beside that of dpre, which the products read in the storage type."""
     return L.host().linear_forward(x, weight, bias, residual, _act(activation), for_backward, out)
 
 
