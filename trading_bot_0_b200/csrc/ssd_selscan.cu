@@ -46,7 +46,8 @@ template <int KS_, int LPC_, int CHB_> struct Sh {
   static constexpr int IT = SEL_T / RS;              // tasks per thread
   static constexpr int BI = (SEL_T * NP + TH - 1) / TH;          // values of B (and of C) per thread
   static constexpr int COPIES = CPW < KS ? CPW : KS; // backward: orders of the states among a warp's lanes (see ChannelSum)
-  static constexpr int BWD_SMEM = (SEL_T * CHB * 4 + 2 * COPIES * SEL_T * NP + W * SEL_T * 2 * NP + 3 * SEL_T * CHB) * 4;
+  static constexpr int BWD_FLOATS = SEL_T * CHB * 9 + 2 * COPIES * SEL_T * NP + W * SEL_T * 2 * NP + 2 * CHB + KS * TH;   // k_sel_bwd's shared memory ..
+  template <typename T> static constexpr int bwd_smem() { return BWD_FLOATS * 4 + 3 * IT * TH * 4 * (int)sizeof(T); }    // .. with the raw values of its tasks
 };
 
 // log(1 + e) for e in [0, 1]: e P(e) with P the least-maximum fit of log1p(e) / e of degree 8 (relative error 3e-8, 1.7e-7 as
@@ -108,18 +109,18 @@ __device__ __forceinline__ f32x2 decay2_again(f32x2 A2, f32x2 s2) {
 template <typename T> struct Raw4;
 template <> struct Raw4<float> { float4 v; };
 template <> struct Raw4<__nv_bfloat16> { uint2 v; };
-__device__ __forceinline__ void zero4(Raw4<float>& r) { r.v = make_float4(0.f, 0.f, 0.f, 0.f); }
-__device__ __forceinline__ void zero4(Raw4<__nv_bfloat16>& r) { r.v = make_uint2(0, 0); }
-__device__ __forceinline__ void load4(const float* p, bool wide, int n, Raw4<float>& r) {   // n = 1..4 values are there
-  if (wide) { r.v = *reinterpret_cast<const float4*>(p); return; }
-  r.v = make_float4(p[0], n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
+// n values are there (at least one; where there are fewer than four the last one stands in for the rest)
+__device__ __forceinline__ void load4(const float* p, bool wide, int n, Raw4<float>& r) {
+  if (wide) r.v = *reinterpret_cast<const float4*>(p);
+  else r.v = make_float4(p[0], p[n > 1 ? 1 : 0], p[n > 2 ? 2 : 0], p[n > 3 ? 3 : 0]);
 }
 __device__ __forceinline__ void load4(const __nv_bfloat16* p, bool wide, int n, Raw4<__nv_bfloat16>& r) {
-  if (wide) { r.v = *reinterpret_cast<const uint2*>(p); return; }
   const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
-  r.v.x = q[0] | (n > 1 ? (uint32_t)q[1] << 16 : 0u);
-  r.v.y = (n > 2 ? q[2] : 0u) | (n > 3 ? (uint32_t)q[3] << 16 : 0u);
+  if (wide) r.v = *reinterpret_cast<const uint2*>(p);
+  else r.v = make_uint2(q[0] | (uint32_t)q[n > 1 ? 1 : 0] << 16, q[n > 2 ? 2 : 0] | (uint32_t)q[n > 3 ? 3 : 0] << 16);
 }
+__device__ __forceinline__ void zero4(Raw4<float>& r) { r.v = make_float4(0.f, 0.f, 0.f, 0.f); }
+__device__ __forceinline__ void zero4(Raw4<__nv_bfloat16>& r) { r.v = make_uint2(0, 0); }
 __device__ __forceinline__ void values4(const Raw4<float>& r, float (&v)[4]) { v[0] = r.v.x; v[1] = r.v.y; v[2] = r.v.z; v[3] = r.v.w; }
 __device__ __forceinline__ void values4(const Raw4<__nv_bfloat16>& r, float (&v)[4]) {
   v[0] = __uint_as_float(r.v.x << 16); v[1] = __uint_as_float(r.v.x & 0xffff0000u);
@@ -529,14 +530,19 @@ template <class S> struct ChannelSum {
 };
 
 template <typename T, class S, bool GATED>
-__global__ void __launch_bounds__(S::TH, S::TH == 128 ? 3 : 1) k_sel_bwd(SelGeo q, SelBwd p) {
+__global__ void __launch_bounds__(S::TH, S::TH == 128 ? 4 : 1) k_sel_bwd(SelGeo q, SelBwd p) {
   constexpr int KS = S::KS, LPC = S::LPC, KP = S::KP, NP = S::NP, CHB = S::CHB, TH = S::TH, IT = S::IT, BI = S::BI, W = S::W, CO = S::COPIES;
-  extern __shared__ __align__(16) float sel_smem[];
-  float4 (*s_v)[CHB] = reinterpret_cast<float4 (*)[CHB]>(sel_smem);    // step, step * x, dy', d step / d raw
-  float (*s_B)[SEL_T][NP] = reinterpret_cast<float (*)[SEL_T][NP]>(sel_smem + SEL_T * CHB * 4);   // [order][token][states]
+  extern __shared__ __align__(16) float sel_smem[];                   // (registers are short here: what a tile needs once lies in it)
+  float2 (*s_a)[CHB] = reinterpret_cast<float2 (*)[CHB]>(sel_smem);    // step, step * x
+  float (*s_y)[CHB] = reinterpret_cast<float (*)[CHB]>(sel_smem + 2 * SEL_T * CHB);               // dy'
+  float (*s_ds)[CHB] = s_y + SEL_T;                                    // d step / d raw
+  float (*s_1)[CHB] = s_ds + SEL_T, (*s_2)[CHB] = s_1 + SEL_T, (*s_3)[CHB] = s_2 + SEL_T;         // g.B, sum of g a h A, C.h
+  float (*s_dD)[CHB] = s_3 + SEL_T, (*s_db)[CHB] = s_dD + SEL_T, *s_bias = s_db[SEL_T], *s_D = s_bias + CHB;
+  float (*s_B)[SEL_T][NP] = reinterpret_cast<float (*)[SEL_T][NP]>(s_D + CHB);                    // [order][token][states]
   float (*s_C)[SEL_T][NP] = s_B + CO;
   float (*s_bc)[SEL_T][2 * NP] = reinterpret_cast<float (*)[SEL_T][2 * NP]>(s_C + CO);            // [warp][token][dB | dC]
-  float (*s_1)[CHB] = reinterpret_cast<float (*)[CHB]>(s_bc + W), (*s_2)[CHB] = s_1 + SEL_T, (*s_3)[CHB] = s_2 + SEL_T;
+  float4* s_dA = reinterpret_cast<float4*>(s_bc + W);                  // [KS / 4][thread]
+  Raw4<T>* s_raw = reinterpret_cast<Raw4<T>*>(s_dA + KS / 4 * TH);     // [x, dy, z][task][thread]
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = tid / LPC, nl = tid % LPC, qc = tid % S::QR * 4, r0 = tid / S::QR;
   const bool tasks = r0 < SEL_T;
@@ -552,19 +558,24 @@ __global__ void __launch_bounds__(S::TH, S::TH == 128 ? 3 : 1) k_sel_bwd(SelGeo 
   const T* cp = (const T*)p.Cm + (long long)it.b * q.csb + (long long)it.g * q.N;
   const long long out0 = (long long)it.b * q.L * q.D + it.d;
   float* bc0 = p.part_bc + ((long long)(blockIdx.x % (q.G * q.nb)) * q.B + me.b) * q.L * (2 * NP);
-  float bias[4], Dv[4], dD[4] = {}, dbias[4] = {};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    bias[k] = p.bias && k < it.n ? p.bias[it.d + k] : 0.f;
-    Dv[k] = p.D && k < it.n ? p.D[it.d + k] : 0.f;
+  for (int e = tid; e < CHB; e += TH) {
+    const Place at = place<S>(q, e);
+    s_bias[e] = p.bias && at.n > 0 ? p.bias[at.d] : 0.f;
+    s_D[e] = p.D && at.n > 0 ? p.D[at.d] : 0.f;
   }
+  if (tasks)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s_dD[r0][qc + k] = s_db[r0][qc + k] = 0.f;
+  __syncthreads();
   const int m = ChannelSum<S>::order(lane);
 
-  f32x2 A[KP], g[KP], dA[KP];                        // g: a_{t+1} g_{t+1}
+  f32x2 A[KP], g[KP];                                // g: a_{t+1} g_{t+1}
   load_state<S>(p.A + (long long)me.d * q.N, q.N, nl, live, m, A);
   load_state<S>(p.dfin ? p.dfin + ((long long)me.b * q.D + me.d) * q.N : nullptr, q.N, nl, live, m, g);
 #pragma unroll
-  for (int k = 0; k < KP; ++k) { A[k] = mul2(A[k], dup2(LOG2E)); dA[k] = 0ull; }
+  for (int k = 0; k < KP; ++k) A[k] = mul2(A[k], dup2(LOG2E));
+#pragma unroll
+  for (int k = 0; k < KS / 4; ++k) s_dA[k * TH + tid] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s = q.segs - 1; s > me.seg; --s) {
     const long long at = ((long long)me.b * q.segs + s) * q.D + me.d;
     f32x2 v[KP];
@@ -577,50 +588,59 @@ __global__ void __launch_bounds__(S::TH, S::TH == 128 ? 3 : 1) k_sel_bwd(SelGeo 
 
   Raw4<T> rx[IT], rd[IT], ry[IT], rz[IT];
   T rb[BI], rc[BI];
+  // Values of a tile into registers, for a tile that has tokens.  Every address is one that may be read (a row past the end becomes
+  // the last one before it) and nothing is chosen among before the values are used: a select would wait for the load (4 x 2048 x 1536:
+  // 343 us with loads under a condition, 321 so; in the forward the clamping costs more than it gives, 104 against 121).
+  const int have = max(it.n, 1);
   auto request = [&](int t0) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int t = t0 + r0 + i * S::RS;
-      zero4(rx[i]); zero4(rd[i]); zero4(ry[i]); zero4(rz[i]);
-      if (tasks && it.n > 0 && t < t_live) {
-        load4(xp + (long long)t * q.xsl, wide, it.n, rx[i]);
-        load4(dtp + (long long)t * q.dtsl, wide, it.n, rd[i]);
-        load4(dyp + (long long)t * q.ysl, wide, it.n, ry[i]);
-        if (GATED) load4(zp + (long long)t * q.zsl, wide, it.n, rz[i]);
-      }
+      const long long t = min(t0 + r0 + i * S::RS, t_live - 1);
+      load4(xp + t * q.xsl, wide, have, rx[i]);
+      load4(dtp + t * q.dtsl, wide, have, rd[i]);
+      load4(dyp + t * q.ysl, wide, have, ry[i]);
+      if (GATED) load4(zp + t * q.zsl, wide, have, rz[i]);
     }
 #pragma unroll
     for (int i = 0; i < BI; ++i) {
-      const int e = tid + i * TH, n = e % NP, t = t0 + e / NP;
-      rb[i] = rc[i] = T(0.f);
-      if (n < q.N && t < t_live && e < SEL_T * NP) { rb[i] = bp[(long long)t * q.bsl + n]; rc[i] = cp[(long long)t * q.csl + n]; }
+      const int e = tid + i * TH, n = min(e % NP, q.N - 1);
+      const long long t = min(t0 + e / NP, t_live - 1);
+      rb[i] = bp[t * q.bsl + n];
+      rc[i] = cp[t * q.csl + n];
     }
   };
+  // the state before token t (of channels and tokens that are not there: of others; nothing comes of it)
   const float* ck0 = p.ckpt + ((long long)me.b * q.nc * q.D + me.d) * NP + nl * KS;
-  auto kept = [&](int t, f32x2 (&v)[KP]) {           // the state before token t
-    if (live && t < t_end) load_padded<S>(ck0 + (long long)(t / SEL_C) * q.D * NP, v);
-    else
-#pragma unroll
-      for (int k = 0; k < KP; ++k) v[k] = 0ull;
-  };
+  auto kept = [&](int t, f32x2 (&v)[KP]) { load_padded<S>(ck0 + (long long)min(t / SEL_C, q.nc - 1) * q.D * NP, v); };
   const int t_last = t_begin + (t_end - t_begin - 1) / SEL_T * SEL_T;
-  request(t_last);
+  if (t_last < t_live) request(t_last);
   f32x2 first[KP];                                   // the state before the next eight tokens to be walked
   kept(t_last + SEL_C, first);
   for (int t0 = t_last; t0 >= t_begin; t0 -= SEL_T) {
-    Raw4<T> kx[IT], ky[IT], kz[IT];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int r = r0 + i * S::RS, t = t0 + r;
-      float x[4], d[4], y[4], z[4];
-      kx[i] = rx[i]; ky[i] = ry[i]; kz[i] = rz[i];
+      float x[4], d[4], y[4], z[4], s[4], ds[4];
+      s_raw[(0 * IT + i) * TH + tid] = rx[i]; s_raw[(1 * IT + i) * TH + tid] = ry[i];
+      if (GATED) s_raw[(2 * IT + i) * TH + tid] = rz[i];
       values4(rx[i], x); values4(rd[i], d); values4(ry[i], y); values4(rz[i], z);
+      const float4 b4 = *reinterpret_cast<const float4*>(s_bias + qc);
+      const float bias[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float s = 0.f, ds = 0.f;
-        if (t < t_live) s = sel_step_d(d[k], bias[k], q.softplus, ds);
+        s[k] = ds[k] = 0.f;
+        const bool ok = t < t_live && k < it.n;
+        if (ok) s[k] = sel_step_d(d[k], bias[k], q.softplus, ds[k]);
         if (GATED) y[k] *= z[k] * sig(z[k]);
-        if (tasks) s_v[r][qc + k] = make_float4(s, s * x[k], y[k], ds);
+        y[k] = ok ? y[k] : 0.f;
+        x[k] = ok ? x[k] : 0.f;
+      }
+      if (tasks) {
+        float4* w = reinterpret_cast<float4*>(&s_a[r][qc]);
+        w[0] = make_float4(s[0], s[0] * x[0], s[1], s[1] * x[1]);
+        w[1] = make_float4(s[2], s[2] * x[2], s[3], s[3] * x[3]);
+        *reinterpret_cast<float4*>(&s_y[r][qc]) = make_float4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<float4*>(&s_ds[r][qc]) = make_float4(ds[0], ds[1], ds[2], ds[3]);
       }
     }
 #pragma unroll
@@ -628,13 +648,15 @@ __global__ void __launch_bounds__(S::TH, S::TH == 128 ? 3 : 1) k_sel_bwd(SelGeo 
       const int e = tid + i * TH;
       if (e < SEL_T * NP) {
         const int r = e / NP, n = e % NP;
+        const bool ok = n < q.N && t0 + r < t_live;
+        const float fb = ok ? (float)rb[i] : 0.f, fc = ok ? (float)rc[i] : 0.f;
 #pragma unroll
-        for (int o = 0; o < CO; ++o) { const int oo = o * (KS / CO); s_B[o][r][n ^ oo] = (float)rb[i]; s_C[o][r][n ^ oo] = (float)rc[i]; }
+        for (int o = 0; o < CO; ++o) { const int oo = o * (KS / CO); s_B[o][r][n ^ oo] = fb; s_C[o][r][n ^ oo] = fc; }
       }
     }
     f32x2 tA[KP] = {};                               // a tile's share of dA: sums of 16, then sums of tiles
     __syncthreads();
-    if (t0 > t_begin) request(t0 - SEL_T);
+    if (t0 > t_begin && t0 - SEL_T < t_live) request(t0 - SEL_T);
     if (t0 >= len) {
       if (t0 > t_begin) kept(t0 - SEL_C, first);
     } else {
@@ -650,7 +672,7 @@ __global__ void __launch_bounds__(S::TH, S::TH == 128 ? 3 : 1) k_sel_bwd(SelGeo 
 #pragma unroll
         for (int i = 0; i < SEL_C; ++i) {
           const int r = half * SEL_C + i;
-          const float2 v = *reinterpret_cast<const float2*>(&s_v[r][c]);
+          const float2 v = s_a[r][c];
           const f32x2 s2 = dup2(v.x), x2 = dup2(v.y);
 #pragma unroll
           for (int k = 0; k < KP; k += 2) {
@@ -666,8 +688,8 @@ __global__ void __launch_bounds__(S::TH, S::TH == 128 ? 3 : 1) k_sel_bwd(SelGeo 
 #pragma unroll
           for (int f = FR - 1; f >= 0; --f) {
             const int i = u + f, r = half * SEL_C + i;
-            const float4 v = s_v[r][c];
-            const f32x2 s2 = dup2(v.x), x2 = dup2(v.y), y2 = dup2(v.z);
+            const float2 v = s_a[r][c];
+            const f32x2 s2 = dup2(v.x), x2 = dup2(v.y), y2 = dup2(s_y[r][c]);
             f32x2 a1 = 0ull, a2 = 0ull, a3 = 0ull;
             float wb[KS], wc[KS];
 #pragma unroll
@@ -709,7 +731,12 @@ __global__ void __launch_bounds__(S::TH, S::TH == 128 ? 3 : 1) k_sel_bwd(SelGeo 
       }
     }
 #pragma unroll
-    for (int k = 0; k < KP; ++k) dA[k] = add2(dA[k], tA[k]);
+    for (int k = 0; k < KS / 4; ++k) {
+      const float4 f = s_dA[k * TH + tid];
+      float t[4];
+      unpack2(tA[2 * k], t[0], t[1]); unpack2(tA[2 * k + 1], t[2], t[3]);
+      s_dA[k * TH + tid] = make_float4(f.x + t[0], f.y + t[1], f.z + t[2], f.w + t[3]);
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
@@ -718,22 +745,29 @@ __global__ void __launch_bounds__(S::TH, S::TH == 128 ? 3 : 1) k_sel_bwd(SelGeo 
       float dx[4] = {}, dd[4] = {}, dz[4] = {};
       if (t < len) {
         float x[4], y[4], z[4];
-        values4(kx[i], x); values4(ky[i], y); values4(kz[i], z);
+        values4(s_raw[(0 * IT + i) * TH + tid], x); values4(s_raw[(1 * IT + i) * TH + tid], y);
+        if (GATED) values4(s_raw[(2 * IT + i) * TH + tid], z);
+        const float4 y4 = *reinterpret_cast<const float4*>(&s_y[r][qc]), ds4 = *reinterpret_cast<const float4*>(&s_ds[r][qc]);
+        const float dy0[4] = {y4.x, y4.y, y4.z, y4.w}, ds[4] = {ds4.x, ds4.y, ds4.z, ds4.w};
         const float4 f1 = *reinterpret_cast<const float4*>(&s_1[r][qc]), f2 = *reinterpret_cast<const float4*>(&s_2[r][qc]);
         const float4 f3 = GATED ? *reinterpret_cast<const float4*>(&s_3[r][qc]) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float gB[4] = {f1.x, f1.y, f1.z, f1.w}, qA[4] = {f2.x, f2.y, f2.z, f2.w}, hC[4] = {f3.x, f3.y, f3.z, f3.w};
+        const float4 D4 = *reinterpret_cast<const float4*>(s_D + qc);
+        float4 aD = *reinterpret_cast<const float4*>(&s_dD[r0][qc]), ab = *reinterpret_cast<const float4*>(&s_db[r0][qc]);
+        float dD[4] = {aD.x, aD.y, aD.z, aD.w}, dbias[4] = {ab.x, ab.y, ab.z, ab.w};
+        const float Dv[4] = {D4.x, D4.y, D4.z, D4.w}, gB[4] = {f1.x, f1.y, f1.z, f1.w}, qA[4] = {f2.x, f2.y, f2.z, f2.w}, hC[4] = {f3.x, f3.y, f3.z, f3.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float4 v = s_v[r][qc + k];
           if (GATED) {
             const float sg = sig(z[k]);
             dz[k] = y[k] * fmaf(Dv[k], x[k], hC[k]) * sg * fmaf(z[k], 1.f - sg, 1.f);
           }
-          dx[k] = fmaf(v.x, gB[k], Dv[k] * v.z);
-          dd[k] = fmaf(x[k], gB[k], qA[k] * LN2) * v.w;
-          dD[k] = fmaf(v.z, x[k], dD[k]);
+          dx[k] = fmaf(s_a[r][qc + k].x, gB[k], Dv[k] * dy0[k]);
+          dd[k] = fmaf(x[k], gB[k], qA[k] * LN2) * ds[k];
+          dD[k] = fmaf(dy0[k], x[k], dD[k]);
           dbias[k] += dd[k];
         }
+        *reinterpret_cast<float4*>(&s_dD[r0][qc]) = make_float4(dD[0], dD[1], dD[2], dD[3]);
+        *reinterpret_cast<float4*>(&s_db[r0][qc]) = make_float4(dbias[0], dbias[1], dbias[2], dbias[3]);
       }
       const long long o = out0 + (long long)t * q.D;
       put4((T*)p.dx + o, wide, it.n, dx); put4((T*)p.ddt + o, wide, it.n, dd);
@@ -754,18 +788,21 @@ __global__ void __launch_bounds__(S::TH, S::TH == 128 ? 3 : 1) k_sel_bwd(SelGeo 
   }
   if (p.dinit && me.seg == 0) store_state<S>(p.dinit + ((long long)me.b * q.D + me.d) * q.N, q.N, nl, live, m, g);
   float* par = p.part_par + ((long long)me.b * q.segs + me.seg) * q.par_row;
+  f32x2 dA[KP];
+#pragma unroll
+  for (int k = 0; k < KS / 4; ++k) {
+    const float4 f = s_dA[k * TH + tid];
+    dA[2 * k] = pack2(f.x, f.y); dA[2 * k + 1] = pack2(f.z, f.w);
+  }
   permute<S>(dA, m);                                 // (its own inverse)
   if (live) store_padded<S>(par + (long long)me.d * NP + nl * KS, dA);
-  if (tasks)                                         // the threads of four channels, in order
-#pragma unroll
-    for (int k = 0; k < 4; ++k) { s_1[r0][qc + k] = dD[k]; s_2[r0][qc + k] = dbias[k]; }
-  __syncthreads();
+  __syncthreads();                                   // the threads of four channels, in order
   for (int e = tid; e < CHB; e += TH) {
     const Place at = place<S>(q, e);
     if (at.n <= 0) continue;
     float a = 0.f, b = 0.f;
 #pragma unroll
-    for (int r = 0; r < S::RS; ++r) { a += s_1[r][e]; b += s_2[r][e]; }
+    for (int r = 0; r < S::RS; ++r) { a += s_dD[r][e]; b += s_db[r][e]; }
     par[(long long)q.D * NP + at.d] = a;
     par[(long long)q.D * (NP + 1) + at.d] = b;
   }
@@ -912,21 +949,18 @@ struct SelPlan {
   size_t ckpt, segst, segdt, part_bc, part_par, fwd_bytes, bwd_bytes;   // offsets and totals
 };
 
-// Parts of the sequence.  n blocks walk the tokens one after the other, `fit` of them at a time on an SM; a lone block takes about half
-// as long for a tile as `fit` side by side.  More parts fill the SMs, but cost a pass of `extra` of the work for the states (or
-// gradients) that the parts begin with, and two tiles or so for a block's start and end.
-int choose_parts(long long n, int L, int fit, double extra) {
+// Parts of the sequence.  n blocks walk the tokens one after the other; below about two of them to an SM the SMs mostly wait, and the
+// sequence is cut into parts, which costs a pass over the steps for the states (or gradients) that the parts begin with.  Measured
+// (us, forward with that pass; parts 1, 6, 12, 24): 1 x 4096 x 1536 (24 blocks) 636, 188, 126, 102; 4 x 2048 x 1536 (96) 337, 184,
+// 183, 191; 64 x 512 x 512 (512) 154 with one part, 195 with two.  Backward (parts 1, 4, 8, 16): 4 x 2048 x 1536 (192 blocks) 655,
+// 467, 446, 434; 2 x 512 x 768 (48) 125, 59, 43, 45; 64 x 512 x 512 (1024) 541, 551, 575, 647.
+int choose_parts(long long n, int L, long long below, int least_tiles) {
   const int tiles = cdiv(L, SEL_T);
-  int best = 1;
-  double least = 1e30;
-  for (int s = 1; s <= 64 && s <= tiles; ++s) {
-    const int per = cdiv(tiles, s);
-    if (cdiv(tiles, per) != s) continue;
-    const long long whole = n * s / (148 * fit), rest = n * s % (148 * fit);
-    const double waves = (double)whole + (rest ? 0.5 + 0.5 * (double)((rest + 147) / 148) / fit : 0.0), cost = waves * (per + 2) * (s > 1 ? 1 + extra : 1.0);
-    if (cost < least) { least = cost; best = s; }
-  }
-  return best;
+  if (n >= below) return 1;
+  long long s = 8 * 148 / n;
+  if (s > tiles / least_tiles) s = tiles / least_tiles;
+  if (s < 2) return 1;
+  return cdiv(tiles, cdiv(tiles, (int)s));
 }
 void set_parts(SelGeo& q, int segs) {
   q.segs = segs;
@@ -961,8 +995,8 @@ int make_sel_plan(const SsdSelDims* d, SelPlan* o) {
     return SSD_ERR_BAD_SHAPE;
   }
   const long long nf = (long long)q.B * q.G * q.nb, nb = (long long)q.B * q.G * o->nb_bwd;
-  o->segs_fwd = choose_parts(nf, q.L, 4, 0.7);
-  o->segs_bwd = choose_parts(nb, q.L, 3, 0.2);
+  o->segs_fwd = choose_parts(nf, q.L, 2 * 148, 2);
+  o->segs_bwd = choose_parts(nb, q.L, 4 * 148, 4);
   if (nf * o->segs_fwd > 0x7fffffffLL || nb * o->segs_bwd > 0x7fffffffLL) { set_error("selscan: too many blocks for one grid"); return SSD_ERR_UNSUPPORTED; }
   q.segs = 1; q.seg_len = 0;
   const int most = o->segs_fwd > o->segs_bwd ? o->segs_fwd : o->segs_bwd;
@@ -1023,8 +1057,8 @@ template <typename T> int sel_backward(SelPlan pl, const SelBwd& p, const SsdSel
     SSD_CUDA_CHECK_LAUNCH("selscan_bwd_parts");
   }
 #define SEL_RUN(S) do { \
-    if (p.z) launch<k_sel_bwd<T, S, true>>(grid, S::TH, S::BWD_SMEM, s, q, p); \
-    else launch<k_sel_bwd<T, S, false>>(grid, S::TH, S::BWD_SMEM, s, q, p); } while (0)
+    if (p.z) launch<k_sel_bwd<T, S, true>>(grid, S::TH, S::bwd_smem<T>(), s, q, p); \
+    else launch<k_sel_bwd<T, S, false>>(grid, S::TH, S::bwd_smem<T>(), s, q, p); } while (0)
   SEL_SHAPE_BWD(SEL_RUN)
 #undef SEL_RUN
   SSD_CUDA_CHECK_LAUNCH("selscan_bwd");
