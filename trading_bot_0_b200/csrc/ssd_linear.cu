@@ -34,8 +34,8 @@ __device__ __forceinline__ void values_of(const uint4& r, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) { const float2 f = umma::unpack_bf16(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
 }
+__device__ __forceinline__ void load_floats(const float* p, float (&v)[1]) { v[0] = *p; }
 template <int V> __device__ __forceinline__ void load_floats(const float* p, float (&v)[V]) {
-  if (V == 1) { v[0] = *p; return; }
 #pragma unroll
   for (int i = 0; i < V / 4; ++i) *reinterpret_cast<float4*>(v + 4 * i) = *reinterpret_cast<const float4*>(p + 4 * i);
 }
@@ -190,17 +190,22 @@ __global__ void __launch_bounds__(256) k_mm_few(MmArgs a) {
 // ---------------------------------------------------------------------------------------------
 // out[m][n] = epilogue(sum_k P(m,k) Q(n,k)) for bf16 operands that a tensor map can describe.
 //
-// A pair of CTAs computes tiles of 256 x bn: every CTA loads 128 rows of P and bn/2 rows of Q per block of 64 k (32 KB at bn = 256),
-// where a CTA on its own would load 48 KB for the same work per SM: at the tensor cores' rate that is 13 instead of 19 TB/s out
-// of the L2.  Warp 0 of each CTA issues the loads (six stages), warp 1 of the leader the MMAs, eight warps per CTA read the
-// accumulators (two of them in TMEM, so that a tile's epilogue runs beside the next tile's products).  Pairs walk the units
-// (split of k, tile row, tile column) with a fixed stride; with splits > 1 a unit leaves fp32 sums in the workspace and k_mm2_join adds
-// them in order.  Every wait is bounded: when one runs out a code goes to the status word and the outputs become NaN.
+// A pair of CTAs computes tiles of 256 x bn: every CTA loads 128 rows of P and bn/2 rows of Q per block of 64 k (32 KB at bn = 256,
+// where a CTA on its own would load 48 KB for the same work per SM).  Warp 0 of each CTA issues the loads (five stages), warp 1 of the
+// leader the MMAs, eight warps per CTA read the accumulators (two of them in TMEM, so that a tile's epilogue runs beside the next
+// tile's products).  Pairs walk the units (split of k, tile row, tile column) with a fixed stride; with splits > 1 a unit leaves fp32
+// sums in the workspace and k_mm2_join adds them in order.  Every wait is bounded: when one runs out a code goes to the status word and
+// the outputs become NaN.
+//
+// Measured, 8192^3: 677 us = 1.62 PFLOP/s (cuBLAS 640 to 680 on the same boards), 4096 x 2048 x 2048 34 us (36); 785 us with loads and
+// MMAs issued by `lane == 0` instead of an elected lane, whatever the tile's width; four stages are as fast as five, three 10 % slower;
+// both accumulators as one tile of 256 x 512, which loads a quarter less, 670 us, but 103 against 77 us at 16384 x 768 x 3352, where
+// its epilogue is not hidden.
 namespace u = umma;
-constexpr int MM_STAGES = 5, MM_BM = 256, MM_EPI = 8, MM_THREADS = 32 * (4 + MM_EPI);
-constexpr int MM_STAGE = 32768;                    // 16 KB of P, 16 KB of Q
-constexpr int MM_SLOT = 6144;                      // output staging of a warp: a box of 32 x 32 fp32 and one of bf16, or two of bf16
+constexpr int MM_BM = 256, MM_EPI = 8, MM_THREADS = 32 * (4 + MM_EPI);
+constexpr int MM_SLOT = 4096;                      // output staging of a warp: a box of 32 x 32 fp32, or two of bf16
 constexpr int MM_ROWS = 8;                         // tile rows walked side by side: the pairs at work share operands in the L2
+constexpr int MM_STAGES = 5, MM_STAGE = 32768;      // 128 rows of P, up to 128 of Q
 constexpr size_t MM_SMEM = (size_t)MM_STAGES * MM_STAGE + MM_EPI * MM_SLOT + 1024;
 
 struct Mm2 {
@@ -254,7 +259,7 @@ k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMa
   __shared__ __align__(8) uint64_t full[MM_STAGES], empty[MM_STAGES], tfull[2], tempty[2];
   __shared__ uint32_t slot;
   __shared__ int dead;
-  __shared__ __align__(16) float s_bias[2][256];
+  __shared__ __align__(16) __nv_bfloat16 s_bias[2][256];
   unsigned char* st = mm_raw + (1024 - (u::smem_u32(mm_raw) & 1023)) % 1024;   // the same offset in both CTAs
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = u::cluster_rank();
@@ -281,21 +286,22 @@ k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMa
     *a.status = code;
     return false;
   };
+  auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, wait(bar, parity, code)) != 0; };   // a warp goes on or gives up as one
   const int half = a.bn / 2;
   if (warp == 0) {
-    if (lane == 0) {
-      const int qbox = QMN ? (half + 63) / 64 : 1;
-      const uint32_t bytes = 2u * (16384u + (QMN ? qbox * 8192u : half * 128u));
-      int s = 0;
-      uint32_t ph = 1;
-      bool ok = true;
-      for (int un = pair; un < a.units && ok; un += npairs) {
-        int sp, r, c;
-        unit_at(a, un, sp, r, c);
-        const int k0 = sp * a.kper, k1 = min(k0 + a.kper, a.kb);
-        const int prow = r * MM_BM + (int)rank * 128, qrow = c * a.bn + (int)rank * half;
-        for (int k = k0; k < k1; ++k) {
-          if (!(ok = wait(&empty[s], ph, 201))) break;
+    const int qbox = QMN ? (half + 63) / 64 : 1;
+    const uint32_t bytes = 2u * (16384u + (QMN ? qbox * 8192u : half * 128u));
+    int s = 0;
+    uint32_t ph = 1;
+    bool ok = true;
+    for (int un = pair; un < a.units && ok; un += npairs) {
+      int sp, r, c;
+      unit_at(a, un, sp, r, c);
+      const int k0 = sp * a.kper, k1 = min(k0 + a.kper, a.kb);
+      const int prow = r * MM_BM + (int)rank * 128, qrow = c * a.bn + (int)rank * half;
+      for (int k = k0; k < k1; ++k) {
+        if (!(ok = wait_all(&empty[s], ph, 201))) break;
+        if (u::elect_one()) {
           unsigned char* sa = st + s * MM_STAGE;
           unsigned char* sb = sa + 16384;
           if (rank == 0) u::mbar_expect_tx(&full[s], bytes);
@@ -311,16 +317,17 @@ k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMa
           } else {
             u::tma_load_2d_pair(sb, &tq, k * 64, qrow, bar);
           }
-          if (++s == MM_STAGES) { s = 0; ph ^= 1; }
         }
-      }
-      if (!ok) {   // let copies in flight land before the shared memory goes back
-        const long long t0 = clock64();
-        while (clock64() - t0 < 4000000) {}
+        __syncwarp();
+        if (++s == MM_STAGES) { s = 0; ph ^= 1; }
       }
     }
+    if (!ok) {   // let copies in flight land before the shared memory goes back
+      const long long t0 = clock64();
+      while (clock64() - t0 < 4000000) {}
+    }
   } else if (warp == 1) {
-    if (rank == 0 && lane == 0) {
+    if (rank == 0) {
       const uint32_t idesc = u::make_idesc(256, a.bn, PMN, QMN);
       int s = 0, buf = 0;
       uint32_t ph = 0, tph = 1;
@@ -328,22 +335,26 @@ k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMa
       for (int un = pair; un < a.units && ok; un += npairs) {
         const int sp = un / (a.ct * a.rt);
         const int k0 = sp * a.kper, k1 = min(k0 + a.kper, a.kb);
-        if (!(ok = wait(&tempty[buf], tph, 202))) break;
+        if (!(ok = wait_all(&tempty[buf], tph, 202))) break;
         u::tc_fence_after();
         for (int k = k0; k < k1; ++k) {
-          if (!(ok = wait(&full[s], ph, 203))) break;
+          if (!(ok = wait_all(&full[s], ph, 203))) break;
           u::tc_fence_after();
-          const uint32_t sa = u::smem_u32(st + s * MM_STAGE), sb = sa + 16384;
-          const uint64_t ad = PMN ? u::desc_sw128_mn(sa, 0, 0, 8192) : u::desc_sw128_k(sa, 0);
-          const uint64_t bd = QMN ? u::desc_sw128_mn(sb, 0, 0, 8192) : u::desc_sw128_k(sb, 0);
+          if (u::elect_one()) {
+            const uint32_t sa = u::smem_u32(st + s * MM_STAGE), sb = sa + 16384;
+            const uint64_t ad = PMN ? u::desc_sw128_mn(sa, 0, 0, 8192) : u::desc_sw128_k(sa, 0);
+            const uint64_t bd = QMN ? u::desc_sw128_mn(sb, 0, 0, 8192) : u::desc_sw128_k(sb, 0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            u::mma_bf16_pair(tmem + buf * 256, u::desc_adv(ad, i * (PMN ? 2048 : 32)), u::desc_adv(bd, i * (QMN ? 2048 : 32)), idesc, k > k0 || i > 0);
-          u::mma_commit_pair(&empty[s]);
+            for (int i = 0; i < 4; ++i)
+              u::mma_bf16_pair(tmem + buf * 256, u::desc_adv(ad, i * (PMN ? 2048 : 32)), u::desc_adv(bd, i * (QMN ? 2048 : 32)), idesc, k > k0 || i > 0);
+            u::mma_commit_pair(&empty[s]);
+          }
+          __syncwarp();
           if (++s == MM_STAGES) { s = 0; ph ^= 1; }
         }
         if (!ok) break;
-        u::mma_commit_pair(&tfull[buf]);
+        if (u::elect_one()) u::mma_commit_pair(&tfull[buf]);
+        __syncwarp();
         buf ^= 1;
         if (!buf) tph ^= 1;
       }
@@ -372,7 +383,7 @@ k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMa
       const bool res = direct && a.vec && a.residual;
       if (res) ask(grp * 32);
       if (direct) {
-        for (int i = tid - 128; i < 256; i += 32 * MM_EPI) s_bias[buf][i] = a.bias && i < ncol ? __bfloat162float(a.bias[n0 + i]) : 0.f;
+        for (int i = tid - 128; i < 256; i += 32 * MM_EPI) s_bias[buf][i] = a.bias && i < ncol ? a.bias[n0 + i] : __nv_bfloat16(0.f);
         asm volatile("bar.sync 1, %0;" ::"n"(32 * MM_EPI) : "memory");
       }
       ok = ok && wait(&tfull[buf], tph, 204);
@@ -414,11 +425,12 @@ k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMa
         if (res && j + 64 < ncol) ask(j + 64);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float4 b = *reinterpret_cast<const float4*>(&s_bias[buf][j + 4 * i]);
-          v[4 * i] += b.x; v[4 * i + 1] += b.y; v[4 * i + 2] += b.z; v[4 * i + 3] += b.w;
+          const uint2 w = *reinterpret_cast<const uint2*>(&s_bias[buf][j + 4 * i]);
+          const float2 b = u::unpack_bf16(w.x), e2 = u::unpack_bf16(w.y);
+          v[4 * i] += b.x; v[4 * i + 1] += b.y; v[4 * i + 2] += e2.x; v[4 * i + 3] += e2.y;
         }
-        auto put = [&](const CUtensorMap* map, int at, bool f32) {   // two boxes in turn: the older store has read its box
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        auto put = [&](const CUtensorMap* map, int at, bool f32) {   // out alone: two boxes in turn, the older store has read its box
+          if (lane == 0) { if (a.pre) u::bulk_wait_read0(); else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
           __syncwarp();
           if (f32) stage_f32(slot_a + at, lane, v); else stage_bf16(slot_a + at, lane, v);
           u::fence_async_smem();
@@ -447,7 +459,7 @@ k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMa
             }
           }
         }
-        put(&tout, a.pre ? 4096 : box * 2048, false);
+        put(&tout, a.pre ? 0 : box * 2048, false);
         box ^= 1;
       }
       u::tc_fence_before();
@@ -465,16 +477,34 @@ k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMa
   if (warp == 2) u::tmem_dealloc_pair(tmem, 512);
 }
 
-// The splits' sums in order, then the epilogue.  Thread = one value; neighbouring threads neighbouring columns.
-__global__ void __launch_bounds__(256) k_mm2_join(Mm2 a, long long rows, long long cols) {
+// The splits' sums in order, then the epilogue.  Thread = V values of a row (four where rows of sums and of out start on 16 and 8 bytes).
+template <int V>
+__global__ void __launch_bounds__(256) k_mm2_join(Mm2 a, long long rows, int cols) {
   pdl_wait();
   const long long n = rows * cols;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    float v = 0.f;
+  const int pieces = cols / V;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * pieces; i += (long long)gridDim.x * 256) {
+    const long long m = i / pieces;
+    const int c = (int)(i - m * pieces) * V;
+    float v[V] = {};
 #pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) v += a.part[s * n + i];
-    const long long m = i / cols;
-    finish_one(a, cols, m, i - m * cols, v);
+    for (int s = 0; s < a.splits; ++s) {
+      float f[V];
+      load_floats(a.part + s * n + m * cols + c, f);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] += f[k];
+    }
+    if (V == 4 && !a.pre && !a.residual) {
+      if (a.bias)
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += __bfloat162float(a.bias[c + k]);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = act_of(v[k], a.act);
+      *reinterpret_cast<uint2*>(a.out + m * a.os + c) = make_uint2(u::pack_bf16(v[0], v[V > 1 ? 1 : 0]), u::pack_bf16(v[V > 2 ? 2 : 0], v[V > 3 ? 3 : 0]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) finish_one(a, cols, m, c + k, v[k]);
+    }
   }
 }
 
@@ -587,9 +617,9 @@ bool map_fits(const void* p, long long rows, long long stride) {
   return ((uintptr_t)p & 15) == 0 && stride % 8 == 0 && rows <= 0x7fffffffLL && stride < (1LL << 38);
 }
 
-// Shape of the tiles for an M x N product over K, estimated in SM clocks: a pair's block of 64 k takes 2 bn on the tensor cores and
-// 256 + bn for its loads; 2500 to fill the pipeline and empty the last accumulator; split sums are written and read at DRAM speed and
-// cost a launch.  With `may_trans` the weights may be the tiles' rows (few tokens).
+// Shape of the tiles for an M x N product over K, estimated in SM clocks: a pair's block of 64 k takes 420 + 1.1 bn (measured at
+// bn 64 to 256); 2500 to fill the pipeline and empty the last accumulator; split sums are written and read, mostly in the L2, and cost a
+// launch.  With `may_trans` the weights may be the tiles' rows (few tokens).
 struct TileShape { int trans, bn, splits, kper; long long rt, ct; double cost; };
 TileShape find_tiles(long long M, long long N, long long K, bool may_trans) {
   const int pairs = 74, kb = (int)((K + 63) / 64);
@@ -600,12 +630,12 @@ TileShape find_tiles(long long M, long long N, long long K, bool may_trans) {
     for (int bn = 32; bn <= 256; bn += 32) {     // what an MMA of a pair takes
       if (bn > 32 && bn - 32 >= C) break;
       const long long ct = (C + bn - 1) / bn;
-      const double tk = 2.0 * bn > 256 + bn ? 2.0 * bn : 256 + bn;
+      const double tk = 420.0 + 1.1 * bn;
       for (int s = 1; s <= 32 && s <= kb; ++s) {
         const int kper = (kb + s - 1) / s;
         if ((kb + kper - 1) / kper != s) continue;
         const double units = (double)rt * ct * s, waves = (double)(long long)((units + pairs - 1) / pairs);
-        const double cost = waves * (kper * tk + 200.0) + 2500.0 + (s > 1 ? 4000.0 + 8.0 * s * M * N / 3400.0 : 0.0);
+        const double cost = waves * (kper * tk + 200.0) + 2500.0 + (s > 1 ? 4000.0 + 8.0 * s * M * N / 6000.0 : 0.0);
         if (cost < best.cost) best = TileShape{trans, bn, s, kper, rt, ct, cost};
       }
     }
@@ -654,8 +684,10 @@ int run_mm2(const char* what, const TileShape& t, Operand P, Operand Q, long lon
 #undef MM2_RUN
   SSD_CUDA_CHECK_LAUNCH(what);
   if (t.splits > 1) {
-    const long long n = (M * N + 255) / 256, most = (long long)sm_count() * 8;
-    launch<k_mm2_join>((unsigned)(n < most ? n : most), 256, 0, s, a, M, N);
+    const bool four = N % 4 == 0 && o.os % 4 == 0 && ((uintptr_t)o.out & 7) == 0;
+    const long long n = (M * N / (four ? 4 : 1) + 255) / 256, most = (long long)sm_count() * 8;
+    if (four) launch<k_mm2_join<4>>((unsigned)(n < most ? n : most), 256, 0, s, a, M, (int)N);
+    else launch<k_mm2_join<1>>((unsigned)(n < most ? n : most), 256, 0, s, a, M, (int)N);
     SSD_CUDA_CHECK_LAUNCH("linear_join");
   }
   return SSD_OK;

@@ -808,21 +808,27 @@ __global__ void __launch_bounds__(S::TH, S::TH == 128 ? 4 : 1) k_sel_bwd(SelGeo 
   }
 }
 
-// dB, dC of a token and group: the channel blocks' shares in order.
+// dB, dC of a token and group: the channel blocks' shares in order.  Thread = four values of a token.
 template <typename T>
 __global__ void __launch_bounds__(256) k_sel_sum_bc(SelGeo q, int NP, const float* __restrict__ part, T* __restrict__ dB, T* __restrict__ dC) {
   pdl_wait();
-  const long long BL = (long long)q.B * q.L, n = BL * q.G * 2 * NP;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const int v = (int)(i % (2 * NP));
-    const long long k = i / (2 * NP), bl = k % BL;
-    const int g = (int)(k / BL), s = v % NP;
-    if (s >= q.N) continue;
-    float a = 0.f;
-#pragma unroll 4
-    for (int j = 0; j < q.nb; ++j) a += part[((long long)(g * q.nb + j) * BL + bl) * (2 * NP) + v];
-    stf((v < NP ? dB : dC) + (bl * q.G + g) * q.N + s, a);
+  const int V = NP / 2;                              // fours per token: dB, then dC
+  const long long BL = (long long)q.B * q.L, n = BL * V, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int g = blockIdx.y;
+  const float4* p = reinterpret_cast<const float4*>(part) + (long long)g * q.nb * n + i;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int j = 0; j < q.nb; ++j) {
+    const float4 f = __ldg(p + j * n);
+    a.x += f.x; a.y += f.y; a.z += f.z; a.w += f.w;
   }
+  const long long bl = i / V;
+  const int v = (int)(i - bl * V) * 4, s = v % NP;
+  T* o = (v < NP ? dB : dC) + (bl * q.G + g) * q.N + s;
+  const float f[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) if (s + k < q.N) stf(o + k, f[k]);
 }
 
 // dA, dD, ddt_bias: the batch rows' (and parts') shares; eight threads per value, in a fixed order.
@@ -852,57 +858,66 @@ __global__ void __launch_bounds__(256) k_sel_sum_par(SelGeo q, int NP, const flo
 
 // ---------------------------------------------------------------------------------------------
 // One step over many streams, in place on the state: the state is read and written once, everything else is small beside it.
-// Four states per thread, dstate / 4 lanes per channel.
+// Four states per thread, dstate / 4 lanes per channel; a thread takes U streams `groups` apart, whose states it asks for together, and
+// reads what belongs to the channel once.
 struct SelStep {
-  int S, D, N, G, Dg, softplus;
+  int S, D, N, G, Dg, softplus, groups, nx;          // nx = blocks of 256 threads over the channels' lanes
   long long xs, dts, bs, cs, zs, ys;
 };
-template <typename T, int LPC, bool VEC>
+template <typename T, int LPC, bool VEC, int U>
 __global__ void __launch_bounds__(256) k_sel_step(SelStep q, SsdStepPtrs p) {
   pdl_wait();
-  const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) / LPC, n = (long long)q.S * q.D;
-  const int nl = threadIdx.x % LPC;
-  const bool live = item < n;
-  const long long i = live ? item : 0;
-  const int s = (int)(i / q.D), d = (int)(i - (long long)s * q.D), g = d / q.Dg;
-  float* hp = p.state + i * q.N + nl * 4;
-  const float* ap = p.A + (long long)d * q.N + nl * 4;
-  const T* bp = (const T*)p.Bm + s * q.bs + (long long)g * q.N + nl * 4;
-  const T* cp = (const T*)p.Cm + s * q.cs + (long long)g * q.N + nl * 4;
-  float h[4], a[4];
-  if (VEC) {
-    const float4 v = *reinterpret_cast<const float4*>(hp), w = __ldg(reinterpret_cast<const float4*>(ap));
-    h[0] = v.x; h[1] = v.y; h[2] = v.z; h[3] = v.w;
-    a[0] = w.x; a[1] = w.y; a[2] = w.z; a[3] = w.w;
-  } else {
+  const int s0 = blockIdx.x / q.nx, unit = (blockIdx.x - s0 * q.nx) * 256 + threadIdx.x;
+  const bool live = unit / LPC < q.D;
+  const int d = live ? unit / LPC : q.D - 1, nl = unit % LPC, n0 = nl * 4, g = d / q.Dg;
+  float h[U][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool ok = nl * 4 + j < q.N;
-      h[j] = ok ? hp[j] : 0.f; a[j] = ok ? __ldg(ap + j) : 0.f;
+  for (int u = 0; u < U; ++u) {
+    const long long s = min(s0 + u * q.groups, q.S - 1);
+    const float* hp = p.state + (s * q.D + d) * q.N + n0;
+    if (VEC) {
+      const float4 v = *reinterpret_cast<const float4*>(hp);
+      h[u][0] = v.x; h[u][1] = v.y; h[u][2] = v.z; h[u][3] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[u][j] = n0 + j < q.N ? hp[j] : 0.f;
     }
   }
-  const float x = (float)((const T*)p.x)[s * q.xs + d];
-  const float st = sel_step((float)((const T*)p.dt)[s * q.dts + d], p.dt_bias ? __ldg(p.dt_bias + d) : 0.f, q.softplus);
-  float y = 0.f;
+  float a[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const bool ok = VEC || nl * 4 + j < q.N;
-    const float b = ok ? (float)bp[j] : 0.f, c = ok ? (float)cp[j] : 0.f;
-    h[j] = fmaf(ex2(st * (a[j] * LOG2E)), h[j], st * x * b);
-    y = fmaf(c, h[j], y);
-  }
-  if (live) {
-    if (VEC) *reinterpret_cast<float4*>(hp) = make_float4(h[0], h[1], h[2], h[3]);
-    else
+  for (int j = 0; j < 4; ++j) a[j] = n0 + j < q.N ? __ldg(p.A + (long long)d * q.N + n0 + j) * LOG2E : 0.f;
+  const float bias = p.dt_bias ? __ldg(p.dt_bias + d) : 0.f, Dv = p.D ? __ldg(p.D + d) : 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) if (nl * 4 + j < q.N) hp[j] = h[j];
-  }
+  for (int u = 0; u < U; ++u) {
+    const int si = s0 + u * q.groups;
+    if (si >= q.S) break;
+    const long long s = si;
+    const T* bp = (const T*)p.Bm + s * q.bs + (long long)g * q.N + n0;
+    const T* cp = (const T*)p.Cm + s * q.cs + (long long)g * q.N + n0;
+    const float x = (float)((const T*)p.x)[s * q.xs + d];
+    const float st = sel_step((float)((const T*)p.dt)[s * q.dts + d], bias, q.softplus);
+    float y = 0.f;
 #pragma unroll
-  for (int o = LPC / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-  if (live && nl == 0) {
-    if (p.D) y = fmaf(__ldg(p.D + d), x, y);
-    if (p.z) { const float z = (float)((const T*)p.z)[s * q.zs + d]; y *= z * sig(z); }
-    stf((T*)p.y + s * q.ys + d, y);
+    for (int j = 0; j < 4; ++j) {
+      const bool ok = VEC || n0 + j < q.N;
+      const float b = ok ? (float)bp[j] : 0.f, c = ok ? (float)cp[j] : 0.f;
+      h[u][j] = fmaf(ex2(st * a[j]), h[u][j], st * x * b);
+      y = fmaf(c, h[u][j], y);
+    }
+    float* hp = p.state + (s * q.D + d) * q.N + n0;
+    if (live) {
+      if (VEC) *reinterpret_cast<float4*>(hp) = make_float4(h[u][0], h[u][1], h[u][2], h[u][3]);
+      else
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (n0 + j < q.N) hp[j] = h[u][j];
+    }
+#pragma unroll
+    for (int o = LPC / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+    if (live && nl == 0) {
+      y = fmaf(Dv, x, y);
+      if (p.z) { const float z = (float)((const T*)p.z)[s * q.zs + d]; y *= z * sig(z); }
+      stf((T*)p.y + s * q.ys + d, y);
+    }
   }
 }
 
@@ -980,6 +995,7 @@ int make_sel_plan(const SsdSelDims* d, SelPlan* o) {
   o->nb_bwd = cdiv(q.Dg, block_channels_bwd(o->NP));
   q.nc = cdiv(q.L, SEL_C);
   q.wide = 0;
+  if (q.G > 65535 || (long long)q.B * q.L * (o->NP / 2) / 256 >= 0x7fffffffLL) { set_error("selscan: too many groups or tokens for one grid"); return SSD_ERR_UNSUPPORTED; }
   if ((long long)q.D * (o->NP + 2) > 0x7ffffff0LL) { set_error("selscan: too many channels (%d)", q.D); return SSD_ERR_UNSUPPORTED; }
   q.par_row = (q.D * (o->NP + 2) + 3) / 4 * 4;
   const long long GN = (long long)q.G * q.N;
@@ -1062,9 +1078,7 @@ template <typename T> int sel_backward(SelPlan pl, const SelBwd& p, const SsdSel
   SEL_SHAPE_BWD(SEL_RUN)
 #undef SEL_RUN
   SSD_CUDA_CHECK_LAUNCH("selscan_bwd");
-  const long long nbc = (long long)q.B * q.L * q.G * 2 * pl.NP;
-  const long long most = (long long)sm_count() * 16;
-  launch<k_sel_sum_bc<T>>((unsigned)((nbc + 255) / 256 < most ? (nbc + 255) / 256 : most), 256, 0, s, q, pl.NP, p.part_bc, (T*)u.dB, (T*)u.dC);
+  launch<k_sel_sum_bc<T>>(dim3((unsigned)(((long long)q.B * q.L * (pl.NP / 2) + 255) / 256), (unsigned)q.G), 256, 0, s, q, pl.NP, p.part_bc, (T*)u.dB, (T*)u.dC);
   SSD_CUDA_CHECK_LAUNCH("selscan_sum_bc");
   launch<k_sel_sum_par>((unsigned)(((long long)q.D * (pl.NP + 2) + 31) / 32), dim3(32, 8), 0, s, q, pl.NP, p.part_par, u.dA, u.dD, u.ddt_bias);
   SSD_CUDA_CHECK_LAUNCH("selscan_sum_par");
@@ -1156,17 +1170,23 @@ int32_t ssd_selscan_step(const SsdSelStepDims* d, const SsdStepPtrs* p, void* cu
     return SSD_ERR_BAD_SHAPE;
   }
   const int lpc = lanes_for(q.N);
-  const long long blocks = ((long long)q.S * q.D * lpc + 255) / 256;
+  if ((long long)q.D * lpc > 0x7fffff00LL) { set_error("selscan step: too many channels (%d)", q.D); return SSD_ERR_UNSUPPORTED; }
+  q.nx = (q.D * lpc + 255) / 256;
+  const bool four = (long long)q.S * q.nx >= 4LL * 148 * 8;   // four streams per thread where the SMs stay full
+  q.groups = four ? (q.S + 3) / 4 : q.S;
+  const long long blocks = (long long)q.groups * q.nx;
   if (blocks > 0x7fffffffLL) { set_error("selscan step: too many blocks for one grid (%lld)", blocks); return SSD_ERR_UNSUPPORTED; }
-  const bool vec = q.N == 4 * lpc && (((uintptr_t)p->state | (uintptr_t)p->A) & 15) == 0;
+  const bool vec = q.N == 4 * lpc && (((uintptr_t)p->state) & 15) == 0;
   cudaStream_t s = (cudaStream_t)cuda_stream;
+#define SEL_GO(T, LPC, VEC) do { \
+    if (four) launch<k_sel_step<T, LPC, VEC, 4>>((unsigned)blocks, 256, 0, s, q, *p); \
+    else launch<k_sel_step<T, LPC, VEC, 1>>((unsigned)blocks, 256, 0, s, q, *p); } while (0)
 #define SEL_RUN(LPC) do { \
-    if (d->dtype == SSD_BF16) { if (vec) launch<k_sel_step<__nv_bfloat16, LPC, true>>((unsigned)blocks, 256, 0, s, q, *p); \
-                                else launch<k_sel_step<__nv_bfloat16, LPC, false>>((unsigned)blocks, 256, 0, s, q, *p); } \
-    else { if (vec) launch<k_sel_step<float, LPC, true>>((unsigned)blocks, 256, 0, s, q, *p); \
-           else launch<k_sel_step<float, LPC, false>>((unsigned)blocks, 256, 0, s, q, *p); } } while (0)
+    if (d->dtype == SSD_BF16) { if (vec) SEL_GO(__nv_bfloat16, LPC, true); else SEL_GO(__nv_bfloat16, LPC, false); } \
+    else { if (vec) SEL_GO(float, LPC, true); else SEL_GO(float, LPC, false); } } while (0)
   switch (lpc) { case 1: SEL_RUN(1); break; case 2: SEL_RUN(2); break; case 4: SEL_RUN(4); break; case 8: SEL_RUN(8); break; default: SEL_RUN(16); }
 #undef SEL_RUN
+#undef SEL_GO
   SSD_CUDA_CHECK_LAUNCH("selscan_step");
   return SSD_OK;
 }

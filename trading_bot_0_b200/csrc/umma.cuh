@@ -215,6 +215,14 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// One lane of a converged warp, always the same.  Loads and MMAs issued under this, in loops that the whole warp runs, get their
+// addresses and descriptors from uniform registers; under `lane == 0` each operand is carried over one by one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // ---- CTA pairs (cta_group::2) ------------------------------------------------------------------
 // Two CTAs of a cluster on one accumulator tile of M = 256: each holds 128 rows of A and half the rows of B in its own shared
 // memory and the accumulator rows of its A in its own TMEM; the CTA of even rank (the leader) issues the MMAs for both.
