@@ -10,6 +10,7 @@
 // the gate) is computed once by one thread of the block, a tile of 16 tokens ahead, and handed over in shared memory.
 #include <initializer_list>
 
+#include "act.cuh"
 #include "common.cuh"
 #include "ssd_internal.h"
 #include "umma.cuh"
@@ -21,7 +22,6 @@ using umma::ex2;
 
 constexpr int SEL_T = 16;             // tokens per tile
 constexpr int SEL_C = 8;              // tokens between the states kept for the backward pass
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct SelGeo {
   int B, L, D, N, G, Dg, nb;          // nb = channel blocks per group
@@ -50,29 +50,10 @@ template <int KS_, int LPC_, int CHB_> struct Sh {
   template <typename T> static constexpr int bwd_smem() { return BWD_FLOATS * 4 + 3 * IT * TH * 4 * (int)sizeof(T); }    // .. with the raw values of its tasks
 };
 
-// log(1 + e) for e in [0, 1]: e P(e) with P the least-maximum fit of log1p(e) / e of degree 8 (relative error 3e-8, 1.7e-7 as
-// evaluated), so that small step sizes keep their digits where log(1 + e) would lose them.
-__device__ __forceinline__ float log1p01(float e) {
-  float p = 0.00523267664f;
-  p = fmaf(p, e, -0.0295051682f);
-  p = fmaf(p, e, 0.0782258369f);
-  p = fmaf(p, e, -0.13663236f);
-  p = fmaf(p, e, 0.191060022f);
-  p = fmaf(p, e, -0.24842981f);
-  p = fmaf(p, e, 0.333190967f);
-  p = fmaf(p, e, -0.499994931f);
-  p = fmaf(p, e, 0.99999997f);
-  return p * e;
-}
-// exp(-|v|), the rounding of the argument made good
-__device__ __forceinline__ float exp_neg(float v) {
-  const float x = -fabsf(v), t = x * LOG2E, r = fmaf(x, LOG2E, -t), e = ex2(t);
-  return fmaf(e, r * LN2, e);
-}
 // softplus(v) = max(v, 0) + log(1 + exp(-|v|))
 __device__ __forceinline__ float sel_step(float raw, float bias, int softplus) {
   const float v = raw + bias;
-  return softplus ? fmaxf(v, 0.f) + log1p01(exp_neg(v)) : v;
+  return softplus ? softplusf_(v) : v;
 }
 // the same, and its derivative 1 / (1 + exp(-v)) from the same exponential
 __device__ __forceinline__ float sel_step_d(float raw, float bias, int softplus, float& d) {
@@ -870,7 +851,11 @@ __global__ void __launch_bounds__(256) k_sel_step(SelStep q, SsdStepPtrs p) {
   const int s0 = blockIdx.x / q.nx, unit = (blockIdx.x - s0 * q.nx) * 256 + threadIdx.x;
   const bool live = unit / LPC < q.D;
   const int d = live ? unit / LPC : q.D - 1, nl = unit % LPC, n0 = nl * 4, g = d / q.Dg;
+  // everything that the U streams need is asked for before any of it is used (a stream past the last reads the last one's)
   float h[U][4];
+  T rx[U], rd[U], rz[U];
+  Raw4<T> rb[U], rc[U];
+  const int have = min(q.N - n0, 4);                 // states of this thread that are there
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const long long s = min(s0 + u * q.groups, q.S - 1);
@@ -880,42 +865,44 @@ __global__ void __launch_bounds__(256) k_sel_step(SelStep q, SsdStepPtrs p) {
       h[u][0] = v.x; h[u][1] = v.y; h[u][2] = v.z; h[u][3] = v.w;
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) h[u][j] = n0 + j < q.N ? hp[j] : 0.f;
+      for (int j = 0; j < 4; ++j) h[u][j] = j < have ? hp[j] : 0.f;
     }
+    rx[u] = ((const T*)p.x)[s * q.xs + d];
+    rd[u] = ((const T*)p.dt)[s * q.dts + d];
+    if (p.z) rz[u] = ((const T*)p.z)[s * q.zs + d];
+    const long long at = (long long)g * q.N + (have > 0 ? n0 : 0);
+    load4((const T*)p.Bm + s * q.bs + at, VEC, have > 0 ? have : 1, rb[u]);
+    load4((const T*)p.Cm + s * q.cs + at, VEC, have > 0 ? have : 1, rc[u]);
   }
   float a[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) a[j] = n0 + j < q.N ? __ldg(p.A + (long long)d * q.N + n0 + j) * LOG2E : 0.f;
+  for (int j = 0; j < 4; ++j) a[j] = j < have ? __ldg(p.A + (long long)d * q.N + n0 + j) * LOG2E : 0.f;
   const float bias = p.dt_bias ? __ldg(p.dt_bias + d) : 0.f, Dv = p.D ? __ldg(p.D + d) : 0.f;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int si = s0 + u * q.groups;
-    if (si >= q.S) break;
-    const long long s = si;
-    const T* bp = (const T*)p.Bm + s * q.bs + (long long)g * q.N + n0;
-    const T* cp = (const T*)p.Cm + s * q.cs + (long long)g * q.N + n0;
-    const float x = (float)((const T*)p.x)[s * q.xs + d];
-    const float st = sel_step((float)((const T*)p.dt)[s * q.dts + d], bias, q.softplus);
-    float y = 0.f;
+    const bool mine = live && s0 + u * q.groups < q.S;
+    const long long s = min(s0 + u * q.groups, q.S - 1);
+    float b[4], c[4], y = 0.f;
+    values4(rb[u], b); values4(rc[u], c);
+    const float x = (float)rx[u], st = sel_step((float)rd[u], bias, q.softplus);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const bool ok = VEC || n0 + j < q.N;
-      const float b = ok ? (float)bp[j] : 0.f, c = ok ? (float)cp[j] : 0.f;
-      h[u][j] = fmaf(ex2(st * a[j]), h[u][j], st * x * b);
-      y = fmaf(c, h[u][j], y);
+      if (!VEC && j >= have) b[j] = c[j] = 0.f;
+      h[u][j] = fmaf(ex2(st * a[j]), h[u][j], st * x * b[j]);
+      y = fmaf(c[j], h[u][j], y);
     }
     float* hp = p.state + (s * q.D + d) * q.N + n0;
-    if (live) {
+    if (mine) {
       if (VEC) *reinterpret_cast<float4*>(hp) = make_float4(h[u][0], h[u][1], h[u][2], h[u][3]);
       else
 #pragma unroll
-        for (int j = 0; j < 4; ++j) if (n0 + j < q.N) hp[j] = h[u][j];
+        for (int j = 0; j < 4; ++j) if (j < have) hp[j] = h[u][j];
     }
 #pragma unroll
     for (int o = LPC / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (live && nl == 0) {
+    if (mine && nl == 0) {
       y = fmaf(Dv, x, y);
-      if (p.z) { const float z = (float)((const T*)p.z)[s * q.zs + d]; y *= z * sig(z); }
+      if (p.z) { const float z = (float)rz[u]; y *= z * sig(z); }
       stf((T*)p.y + s * q.ys + d, y);
     }
   }
@@ -1176,7 +1163,8 @@ int32_t ssd_selscan_step(const SsdSelStepDims* d, const SsdStepPtrs* p, void* cu
   q.groups = four ? (q.S + 3) / 4 : q.S;
   const long long blocks = (long long)q.groups * q.nx;
   if (blocks > 0x7fffffffLL) { set_error("selscan step: too many blocks for one grid (%lld)", blocks); return SSD_ERR_UNSUPPORTED; }
-  const bool vec = q.N == 4 * lpc && (((uintptr_t)p->state) & 15) == 0;
+  const int es = d->dtype == SSD_BF16 ? 2 : 4;       // four states, and four values of B and C, at a time
+  const bool vec = q.N == 4 * lpc && ((uintptr_t)p->state & 15) == 0 && (((uintptr_t)p->Bm | (uintptr_t)p->Cm) & (4 * es - 1)) == 0 && q.bs % 4 == 0 && q.cs % 4 == 0;
   cudaStream_t s = (cudaStream_t)cuda_stream;
 #define SEL_GO(T, LPC, VEC) do { \
     if (four) launch<k_sel_step<T, LPC, VEC, 4>>((unsigned)blocks, 256, 0, s, q, *p); \
