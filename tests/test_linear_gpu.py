@@ -155,6 +155,16 @@ def test_gradients_against_differences(lib):
             assert abs(num - ana) <= tol, (act, name, num, ana, tol)
 
 
+@pytest.mark.parametrize("M", [5, 100, 700])
+def test_residual_in_place(lib, M):
+    """The residual's own memory as the output, for the kernels of few, some and many rows."""
+    from trading_bot_0_b200 import linear as LN
+    x, w, b, r, _ = (dev(v) for v in operands(M, 192, 520, "bf16", True, True))
+    want = LN.linear_forward(x, w, b, r, activation="silu")[0]
+    mine = r.clone()
+    assert torch.equal(LN.linear_forward(x, w, b, mine, activation="silu", out=mine)[0], want)
+
+
 @pytest.mark.parametrize("M", [2, 24, 300])
 def test_graph_and_stream(lib, M):
     from trading_bot_0_b200 import linear as LN
@@ -189,6 +199,10 @@ def test_operands_that_do_not_fit_are_refused(lib):
                      ((x, w), dict(out=torch.empty(6, 40, device=DEV)))):
         with pytest.raises(ValueError):
             LN.linear_forward(*args, **kw)
+    with pytest.raises(ValueError, match="overlaps"):
+        LN.linear_forward(x, torch.zeros(32, 32, dtype=torch.bfloat16, device=DEV), out=x)
+    inplace = r.clone()                                  # (the residual may be the output)
+    assert torch.equal(LN.linear_forward(x, w, b, inplace, out=inplace)[0], LN.linear_forward(x, w, b, r)[0])
     with pytest.raises(ValueError, match="pre"):
         LN.linear_backward(dout, x, w, activation="silu")
     with pytest.raises(ValueError):

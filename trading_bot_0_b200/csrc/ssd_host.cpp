@@ -635,6 +635,11 @@ void linear_fwd(const Tensor& x, const Tensor& w, const Tensor* bias, const Tens
     d.residual_stride_row = apart(rr, 0);
   }
   if (out.defined()) {
+    auto shares = [&](const Tensor& t, int64_t rows, int64_t stride, int64_t features) {   // bytes with `out`
+      const char *a = (const char*)t.data_ptr(), *b = (const char*)out.data_ptr();
+      return a < b + out.nbytes() && b < a + ((rows - 1) * stride + features) * t.element_size();
+    };
+    if (shares(xr, xr.size(0), xr.stride(0), d.in_features) || shares(w, N, d.in_features, d.in_features)) fail("linear: out: overlaps x or weight");
     if (out.scalar_type() != x.scalar_type() || out.device() != dev || !out.is_contiguous() || out.dim() != x.dim() || out.numel() != d.rows * N || out.size(-1) != N)
       fail("linear: out: expected a contiguous tensor of x's leading dims with ", N, " values in the last, ", x.scalar_type(), " on ", dev,
            ", got ", out.sizes(), " ", out.scalar_type(), " on ", out.device());
