@@ -72,6 +72,7 @@ __device__ __forceinline__ void unpack_raw(const RawN<float, 8>& r, float (&v)[8
   v[0] = r.a.x; v[1] = r.a.y; v[2] = r.a.z; v[3] = r.a.w; v[4] = r.b.x; v[5] = r.b.y; v[6] = r.b.z; v[7] = r.b.w;
 }
 __device__ __forceinline__ void unpack_raw(const RawN<float, 4>& r, float (&v)[4]) { v[0] = r.a.x; v[1] = r.a.y; v[2] = r.a.z; v[3] = r.a.w; }
+__device__ __forceinline__ void unpack_raw(const RawN<float, 2>& r, float (&v)[2]) { v[0] = r.a.x; v[1] = r.a.y; }
 __device__ __forceinline__ uint32_t bfpack_(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -214,10 +215,20 @@ struct Carry {
   const int* lengths;      // [B], or null
   int tiles;               // per sequence
 };
+struct CarryBwd {          // backward: din and dhist dense
+  const void *dout, *dnew;
+  long long dout_sb, dout_sl;
+  void *din, *dhist;
+  int rows, tiles;         // register kernel: rows of items, tiles per sequence
+};
 __device__ __forceinline__ int carry_len(const SsdConvDims& d, const Carry& q, int b) {
   return q.lengths ? min(max(__ldg(q.lengths + b), 0), d.seqlen) : d.seqlen;
 }
 
+// backward: rows of ext that are there, where d.seqlen counts the history's K - 1 rows too
+__device__ __forceinline__ int carry_ext(const SsdConvDims& d, const Carry& q, int b, int K) {
+  return K - 1 + (q.lengths ? min(max(__ldg(q.lengths + b), 0), d.seqlen - (K - 1)) : d.seqlen - (K - 1));
+}
 // CARRY: rows before the sequence's first come from the history, and the CTAs of a sequence's first tile write the new one.
 template <typename T, int K, bool CARRY>
 __global__ void __launch_bounds__(CONVS_THREADS, CONVS_CTAS_PER_SM)
@@ -494,10 +505,14 @@ template <int K> struct ConvWalk {
   }
 };
 
-template <typename T, int K>
+// CARRY: the sequences are ext (history, then the input: d.seqlen counts both), rows of the gradient stand K - 1 later, rows before the
+// input's first go to dhist, and the gradient of the new history comes on top at its rows.  The sigmoid is exp and a division
+// there in both storage types: dweight and dbias are fp32.
+template <typename T, int K, bool CARRY>
 __global__ void __launch_bounds__(CONVS_THREADS, CONVB_CTAS_PER_SM)
 k_conv_bwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__ weight, const float* __restrict__ bias,
-              ConvSegs segs, T* __restrict__ din, long long din_stride_b, long long din_stride_l, float* __restrict__ partial) {
+              ConvSegs segs, T* __restrict__ din, long long din_stride_b, long long din_stride_l, float* __restrict__ partial, Carry q,
+              CarryBwd cg) {
   pdl_wait();
   constexpr int NC = 16 / (int)sizeof(T);            // channels per 16-byte copy piece
   constexpr int NP = 8 / (int)sizeof(T);             // channels per thread in the arithmetic
@@ -518,13 +533,16 @@ k_conv_bwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__
     if (a.live()) {
       const int t = a.s + rr, end = min(a.t1 + K - 1, d.seqlen);
       unsigned char* sp = ring + stage * CONVB_STAGE_BYTES + rr * CONVS_ROWB + cv * 16;
-      const T* si_ = ibase + (long long)a.b * d.in_stride_b + (long long)t * d.in_stride_l;
-      const T* sg = gbase + (long long)a.b * gsb + (long long)t * gsl;
+      const int lag = CARRY ? K - 1 : 0, len = CARRY ? carry_ext(d, q, a.b, K) : d.seqlen;   // len: rows of ext that are there
+      const T* si_ = ibase + (long long)a.b * d.in_stride_b + (long long)(t - lag) * d.in_stride_l;
+      const T* sg = gbase + (long long)a.b * gsb + (long long)(t - lag) * gsl;
 #pragma unroll
       for (int j = 0; j < CONVB_RS / 2; ++j) {
         const int tj = t + 2 * j;
-        const bool iok = cok && tj >= 0 && tj < end, gok = cok && tj >= a.t0 && tj < end;
-        cp_async16(sp + 2 * j * CONVS_ROWB, iok ? (const void*)si_ : (const void*)in, iok);
+        const bool old = CARRY && tj < K - 1;
+        const bool iok = cok && tj >= 0 && tj < end && tj < len && (!old || q.history), gok = cok && tj >= a.t0 && tj < end && tj < len && !old;
+        const T* from = old ? (const T*)q.history + ((long long)a.b * (K - 1) + tj) * d.channels + cc : si_;
+        cp_async16(sp + 2 * j * CONVS_ROWB, iok ? (const void*)from : (const void*)in, iok);
         cp_async16(sp + (CONVB_RS + 2 * j) * CONVS_ROWB, gok ? (const void*)sg : (const void*)in, gok);
         si_ += 2 * d.in_stride_l; sg += 2 * gsl;
       }
@@ -568,7 +586,8 @@ k_conv_bwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__
     const unsigned char* sgo = sin + CONVB_RS * CONVS_ROWB;
     stage = stage + 1 == CONVB_STAGES ? 0 : stage + 1;
     const int end = min(cur.t1 + K - 1, d.seqlen);
-    T* dp = din + (long long)cur.b * din_stride_b + (long long)(cur.s - (K - 1)) * din_stride_l + c0;
+    T* dp = din + (long long)cur.b * din_stride_b + (long long)(cur.s - (K - 1) - (CARRY ? K - 1 : 0)) * din_stride_l + c0;
+    const int clen = CARRY ? carry_ext(d, q, cur.b, K) - (K - 1) : 0;
     auto rows8 = [&](auto whole) {   // WHOLE: every row of the stage is the share's own and completes a row of din
       constexpr bool WHOLE = decltype(whole)::value;
       const bool act = WHOLE || d.activation;
@@ -593,7 +612,8 @@ k_conv_bwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__
               for (int k = 0; k < K; ++k) a2 = fma2(w[j][k], win[k][j], a2);
               float a0, a1;
               unpack2(a2, a0, a1);
-              const float s0 = sig_<T>(a0), s1 = sig_<T>(a1);
+              typedef typename std::conditional<CARRY, float, T>::type S;
+              const float s0 = sig_<S>(a0), s1 = sig_<S>(a1);
               // silu'(a) = s (1 + a (1 - s))
               g = fma2(g, pack2(fmaf(s0, fmaf(-a0, s0, a0), s0), fmaf(s1, fmaf(-a1, s1, a1), s1)), 0ull);
             }
@@ -617,7 +637,21 @@ k_conv_bwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__
             for (int q = 0; q < K; ++q) a2 = fma2(w[j][K - 1 - q], dwin[q][j], a2);
             unpack2(a2, o[2 * j], o[2 * j + 1]);
           }
-          store_n(dp, o);
+          if (CARRY && !WHOLE) {
+            const int t = s - (K - 1), hr = t - clen;
+            if (cg.dnew && hr >= 0 && hr < K - 1) {
+              RawN<T, NP> r;
+              float v[NP];
+              lds_raw<T, NP>((const T*)cg.dnew + ((long long)cur.b * (K - 1) + hr) * d.channels + c0, r);
+              unpack_raw(r, v);
+#pragma unroll
+              for (int j = 0; j < NP; ++j) o[j] += v[j];
+            }
+            if (t >= K - 1) store_n(dp, o);
+            else if (cg.dhist) store_n((T*)cg.dhist + ((long long)cur.b * (K - 1) + t) * d.channels + c0, o);
+          } else {
+            store_n(dp, o);
+          }
         }
         dp += din_stride_l;
 #pragma unroll
@@ -626,7 +660,8 @@ k_conv_bwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__
           for (int j = 0; j < NH; ++j) { win[k][j] = win[k + 1][j]; dwin[k][j] = dwin[k + 1][j]; }
       }
     };
-    if (d.activation && cur.s >= cur.t0 + K - 1 && cur.s + CONVB_RS <= cur.t1) rows8(std::true_type());
+    if (d.activation && cur.s >= cur.t0 + K - 1 && cur.s + CONVB_RS <= cur.t1 &&
+        (!CARRY || (cur.s >= 2 * (K - 1) && cur.s + CONVB_RS - K < clen))) rows8(std::true_type());
     else rows8(std::false_type());
   }
   cp_async_wait<0>();
@@ -1056,12 +1091,6 @@ __global__ void __launch_bounds__(CONV_THREADS) k_carry_fwd(SsdConvDims d, Carry
 // ext rows) pairs, counts dpre of its own rows into dweight and dbias (tile sums first, then their sum) and leaves one partial row.
 // The sigmoid is exp and a division here in both storage types: dweight and dbias are fp32.
 constexpr int CARRY_TLB = 64, CARRY_ROWS = 1024;
-struct CarryBwd {
-  const void *dout, *dnew;
-  long long dout_sb, dout_sl;
-  void *din, *dhist;
-  int rows, tiles;
-};
 template <typename T, int K>
 __global__ void __launch_bounds__(CONV_THREADS) k_carry_bwd(SsdConvDims d, Carry q, CarryBwd g, const T* __restrict__ in,
                                                             const float* __restrict__ weight, const float* __restrict__ bias,
@@ -1256,6 +1285,23 @@ int norm_blocks(const SsdNormDims* d) {
   return (int)(need < 1184 ? need : 1184);
 }
 
+// Backward with a history: staged where a row fills half a channel block, as without one.  Blocks of a channel block, which are the rows
+// of partial sums: what fits the SMs and the tokens' shares.
+bool carry_staged(const SsdConvDims* d) { return (long long)d->channels * (d->dtype == SSD_BF16 ? 2 : 4) >= CONVS_ROWB / 2; }
+SsdConvDims carry_ext_dims(const SsdConvDims* d) {
+  SsdConvDims e = *d;
+  e.seqlen += d->width - 1;
+  return e;
+}
+long long carry_partials(const SsdConvDims* d) {
+  if (!carry_staged(d)) return carry_rows(d);
+  const SsdConvDims e = carry_ext_dims(d);
+  const int ncb = (d->channels * (d->dtype == SSD_BF16 ? 2 : 4) + CONVS_ROWB - 1) / CONVS_ROWB;
+  long long nx = 148LL * CONVB_CTAS_PER_SM / ncb;
+  if (nx > conv_shares(&e)) nx = conv_shares(&e);
+  return nx < 1 ? 1 : nx;
+}
+
 int check_conv(const SsdConvDims* d) {
   if (!d) { set_error("dims is NULL"); return SSD_ERR_NULL_POINTER; }
   if (d->batch <= 0 || d->seqlen <= 0 || d->channels <= 0) { set_error("conv1d: batch, seqlen and channels must be positive"); return SSD_ERR_BAD_SHAPE; }
@@ -1378,7 +1424,7 @@ int32_t ssd_conv1d_backward(const SsdConvDims* dims, const void* in, const float
     if (nx < 1) nx = 1;
     const dim3 grid((unsigned)nx, (unsigned)ncb);
 #define CONV_BWD_SM(T, K) \
-      launch<k_conv_bwd_sm<T, K>>(grid, CONVS_THREADS, CONVB_SMEM, s, *dims, (const T*)in, weight, bias, segs, (T*)din, din_stride_b, din_stride_l, partial)
+      launch<k_conv_bwd_sm<T, K, false>>(grid, CONVS_THREADS, CONVB_SMEM, s, *dims, (const T*)in, weight, bias, segs, (T*)din, din_stride_b, din_stride_l, partial, Carry{}, CarryBwd{})
     if (dims->dtype == SSD_BF16) {
       if (dims->width == 4) CONV_BWD_SM(__nv_bfloat16, 4); else if (dims->width == 3) CONV_BWD_SM(__nv_bfloat16, 3); else CONV_BWD_SM(__nv_bfloat16, 2);
     } else {
@@ -1471,7 +1517,7 @@ int32_t ssd_conv1d_carry_forward(const SsdConvDims* dims, const void* in, const 
 size_t ssd_conv1d_carry_workspace_bytes(const SsdConvDims* dims) {
   clear_error();
   if (check_conv(dims)) return 0;
-  return (size_t)carry_rows(dims) * dims->channels * (dims->width + 1) * sizeof(float);
+  return (size_t)carry_partials(dims) * dims->channels * (dims->width + 1) * sizeof(float);
 }
 
 int32_t ssd_conv1d_carry_backward(const SsdConvDims* dims, const void* in, const float* weight, const float* bias, const void* history,
@@ -1487,17 +1533,34 @@ int32_t ssd_conv1d_carry_backward(const SsdConvDims* dims, const void* in, const
     set_error("conv1d carry backward: dout rows must cover the channels, strides multiples of 16 bytes");
     return SSD_ERR_BAD_ALIGNMENT;
   }
-  const size_t need = (size_t)carry_rows(dims) * dims->channels * (dims->width + 1) * sizeof(float);
+  const size_t need = (size_t)carry_partials(dims) * dims->channels * (dims->width + 1) * sizeof(float);
   if (workspace_bytes < need) { set_error("conv1d carry backward: workspace too small: %zu < %zu", workspace_bytes, need); return SSD_ERR_WORKSPACE_TOO_SMALL; }
   cudaStream_t s = (cudaStream_t)cuda_stream;
   const Carry q{history, lengths, 0};
   const CarryBwd g{dout, dnew_history, dout_stride_b, dout_stride_l, din, dhistory, carry_rows(dims), carry_bwd_tiles(dims)};
+  const int n = dims->channels * (dims->width + 1);
+  if (carry_staged(dims)) {
+    const SsdConvDims e = carry_ext_dims(dims);
+    const int ncb = (dims->channels * es + CONVS_ROWB - 1) / CONVS_ROWB;
+    if (ncb > 65535) { set_error("conv1d carry backward: too many channels"); return SSD_ERR_UNSUPPORTED; }
+    const int nx = (int)carry_partials(dims);
+    ConvSegs segs;
+    for (int i = 0; i < 3; ++i) { segs.ptr[i] = i ? nullptr : dout; segs.c_begin[i] = i ? 0x7fffffff : 0; segs.stride_b[i] = i ? 0 : dout_stride_b; segs.stride_l[i] = i ? 0 : dout_stride_l; }
+    segs.n = 1;
+#define CARRY_RUN(T, K) launch<k_conv_bwd_sm<T, K, true>>(dim3((unsigned)nx, (unsigned)ncb), CONVS_THREADS, CONVB_SMEM, s, e, (const T*)in, weight, bias, segs, (T*)din, \
+                                                          (long long)dims->seqlen * dims->channels, (long long)dims->channels, (float*)workspace, q, g)
+    CARRY_BY_TYPE(CARRY_RUN);
+#undef CARRY_RUN
+    SSD_CUDA_CHECK_LAUNCH("conv1d_carry_bwd");
+    launch<k_conv_reduce>((n + 31) / 32, dim3(32, RED_GROUPS), 0, s, nx, dims->channels, dims->width, (const float*)workspace, dweight, dbias);
+    SSD_CUDA_CHECK_LAUNCH("conv1d_carry_reduce");
+    return SSD_OK;
+  }
   const unsigned grid = (unsigned)(((long long)g.rows * (dims->channels / 4) + CONV_THREADS - 1) / CONV_THREADS);
 #define CARRY_RUN(T, K) launch<k_carry_bwd<T, K>>(grid, CONV_THREADS, 0, s, *dims, q, g, (const T*)in, weight, bias, (float*)workspace)
   CARRY_BY_TYPE(CARRY_RUN);
 #undef CARRY_RUN
   SSD_CUDA_CHECK_LAUNCH("conv1d_carry_bwd");
-  const int n = dims->channels * (dims->width + 1);
   launch<k_conv_reduce>((n + 31) / 32, dim3(32, RED_GROUPS), 0, s, g.rows, dims->channels, dims->width, (const float*)workspace, dweight, dbias);
   SSD_CUDA_CHECK_LAUNCH("conv1d_carry_reduce");
   return SSD_OK;
