@@ -324,7 +324,10 @@ k_conv_fwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__
         unpack2(a2, a, b);
         o[2 * j] = d.activation ? a * sig_<T>(a) : a;
         o[2 * j + 1] = d.activation ? b * sig_<T>(b) : b;
-        if (CARRY && t0 + i >= len) o[2 * j] = o[2 * j + 1] = 0.f;
+      }
+      if (CARRY && t0 + i >= len) {                  // (the same for a whole warp)
+#pragma unroll
+        for (int j = 0; j < NP; ++j) o[j] = 0.f;
       }
       if (t0 + i < d.seqlen) store_n(op, o);
       op += d.out_stride_l;

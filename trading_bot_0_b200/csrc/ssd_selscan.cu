@@ -789,19 +789,30 @@ __global__ void __launch_bounds__(S::TH, S::TH == 128 ? 4 : 1) k_sel_bwd(SelGeo 
   }
 }
 
-// dB, dC of a token and group: the channel blocks' shares in order.  Thread = four values of a token.
+// dB, dC of a token and group: the channel blocks' shares.  64 times four values to a block; four threads take every fourth share each,
+// and their sums are added in order.
 template <typename T>
 __global__ void __launch_bounds__(256) k_sel_sum_bc(SelGeo q, int NP, const float* __restrict__ part, T* __restrict__ dB, T* __restrict__ dC) {
+  __shared__ float4 sum[3][64];
   pdl_wait();
-  const int V = NP / 2;                              // fours per token: dB, then dC
-  const long long BL = (long long)q.B * q.L, n = BL * V, i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
+  const int V = NP / 2, lane = threadIdx.x & 63, r = threadIdx.x >> 6;   // V fours per token: dB, then dC
+  const long long BL = (long long)q.B * q.L, n = BL * V, i = (long long)blockIdx.x * 64 + lane;
   const int g = blockIdx.y;
-  const float4* p = reinterpret_cast<const float4*>(part) + (long long)g * q.nb * n + i;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (i < n) {
+    const float4* p = reinterpret_cast<const float4*>(part) + (long long)g * q.nb * n + i;
 #pragma unroll 8
-  for (int j = 0; j < q.nb; ++j) {
-    const float4 f = __ldg(p + j * n);
+    for (int j = r; j < q.nb; j += 4) {
+      const float4 f = __ldg(p + j * n);
+      a.x += f.x; a.y += f.y; a.z += f.z; a.w += f.w;
+    }
+  }
+  if (r) sum[r - 1][lane] = a;
+  __syncthreads();
+  if (r || i >= n) return;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const float4 f = sum[k][lane];
     a.x += f.x; a.y += f.y; a.z += f.z; a.w += f.w;
   }
   const long long bl = i / V;
@@ -851,59 +862,74 @@ __global__ void __launch_bounds__(256) k_sel_step(SelStep q, SsdStepPtrs p) {
   const int s0 = blockIdx.x / q.nx, unit = (blockIdx.x - s0 * q.nx) * 256 + threadIdx.x;
   const bool live = unit / LPC < q.D;
   const int d = live ? unit / LPC : q.D - 1, nl = unit % LPC, n0 = nl * 4, g = d / q.Dg;
-  // everything that the U streams need is asked for before any of it is used (a stream past the last reads the last one's)
+  // everything that the U streams need is asked for before any of it is used (a stream past the last reads the first one's)
   float h[U][4];
   T rx[U], rd[U], rz[U];
   Raw4<T> rb[U], rc[U];
   const int have = min(q.N - n0, 4);                 // states of this thread that are there
+  const long long at = (long long)g * q.N + (have > 0 ? n0 : 0);
+  float* const hp = p.state + ((long long)s0 * q.D + d) * q.N + n0;
+  const T *xp = (const T*)p.x + s0 * q.xs + d, *dtp = (const T*)p.dt + s0 * q.dts + d, *zp = (const T*)p.z + s0 * q.zs + d;
+  const T *bp = (const T*)p.Bm + s0 * q.bs + at, *cp = (const T*)p.Cm + s0 * q.cs + at;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const long long s = min(s0 + u * q.groups, q.S - 1);
-    const float* hp = p.state + (s * q.D + d) * q.N + n0;
+    const long long k = s0 + u * q.groups < q.S ? (long long)u * q.groups : 0;
+    const float* hu = hp + k * q.D * q.N;
     if (VEC) {
-      const float4 v = *reinterpret_cast<const float4*>(hp);
+      const float4 v = *reinterpret_cast<const float4*>(hu);
       h[u][0] = v.x; h[u][1] = v.y; h[u][2] = v.z; h[u][3] = v.w;
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) h[u][j] = j < have ? hp[j] : 0.f;
+      for (int j = 0; j < 4; ++j) h[u][j] = j < have ? hu[j] : 0.f;
     }
-    rx[u] = ((const T*)p.x)[s * q.xs + d];
-    rd[u] = ((const T*)p.dt)[s * q.dts + d];
-    if (p.z) rz[u] = ((const T*)p.z)[s * q.zs + d];
-    const long long at = (long long)g * q.N + (have > 0 ? n0 : 0);
-    load4((const T*)p.Bm + s * q.bs + at, VEC, have > 0 ? have : 1, rb[u]);
-    load4((const T*)p.Cm + s * q.cs + at, VEC, have > 0 ? have : 1, rc[u]);
+    rx[u] = xp[k * q.xs];
+    rd[u] = dtp[k * q.dts];
+    if (p.z) rz[u] = zp[k * q.zs];
+    load4(bp + k * q.bs, VEC, have > 0 ? have : 1, rb[u]);
+    load4(cp + k * q.cs, VEC, have > 0 ? have : 1, rc[u]);
   }
   float a[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) a[j] = j < have ? __ldg(p.A + (long long)d * q.N + n0 + j) * LOG2E : 0.f;
   const float bias = p.dt_bias ? __ldg(p.dt_bias + d) : 0.f, Dv = p.D ? __ldg(p.D + d) : 0.f;
+  // a channel's lanes share out the softplus of its streams
+  float step[U];
+  if (U > 1 && LPC >= U) {
+    float mine = (float)rd[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u) mine = nl % U == u ? (float)rd[u] : mine;
+    mine = sel_step(mine, bias, q.softplus);
+#pragma unroll
+    for (int u = 0; u < U; ++u) step[u] = __shfl_sync(0xffffffffu, mine, u, LPC);
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) step[u] = sel_step((float)rd[u], bias, q.softplus);
+  }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const bool mine = live && s0 + u * q.groups < q.S;
-    const long long s = min(s0 + u * q.groups, q.S - 1);
     float b[4], c[4], y = 0.f;
     values4(rb[u], b); values4(rc[u], c);
-    const float x = (float)rx[u], st = sel_step((float)rd[u], bias, q.softplus);
+    const float x = (float)rx[u], sx = step[u] * x;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (!VEC && j >= have) b[j] = c[j] = 0.f;
-      h[u][j] = fmaf(ex2(st * a[j]), h[u][j], st * x * b[j]);
+      h[u][j] = fmaf(ex2(step[u] * a[j]), h[u][j], sx * b[j]);
       y = fmaf(c[j], h[u][j], y);
     }
-    float* hp = p.state + (s * q.D + d) * q.N + n0;
     if (mine) {
-      if (VEC) *reinterpret_cast<float4*>(hp) = make_float4(h[u][0], h[u][1], h[u][2], h[u][3]);
+      float* hu = hp + (long long)u * q.groups * q.D * q.N;
+      if (VEC) *reinterpret_cast<float4*>(hu) = make_float4(h[u][0], h[u][1], h[u][2], h[u][3]);
       else
 #pragma unroll
-        for (int j = 0; j < 4; ++j) if (j < have) hp[j] = h[u][j];
+        for (int j = 0; j < 4; ++j) if (j < have) hu[j] = h[u][j];
     }
 #pragma unroll
     for (int o = LPC / 2; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
     if (mine && nl == 0) {
       y = fmaf(Dv, x, y);
       if (p.z) { const float z = (float)rz[u]; y *= z * sig(z); }
-      stf((T*)p.y + s * q.ys + d, y);
+      stf((T*)p.y + (s0 + (long long)u * q.groups) * q.ys + d, y);
     }
   }
 }
@@ -982,7 +1008,7 @@ int make_sel_plan(const SsdSelDims* d, SelPlan* o) {
   o->nb_bwd = cdiv(q.Dg, block_channels_bwd(o->NP));
   q.nc = cdiv(q.L, SEL_C);
   q.wide = 0;
-  if (q.G > 65535 || (long long)q.B * q.L * (o->NP / 2) / 256 >= 0x7fffffffLL) { set_error("selscan: too many groups or tokens for one grid"); return SSD_ERR_UNSUPPORTED; }
+  if (q.G > 65535 || (long long)q.B * q.L * (o->NP / 2) / 64 >= 0x7fffffffLL) { set_error("selscan: too many groups or tokens for one grid"); return SSD_ERR_UNSUPPORTED; }
   if ((long long)q.D * (o->NP + 2) > 0x7ffffff0LL) { set_error("selscan: too many channels (%d)", q.D); return SSD_ERR_UNSUPPORTED; }
   q.par_row = (q.D * (o->NP + 2) + 3) / 4 * 4;
   const long long GN = (long long)q.G * q.N;
@@ -1065,7 +1091,7 @@ template <typename T> int sel_backward(SelPlan pl, const SelBwd& p, const SsdSel
   SEL_SHAPE_BWD(SEL_RUN)
 #undef SEL_RUN
   SSD_CUDA_CHECK_LAUNCH("selscan_bwd");
-  launch<k_sel_sum_bc<T>>(dim3((unsigned)(((long long)q.B * q.L * (pl.NP / 2) + 255) / 256), (unsigned)q.G), 256, 0, s, q, pl.NP, p.part_bc, (T*)u.dB, (T*)u.dC);
+  launch<k_sel_sum_bc<T>>(dim3((unsigned)(((long long)q.B * q.L * (pl.NP / 2) + 63) / 64), (unsigned)q.G), 256, 0, s, q, pl.NP, p.part_bc, (T*)u.dB, (T*)u.dC);
   SSD_CUDA_CHECK_LAUNCH("selscan_sum_bc");
   launch<k_sel_sum_par>((unsigned)(((long long)q.D * (pl.NP + 2) + 31) / 32), dim3(32, 8), 0, s, q, pl.NP, p.part_par, u.dA, u.dD, u.ddt_bias);
   SSD_CUDA_CHECK_LAUNCH("selscan_sum_par");
