@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(256) k_join(MmArgs a) {
 
 // Few rows (up to eight tokens): bound by one reading of the weights and, below some megabytes, by latency, so one launch and every
 // load of a weight row in flight at once.  Warp = F output features and all tokens, lane = 16 bytes of k at a time; x comes out of
-// the L1, F features share a reading of it.
+// the L1, F features share a reading of it.  4 x 1536 x 768: 5.5 us, a launch and one latency.
 template <typename T, int RM, int F>
 __global__ void __launch_bounds__(256) k_mm_few(MmArgs a) {
   constexpr int V = 16 / (int)sizeof(T);
@@ -211,8 +211,9 @@ __global__ void __launch_bounds__(256) k_mm_few(MmArgs a) {
 // sums in the workspace and k_mm2_join adds them in order.  Every wait is bounded: when one runs out a code goes to the status word and
 // the outputs become NaN.
 //
-// Measured, 8192^3: 677 us = 1.62 PFLOP/s (cuBLAS 640 to 680 on the same boards), 4096 x 2048 x 2048 34 us (36); 785 us with loads and
-// MMAs issued by `lane == 0` instead of an elected lane, whatever the tile's width; four stages are as fast as five, three 10 % slower;
+// Measured with cuBLAS beside it in one run: 8192^3 694 us = 1.58 PFLOP/s (647), 16384 x 768 x 3352 76 (72), 4096 x 2048 x 2048 45 (41),
+// 512 x 768 x 1536 14 (8).  8192^3 before and after on one board: 785 us with loads and MMAs issued by `lane == 0`, 677 by an elected
+// lane, whatever the tile's width; four stages are as fast as five, three 10 % slower;
 // both accumulators as one tile of 256 x 512, which loads a quarter less, 670 us, but 103 against 77 us at 16384 x 768 x 3352, where
 // its epilogue is not hidden.
 namespace u = umma;
