@@ -454,7 +454,8 @@ SSD_API int32_t ssd_conv1d_step(const SsdConvDims* dims, const void* in, const f
  * the tensor cores; all other sizes, strides and fp32 on the CUDA cores in fp32.  `pre` (optional, dense, fp32) receives
  * x W^T + bias for the backward, which needs it where act is not NONE.  Backward: dpre = dout * act'(pre), dx = dpre W,
  * dweight = dpre^T x, dbias = sum of dpre over the rows; each of the three is optional.
- * `out` may be the residual, but must not overlap x or weight.
+ * `out` may be the residual (same address, same row stride), and must
+ * not overlap it otherwise, nor x, weight or bias.
  */
 typedef enum SsdAct { SSD_ACT_NONE = 0, SSD_ACT_SILU = 1, SSD_ACT_SOFTPLUS = 2, SSD_ACT_RELU2 = 3 } SsdAct;   /* RELU2: max(v,0)^2 */
 typedef struct SsdLinearDims {

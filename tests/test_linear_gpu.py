@@ -209,3 +209,18 @@ def test_operands_that_do_not_fit_are_refused(lib):
         LN.linear_backward(dout[:, :-1], x, w)
     with pytest.raises(T._lib.SsdError, match="positive"):
         LN.linear_forward(x[:0], w)
+
+
+def test_output_that_overlaps_a_part_of_the_residual_is_refused(lib):
+    """Blocks would read values of the residual that others have written; refused before any launch."""
+    from trading_bot_0_b200 import linear as LN
+    x, w, b, _, _ = (dev(v) for v in operands(6, 32, 40, "bf16", True, True))
+    buf = torch.zeros(13 * 40, dtype=torch.bfloat16, device=DEV)
+    out = buf[:240].view(6, 40)
+    for r in (buf[40:280].view(6, 40), buf[8:248].view(6, 40), buf[:480].view(6, 80)[:, :40]):   # rows later, values later, rows further apart
+        with pytest.raises(ValueError, match="residual"):
+            LN.linear_forward(x, w, b, r, out=out)
+    with pytest.raises(ValueError, match="bias"):
+        LN.linear_forward(x, w, buf[200:240], out=out)
+    apart = buf[240:480].view(6, 40)                      # directly behind it: nothing shared
+    assert torch.equal(LN.linear_forward(x, w, b, apart, out=out)[0], LN.linear_forward(x, w, b, apart.clone())[0])

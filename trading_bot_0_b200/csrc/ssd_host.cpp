@@ -640,6 +640,10 @@ void linear_fwd(const Tensor& x, const Tensor& w, const Tensor* bias, const Tens
       return a < b + out.nbytes() && b < a + ((rows - 1) * stride + features) * t.element_size();
     };
     if (shares(xr, xr.size(0), xr.stride(0), d.in_features) || shares(w, N, d.in_features, d.in_features)) fail("linear: out: overlaps x or weight");
+    if (bias && shares(*bias, 1, 0, N)) fail("linear: out: overlaps bias");
+    // a value of the residual is read by the thread that writes the same element of `out`: its memory, or none of it
+    if (rr.defined() && !(rr.data_ptr() == out.data_ptr() && (d.rows == 1 || rr.stride(0) == N)) && shares(rr, d.rows, rr.stride(0), N))
+      fail("linear: out: overlaps a part of residual; it has to be the residual itself or apart from it");
     if (out.scalar_type() != x.scalar_type() || out.device() != dev || !out.is_contiguous() || out.dim() != x.dim() || out.numel() != d.rows * N || out.size(-1) != N)
       fail("linear: out: expected a contiguous tensor of x's leading dims with ", N, " values in the last, ", x.scalar_type(), " on ", dev,
            ", got ", out.sizes(), " ", out.scalar_type(), " on ", out.device());
