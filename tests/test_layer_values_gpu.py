@@ -34,3 +34,86 @@ def test_silu_of_the_convolution_keeps_its_tails(lib, dtype, C):
     many = dev(x[0]).repeat(40, 1)                       # streams enough for a thread to take several, the last ones fewer
     some = P.conv1d_step(torch.zeros(len(many), K - 1, C, dtype=t, device=DEV), many, dev(w))
     assert torch.equal(some.view(40, 641, C), step.expand(40, 641, C))
+
+
+def _scan(dtype, B=2, L=21, D=24, N=8, seed=7):
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g)
+    t = TD[dtype]
+    return dict(x=n(B, L, D).to(t), dt=(0.5 * n(B, L, D) - 2.0).to(t), A=-(0.2 + 4.0 * torch.rand(D, N, generator=g)), Bm=n(B, L, 1, N).to(t),
+                Cm=n(B, L, 1, N).to(t), D=n(D), z=n(B, L, D).to(t), init_state=n(B, D, N)), n(B, L, D).to(t), n(B, D, N)
+
+
+ORDER = ("x", "dt", "A", "Bm", "Cm", "D", "z", "init_state")
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_steps_that_are_switched_off(lib, dtype):
+    """A step size of -inf, or of the type's lowest value, is a softplus of 0: the token leaves the state as it is, bit for bit, and takes
+    no gradient; so does a channel whose bias is -inf.  Against the 64-bit recurrence with the bound of its own test."""
+    from tests.test_selective_gpu import assert_near, _tokens
+    from trading_bot_0_b200 import selective as S
+    o, dy, dfin = _scan(dtype)
+    B, L, D = o["x"].shape
+    N = o["A"].shape[1]
+    low = torch.finfo(TD[dtype]).min
+    o["dt"][:, 3] = -float("inf")
+    o["dt"][0, 5:9, ::2] = low
+    o["dt"][1, 10:18] = -2.4e38                           # (log2 e times this is past fp32)
+    o["dt"][:, -1] = -float("inf")
+    bias = torch.zeros(D)
+    bias[4] = -float("inf")
+    ref, mag = (O.selective_scan_ref(*(o[k] for k in ORDER), dt_bias=bias, dt_softplus=True, dy=dy, dfinal=dfin, magnitude=m) for m in (False, True))
+    tok = _tokens(o, dict(dt_bias=bias, dt_softplus=True), L)
+    a = [dev(o[k]) for k in ORDER]
+    kd = dict(dt_bias=dev(bias), dt_softplus=True)
+    y, fin, ws = S.selective_scan_forward(*a, for_backward=True, **kd)
+    assert_near("y", y, ref["y"], mag["y"], tok, N)
+    assert_near("final_state", fin, ref["final_state"], mag["final_state"], tok, 0)
+    assert torch.equal(fin[:, 4].cpu(), o["init_state"][:, 4])
+    g = S.selective_scan_backward(dev(dy), *a, dev(dfin), workspace=ws, **kd)
+    for k, terms in dict(dx=N, ddt=N, dz=N, dA=B * L, dD=B * L, ddt_bias=B * L + N, dB=D, dC=D, dinit=0).items():
+        assert_near(k, g[k], ref[k], mag[k], tok, terms)
+    assert (g["ddt"][:, 3] == 0).all() and (g["ddt"][..., 4] == 0).all()
+    st = a[7].clone()
+    ys = [S.selective_step(st, a[0][:, t], a[1][:, t], a[2], a[3][:, t], a[4][:, t], a[5], a[6][:, t], **kd) for t in range(L)]
+    assert_near("steps", torch.stack(ys, 1), ref["y"], mag["y"], tok, N)
+    before = st.clone()
+    S.selective_step(st, a[0][:, 3], a[1][:, 3], a[2], a[3][:, 3], a[4][:, 3], a[5], a[6][:, 3], **kd)
+    assert torch.equal(st, before)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_a_step_as_large_as_the_type(lib, dtype):
+    """softplus of the largest values is the value: with x = 0 there, everything is forgotten and nothing added."""
+    from trading_bot_0_b200 import selective as S
+    o, _, _ = _scan(dtype)
+    o["dt"][:, 6] = torch.finfo(TD[dtype]).max
+    o["x"][:, 6] = 0
+    a = [dev(o[k]) for k in ORDER]
+    y, _, _ = S.selective_scan_forward(*a, dt_softplus=True)
+    assert (y[:, 6] == 0).all() and torch.isfinite(y).all()
+    cut, _, _ = S.selective_scan_forward(*(v[:, 7:] if v.dim() > 2 and v.shape[1] == 21 else v for v in a[:7]), torch.zeros_like(a[7]), dt_softplus=True)
+    half = torch.finfo(TD[dtype]).eps
+    assert ((y[:, 7:] - cut).float().abs() <= half * cut.float().abs() + 2.0 ** -18).all()     # (tiles of 16 tokens start elsewhere)
+
+
+ENDS = [float("inf"), -float("inf"), float("nan"), 3.3e38, -3.3e38, 2.4e38, -2.4e38, 0.0]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("M,K", [(3, 64), (40, 64), (300, 64), (50, 33), (64, 1536)])    # few rows, tensor cores or CUDA cores, splits
+def test_softplus_of_the_projection_at_its_ends(lib, dtype, M, K):
+    """The pre-activation is the bias (x is zero): inf, 0, NaN, the value itself; slopes 1, 0, NaN."""
+    from trading_bot_0_b200 import linear as LN
+    N = 48
+    x, w = torch.zeros(M, K, dtype=TD[dtype]), torch.ones(N, K, dtype=TD[dtype])
+    b = torch.tensor(ENDS).repeat(N // len(ENDS)).to(TD[dtype])
+    want = torch.where(b < -1e30, 0.0, torch.where(b == 0, torch.log(torch.tensor(2.0)), b.float())).to(TD[dtype]).expand(M, N)
+    out, pre = LN.linear_forward(dev(x), dev(w), dev(b), activation="softplus", for_backward=True)
+    eps = torch.finfo(TD[dtype]).eps
+    assert torch.allclose(out.cpu().float(), want.float(), rtol=eps, atol=0, equal_nan=True)
+    _, _, db = LN.linear_backward(torch.ones(M, N, dtype=TD[dtype], device=DEV), dev(x), dev(w), pre, activation="softplus", want_dx=False,
+                                  want_dweight=False)
+    slope = torch.where(b.isnan(), b.float(), torch.sigmoid(b.float())) * M
+    assert torch.allclose(db.cpu().float(), slope, rtol=eps, atol=0, equal_nan=True)

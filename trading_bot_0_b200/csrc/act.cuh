@@ -20,10 +20,11 @@ __device__ __forceinline__ float log1p01(float e) {
   p = fmaf(p, e, 0.99999997f);
   return p * e;
 }
-// exp(-|v|), the rounding of the argument made good
+// exp(-|v|), the rounding of the argument made good where there is anything left of the result (t may be -inf, and is from |v| = 2.36e38
+// on: the remainder is no number then; a NaN stays one)
 __device__ __forceinline__ float exp_neg(float v) {
   const float x = -fabsf(v), t = x * LOG2E, r = fmaf(x, LOG2E, -t), e = umma::ex2(t);
-  return fmaf(e, r * LN2, e);
+  return t < -200.f ? e : fmaf(e, r * LN2, e);
 }
 __device__ __forceinline__ float softplusf_(float v) { return fmaxf(v, 0.f) + log1p01(exp_neg(v)); }
 
