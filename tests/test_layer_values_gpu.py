@@ -117,3 +117,31 @@ def test_softplus_of_the_projection_at_its_ends(lib, dtype, M, K):
                                   want_dweight=False)
     slope = torch.where(b.isnan(), b.float(), torch.sigmoid(b.float())) * M
     assert torch.allclose(db.cpu().float(), slope, rtol=eps, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("act", ["none", "silu", "softplus", "relu2"])
+@pytest.mark.parametrize("M,K,N", [(3, 64, 48), (3, 64, 8200), (40, 64, 48), (64, 1536, 128), (300, 64, 520), (50, 33, 40), (64, 1540, 40), (2100, 40, 1300)])
+def test_nan_goes_through_every_activation(lib, dtype, act, M, K, N):
+    """A NaN in one row of x or in one bias makes that row and that column NaN, in the output and in the gradients that meet it, and
+    nothing else; on the kernels of few rows, of the tensor cores (with and without splits) and of the CUDA cores."""
+    from trading_bot_0_b200 import linear as LN
+    g = torch.Generator().manual_seed(M + K)
+    n = lambda *s: torch.randn(*s, generator=g).to(TD[dtype])
+    x, w, b, r, dout = n(M, K), (n(N, K).float() / K ** 0.5).to(TD[dtype]), n(N), n(M, N), n(M, N)
+    x[1, 5], b[7] = float("nan"), float("nan")
+    bad = torch.zeros(M, N, dtype=torch.bool)
+    bad[1], bad[:, 7] = True, True
+    out, pre = LN.linear_forward(dev(x), dev(w), dev(b), dev(r), activation=act, for_backward=True)
+    assert torch.equal(out.isnan().cpu(), bad)
+    if act == "none":
+        return
+    dx, dw, db = LN.linear_backward(dev(dout), dev(x), dev(w), pre, activation=act)
+    assert db.isnan().all()                               # (every column has the bad row in its sum)
+    assert dx.isnan().all()                               # (every row has the bad column)
+    finite = x.clone()
+    finite[1, 5] = 0.5
+    _, pre = LN.linear_forward(dev(finite), dev(w), dev(b), dev(r), activation=act, for_backward=True)
+    dx, dw, db = LN.linear_backward(dev(dout), dev(finite), dev(w), pre, activation=act)
+    col = torch.arange(N) == 7
+    assert torch.equal(db.isnan().cpu(), col) and torch.equal(dw.isnan().any(1).cpu(), col) and dw[7].isnan().all()

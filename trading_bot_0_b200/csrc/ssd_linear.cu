@@ -12,16 +12,17 @@
 namespace ssd {
 namespace {
 
+__device__ __forceinline__ float relu(float v) { return v < 0.f ? 0.f : v; }   // (fmaxf would turn NaN into 0)
 __device__ __forceinline__ float act_of(float v, int act) {
   if (act == SSD_ACT_SILU) return v * __fdividef(1.f, 1.f + __expf(-v));
   if (act == SSD_ACT_SOFTPLUS) return softplusf_(v);
-  if (act == SSD_ACT_RELU2) { const float r = fmaxf(v, 0.f); return r * r; }
+  if (act == SSD_ACT_RELU2) { const float r = relu(v); return r * r; }
   return v;
 }
 __device__ __forceinline__ float dact_of(float v, int act) {
   if (act == SSD_ACT_SILU) { const float s = __fdividef(1.f, 1.f + __expf(-v)); return s * fmaf(v, 1.f - s, 1.f); }
   if (act == SSD_ACT_SOFTPLUS) return __fdividef(1.f, 1.f + __expf(-v));
-  if (act == SSD_ACT_RELU2) return 2.f * fmaxf(v, 0.f);
+  if (act == SSD_ACT_RELU2) return 2.f * relu(v);
   return 1.f;
 }
 
