@@ -75,13 +75,14 @@ __device__ __forceinline__ f32x2 dup2(float v) { return pack2(v, v); }
 __device__ __forceinline__ f32x2 ex2_2(f32x2 v) { float a, b; unpack2(v, a, b); return pack2(ex2(a), ex2(b)); }
 // exp(s A) for a pair of decays (A2 = A log2 e).  ex2.approx is 2e-8 low on average over the arguments that decays have (1.7e-8 to
 // 2.6e-8 in every interval measured between -0.75 and -0.001; rms 4e-8); a state is a product of hundreds of them, where an offset
-// adds up and scatter does not, so the argument is raised by 2e-8 log2 e.
-__device__ __forceinline__ f32x2 decay2(f32x2 A2, f32x2 s2) { return ex2_2(fma2(A2, s2, pack2(2.9e-8f, 2.9e-8f))); }
+// adds up and scatter does not, so the argument is raised by 2e-8 log2 e.  (A step of 0 gives 1 exactly all the same.)
+constexpr float DECAY_UP = 2.9e-8f;
+__device__ __forceinline__ f32x2 decay2(f32x2 A2, f32x2 s2) { return ex2_2(fma2(A2, s2, pack2(DECAY_UP, DECAY_UP))); }
 
 // The same once more (a value that the compiler does not keep from the first time).
 __device__ __forceinline__ f32x2 decay2_again(f32x2 A2, f32x2 s2) {
   float a, b;
-  unpack2(fma2(A2, s2, pack2(2.9e-8f, 2.9e-8f)), a, b);
+  unpack2(fma2(A2, s2, pack2(DECAY_UP, DECAY_UP)), a, b);
   asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
   asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
   return pack2(a, b);
@@ -922,7 +923,7 @@ __global__ void __launch_bounds__(256) k_sel_step(SelStep q, SsdStepPtrs p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (!VEC && j >= have) b[j] = c[j] = 0.f;
-      h[u][j] = fmaf(ex2(step[u] * a[j]), h[u][j], sx * b[j]);
+      h[u][j] = fmaf(ex2(fmaf(step[u], a[j], DECAY_UP)), h[u][j], sx * b[j]);
       y = fmaf(c[j], h[u][j], y);
     }
     if (mine) {
