@@ -592,7 +592,9 @@ CarryGrads carry_backward(const Tensor& in, const Tensor& weight, const Tensor* 
 // [.., features] as rows of `features` dense values; a copy only where the rows have no one distance.
 Tensor as_rows(const char* name, const Tensor& t, int64_t features) {
   if (t.dim() < 1 || t.size(-1) != features) fail("linear: ", name, ": expected ", features, " values in the last dim, got ", t.sizes());
-  Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / features, features});
+  int64_t rows = 1;                                 // (not numel / features, which may be none; the library refuses that)
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) rows *= t.size(i);
+  Tensor r = t.dim() == 2 ? t : t.reshape({rows, features});
   if ((features > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < features)) r = r.contiguous();
   return r;
 }
