@@ -39,3 +39,68 @@ def test_a_mixer_without_a_rank_is_refused(lib):
         T.selective_mixer(rand(2, 5, 24), **p)
     with pytest.raises(T._lib.SsdError, match="positive"):
         T.selective_mixer_step(rand(2, 24), rand(2, 3, D), torch.zeros(2, D, N, device=DEV), **p)
+
+
+def test_a_node_notices_that_its_tensor_was_stepped(lib):
+    """A step, or an output over a tensor that a node has saved: backward raises, as after torch's own in-place calls."""
+    import trading_bot_0_b200 as T
+    from trading_bot_0_b200 import linear as LN, prepost as P, selective as S
+    f = torch.float32
+    raises = lambda: pytest.raises(RuntimeError, match="modified by an inplace operation")
+    B, L, D, N = 2, 6, 16, 8
+    x, w, hist = rand(B, L, D).requires_grad_(), rand(D, 4, dtype=f), rand(B, 3, D)
+    out, _ = P.causal_conv1d_carry(x, w, None, hist)
+    P.conv1d_step(hist, rand(B, D), w)
+    with raises():
+        out.sum().backward()
+    out, _ = P.causal_conv1d_carry(x, w, None, rand(B, 3, D))
+    P.conv1d_step(rand(B, 3, D), rand(B, D), w, out=x.detach()[:, 0])
+    with raises():
+        out.sum().backward()
+    A, bc, st = -torch.ones(D, N, device=DEV), rand(B, L, N), rand(B, D, N, dtype=f)
+    y, _ = S.selective_scan(x, x, A, bc, bc, init_state=st)
+    S.selective_step(st, rand(B, D), rand(B, D), A, rand(B, N), rand(B, N))
+    with raises():
+        y.sum().backward()
+    z = rand(B, L, D)
+    y, _ = S.selective_scan(x, x, A, bc, bc, z=z)
+    S.selective_step(st, rand(B, D), rand(B, D), A, rand(B, N), rand(B, N), y=z[:, 2])
+    with raises():
+        y.sum().backward()
+    W = rand(D, D).requires_grad_()
+    u = rand(B, D)
+    o = LN.linear(u, W)
+    LN.linear_forward(rand(B, D), rand(D, D), out=u)
+    with raises():
+        o.sum().backward()
+    H, Pd = 2, 8
+    xs, dt, st4 = rand(B, L, H, Pd, dtype=f).requires_grad_(), rand(B, L, H, dtype=f).abs(), rand(B, H, Pd, N, dtype=f)
+    a, b4 = -torch.ones(H, device=DEV), rand(B, L, 1, N, dtype=f)
+    y, _ = T.ssd_scan(xs, dt, a, b4, b4, init_state=st4)
+    T.state_update(st4, xs.detach()[:, 0], dt[:, 0], a, b4[:, 0], b4[:, 0])
+    with raises():
+        y.sum().backward()
+
+
+def test_steps_count_as_one_change_each(lib):
+    from trading_bot_0_b200 import linear as LN, prepost as P, selective as S
+    f = torch.float32
+    B, D, N = 3, 16, 8
+    hist, st, y, o, W = rand(B, 3, D), rand(B, D, N, dtype=f), rand(B, D), rand(B, D), rand(D, D)
+    args = (rand(B, D), rand(D, 4, dtype=f)), (rand(B, D), rand(B, D), -torch.ones(D, N, device=DEV), rand(B, N), rand(B, N))
+    for i in range(1, 4):
+        P.conv1d_step(hist, *args[0], out=o)
+        S.selective_step(st, *args[1], y=y)
+        assert hist._version == st._version == y._version == o._version == i
+    LN.linear_forward(y, W, out=o)
+    assert o._version == 4 and y._version == 3
+    v = o._version
+    with pytest.raises(ValueError):
+        LN.linear_forward(y, W, rand(D + 1), out=o)
+    assert o._version == v
+    with torch.inference_mode():                          # tensors that keep no count, inside the mode and after it
+        h2, s2 = rand(B, 3, D), rand(B, D, N, dtype=f)
+        P.conv1d_step(h2, *args[0])
+        S.selective_step(s2, *args[1])
+    P.conv1d_step(h2, *args[0])
+    S.selective_step(s2, *args[1])

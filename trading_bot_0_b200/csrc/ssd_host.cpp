@@ -177,6 +177,9 @@ void check_values_f32(const char* name, const Tensor* t, int64_t n, const at::De
 Tensor empty(at::IntArrayRef shape, at::ScalarType dtype, const at::Device& dev) {
   return at::detail::empty_cuda(shape, dtype, dev, std::nullopt);
 }
+// A tensor of the caller's was written: autograd counts it, as of torch's own in-place calls, so that a node that saved the tensor
+// refuses to go on with other values.  (Tensors of the inference mode keep no count.)
+void written(const Tensor& t) { if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); }
 void* ptr(const Tensor* t) { return t && t->defined() ? t->data_ptr() : nullptr; }
 float* fptr(const Tensor* t) { return (float*)ptr(t); }
 void* stream_of(const at::Device& d) { return c10::cuda::getCurrentCUDAStream(d.index()).stream(); }
@@ -636,7 +639,8 @@ void linear_fwd(const Tensor& x, const Tensor& w, const Tensor* bias, const Tens
     rr = as_rows("residual", *res, N);
     d.residual_stride_row = apart(rr, 0);
   }
-  if (out.defined()) {
+  const bool given = out.defined();
+  if (given) {
     auto shares = [&](const Tensor& t, int64_t rows, int64_t stride, int64_t features) {   // bytes with `out`
       const char *a = (const char*)t.data_ptr(), *b = (const char*)out.data_ptr();
       return a < b + out.nbytes() && b < a + ((rows - 1) * stride + features) * t.element_size();
@@ -655,6 +659,7 @@ void linear_fwd(const Tensor& x, const Tensor& w, const Tensor* bias, const Tens
   if (for_backward && act) pre = like_rows(x, N, at::kFloat);
   Tensor ws = bytes_on(api.linear_workspace_bytes(&d, SSD_PASS_FWD), dev);
   check_rc(api.linear_forward(&d, ptr(&xr), ptr(&w), ptr(bias), ptr(&rr), ptr(&out), ptr(&pre), ws.data_ptr(), (size_t)ws.numel(), stream_of(dev)));
+  if (given) written(out);
 }
 struct LinGrads { Tensor dx, dw, db; };
 LinGrads linear_bwd(const Tensor& dout, const Tensor& x, const Tensor& w, const Tensor* pre, int64_t act, bool want_dx, bool want_dw, bool want_db) {
@@ -929,6 +934,8 @@ PyObject* py_state_update(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     s.p.y = ptr(&y);
     const c10::cuda::CUDAGuard guard(dev);
     check_rc(api.state_update(&s.d, &s.p, stream_of(dev)));
+    written(state);
+    if (y_in) written(y);
     return wrap(y);
   });
 }
@@ -1184,6 +1191,8 @@ PyObject* py_sel_step(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     p.state = fptr(&state); p.x = ptr(&x); p.dt = ptr(&dt); p.A = fptr(&A); p.Bm = ptr(&Bm); p.Cm = ptr(&Cm); p.D = fptr(D); p.z = ptr(z);
     p.y = ptr(&y); p.dt_bias = fptr(bias);
     check_rc(api.selscan_step(&d, &p, stream_of(dev)));
+    written(state);
+    if (y_in) written(y);
     return wrap(y);
   });
 }
@@ -1238,6 +1247,8 @@ PyObject* py_conv_step(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     d.out_stride_b = out.size(0) > 1 ? out.stride(0) : out.size(1);
     if (out.size(0) > 1 && out.stride(0) < out.size(1)) fail("conv1d: out: rows must lie apart");
     check_rc(api.conv1d_step(&d, ptr(&in), fptr(&w), fptr(b), ptr(&hist), ptr(&out), stream_of(dev)));
+    written(hist);
+    if (out_in) written(out);
     return wrap(out);
   });
 }
