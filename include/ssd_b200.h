@@ -423,7 +423,8 @@ SSD_API int32_t ssd_selscan_forward(const SsdSelDims* dims, const SsdSelFwdPtrs*
                                     void* cuda_stream);
 SSD_API int32_t ssd_selscan_backward(const SsdSelDims* dims, const SsdSelBwdPtrs* p, void* workspace, size_t workspace_bytes,
                                      void* cuda_stream);
-/* One timestep, in place on `state` [S,D,N]; A is [D,N], the other fields of SsdStepPtrs as named there with [S,D] for [S,H,P]. */
+/* One timestep, in place on `state` [S,D,N]; A is [D,N], the other fields of SsdStepPtrs as named there with [S,D] for [S,H,P].  y may
+ * be x, dt or z itself (same address and stride); y and state share no memory with an operand otherwise, nor with one another. */
 SSD_API int32_t ssd_selscan_step(const SsdSelStepDims* dims, const SsdStepPtrs* p, void* cuda_stream);
 
 /*
@@ -432,8 +433,9 @@ SSD_API int32_t ssd_selscan_step(const SsdSelStepDims* dims, const SsdStepPtrs* 
  *     out[b,t,c] = act(bias[c] + sum_k weight[c,k] * ext[b,t+k,c]),   new_history[b,j,c] = ext[b,len_b+j,c]  (j < width-1)
  * where len_b = lengths[b] (optional, device int32, taken as 0 .. seqlen) or seqlen.  Rows at or past len_b are not read; their
  * outputs and gradients are zeros.  The backward takes the gradients of both outputs and gives those of in, history, weight and
- * bias.  history and new_history must not overlap.  ssd_conv1d_step is one token per stream (batch = streams, seqlen = 1,
- * in_stride_b / out_stride_b between streams), in place on `history`.  Channels, strides and alignment as above.
+ * bias.  Outputs must not overlap operands (history and new_history are checked).  ssd_conv1d_step is one token per stream (batch =
+ * streams, seqlen = 1, in_stride_b / out_stride_b between streams), in place on `history`; out may be `in` itself (same address and
+ * stride), and out and history share no memory with an operand otherwise.  Channels, strides and alignment as above.
  */
 SSD_API int32_t ssd_conv1d_carry_forward(const SsdConvDims* dims, const void* in, const float* weight,
                                          const float* bias /* optional */, const void* history /* optional */,

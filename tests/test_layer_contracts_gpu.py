@@ -104,3 +104,46 @@ def test_steps_count_as_one_change_each(lib):
         S.selective_step(s2, *args[1])
     P.conv1d_step(h2, *args[0])
     S.selective_step(s2, *args[1])
+
+
+@pytest.mark.parametrize("S_,D,N", [(5, 24, 8), (1, 40, 16), (300, 264, 16), (1201, 256, 64)])
+def test_steps_write_over_their_own_operands_or_between_them(lib, S_, D, N):
+    """The output over x, dt, z or the convolution's input themselves, and in rows between the input's: the same bits as apart."""
+    from trading_bot_0_b200 import prepost as P, selective as S
+    f = torch.float32
+    x, dt, z, B, C, A, w, st, h = (rand(S_, D), rand(S_, D), rand(S_, D), rand(S_, N), rand(S_, N), -rand(D, N, dtype=f).abs(), rand(D, 4, dtype=f),
+                                   rand(S_, D, N, dtype=f), rand(S_, 3, D))
+
+    def scan(x, dt, z, y=None):
+        s = st.clone()
+        return S.selective_step(s, x, dt, A, B, C, None, z, y=y, dt_softplus=True), s
+    want, state = scan(x, dt, z)
+    for i in range(3):
+        own = [x.clone(), dt.clone(), z.clone()]
+        y, s = scan(*own, y=own[i])
+        assert torch.equal(y, want) and torch.equal(s, state) and y.data_ptr() == own[i].data_ptr()
+    wide = torch.zeros(S_, 2 * D + 8, dtype=BF, device=DEV)
+    wide[:, :D] = x
+    y, s = scan(wide[:, :D], dt, z, y=wide[:, D:2 * D])
+    assert torch.equal(y, want) and torch.equal(s, state) and torch.equal(wide[:, :D], x)
+    out = P.conv1d_step(hist := h.clone(), x, w)
+    own = x.clone()
+    assert torch.equal(P.conv1d_step(h2 := h.clone(), own, w, out=own), out) and torch.equal(h2, hist)
+    assert torch.equal(P.conv1d_step(h3 := h.clone(), wide[:, :D], w, out=wide[:, D:2 * D]), out) and torch.equal(h3, hist)
+
+
+def test_step_outputs_that_share_memory_are_refused(lib):
+    import trading_bot_0_b200 as T
+    from trading_bot_0_b200 import prepost as P, selective as S
+    f, S_, D, N = torch.float32, 4, 16, 16
+    buf = torch.zeros(S_ * 2, D, dtype=BF, device=DEV)
+    x, B, C, A, w = buf[:S_], rand(S_, N), rand(S_, N), -torch.ones(D, N, device=DEV), rand(D, 4, dtype=f)
+    st, h = rand(S_, D, N, dtype=f), rand(S_, 3, D)
+    for y in (B, C, buf[1:S_ + 1], st.view(BF).view(-1)[:S_ * D].view(S_, D)):
+        with pytest.raises(T._lib.SsdError, match="share"):
+            S.selective_step(st, x, x, A, B, C, y=y)
+    for out in (buf[1:S_ + 1], h.view(-1)[:S_ * D].view(S_, D)):
+        with pytest.raises(T._lib.SsdError, match="share"):
+            P.conv1d_step(h, x, w, out=out)
+    with pytest.raises(T._lib.SsdError, match="share"):
+        P.conv1d_step(h, h[:, 2], w)

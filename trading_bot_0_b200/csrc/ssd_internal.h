@@ -55,4 +55,18 @@ int sp_total_logdecay(const Geo& g, const float* cs, float* out, cudaStream_t s)
 int sp_prefix_state(const float* gs, const float* gl, int world, int rank, int direction, long long bh,
                     long long elems, const float* init, float* out, cudaStream_t s);
 
+// `n` rows of `width` bytes, `stride` bytes apart; and whether two such have a byte in common: rows that lie between one another do not
+// (where the strides agree; else everything between the first byte and the last counts).
+struct Rows { const void* p; long long n, stride, width; };
+inline bool rows_share(const Rows& a, const Rows& b) {
+  if (!a.p || !b.p) return false;
+  const long long d = (long long)((uintptr_t)b.p - (uintptr_t)a.p);
+  if (d >= (a.n - 1) * a.stride + a.width || -d >= (b.n - 1) * b.stride + b.width) return false;
+  const long long s = a.stride;
+  if (a.n == 1 || b.n == 1 || s != b.stride || a.width > s || b.width > s) return true;
+  const long long k = d >= 0 ? d / s : -((-d + s - 1) / s), r = d - k * s;   // row j of b begins r bytes into row j + k of a
+  auto rows_meet = [&](long long off) { return off < a.n && -off < b.n; };
+  return (r < a.width && rows_meet(k)) || (r + b.width > s && rows_meet(k + 1));
+}
+
 }  // namespace ssd

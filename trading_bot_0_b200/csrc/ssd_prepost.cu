@@ -1586,8 +1586,17 @@ int32_t ssd_conv1d_step(const SsdConvDims* dims, const void* in, const float* we
   const int rc = check_carry("conv1d step", dims, {in, history, out}, {});
   if (rc) return rc;
   if (!weight) { set_error("conv1d step: weight is NULL"); return SSD_ERR_NULL_POINTER; }
-  const int es = dims->dtype == SSD_BF16 ? 2 : 4;
+  const int es = dims->dtype == SSD_BF16 ? 2 : 4;    // bytes per element
   cudaStream_t s = (cudaStream_t)cuda_stream;
+  const long long S = dims->batch, C = dims->channels;
+  const Rows hist{history, 1, 0, S * (dims->width - 1) * C * es}, ins{in, S, dims->in_stride_b * es, C * es}, outs{out, S, dims->out_stride_b * es, C * es},
+      ws{weight, 1, 0, C * dims->width * 4}, bs{bias, 1, 0, C * 4};
+  const bool itself = in == out && (S == 1 || ins.stride == outs.stride);   // (a thread reads its channels' input before it writes them)
+  if (rows_share(hist, ins) || rows_share(hist, outs) || rows_share(hist, ws) || rows_share(hist, bs) || rows_share(outs, ws) || rows_share(outs, bs) ||
+      (!itself && rows_share(outs, ins))) {
+    set_error("conv1d step: history or out share memory with an operand (out may be the input itself)");
+    return SSD_ERR_BAD_SHAPE;
+  }
   const long long vecs = dims->channels * es / 16;
   const bool four = dims->batch * vecs >= 4LL * sm_count() * 512;   // a thread of four streams still leaves 16 warps to an SM
   const long long blocks = ((four ? (dims->batch + 3LL) / 4 : dims->batch) * vecs + 255) / 256;

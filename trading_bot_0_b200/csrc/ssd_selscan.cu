@@ -1191,6 +1191,21 @@ int32_t ssd_selscan_step(const SsdSelStepDims* d, const SsdStepPtrs* p, void* cu
     set_error("selscan step: strides must be at least the dense row size");
     return SSD_ERR_BAD_SHAPE;
   }
+  // what a thread writes is read by no other: y may be x, dt or z itself (a channel's lanes have read theirs by then), nothing else shared
+  const int es = d->dtype == SSD_BF16 ? 2 : 4;
+  auto of_streams = [&](const void* p, long long stride, long long width) { return Rows{p, q.S, stride * es, width * es}; };
+  const Rows state{p->state, 1, 0, (long long)q.S * q.D * q.N * 4}, y = of_streams(p->y, q.ys, q.D);
+  const Rows ins[] = {of_streams(p->x, q.xs, q.D), of_streams(p->dt, q.dts, q.D), of_streams(p->z, q.zs, q.D), of_streams(p->Bm, q.bs, GN),
+                      of_streams(p->Cm, q.cs, GN), {p->A, 1, 0, (long long)q.D * q.N * 4}, {p->D, 1, 0, q.D * 4LL}, {p->dt_bias, 1, 0, q.D * 4LL}};
+  if (rows_share(state, y)) { set_error("selscan step: state and y share memory"); return SSD_ERR_BAD_SHAPE; }
+  for (int i = 0; i < 8; ++i) {
+    const bool itself = i < 3 && ins[i].p == y.p && (q.S == 1 || ins[i].stride == y.stride);
+    if (rows_share(state, ins[i]) || (!itself && rows_share(y, ins[i]))) {
+      static const char* const names[] = {"x", "dt", "z", "B", "C", "A", "D", "dt_bias"};
+      set_error("selscan step: %s shares memory with the state or, without being it, with y", names[i]);
+      return SSD_ERR_BAD_SHAPE;
+    }
+  }
   const int lpc = lanes_for(q.N);
   if ((long long)q.D * lpc > 0x7fffff00LL) { set_error("selscan step: too many channels (%d)", q.D); return SSD_ERR_UNSUPPORTED; }
   q.nx = (q.D * lpc + 255) / 256;
@@ -1198,7 +1213,7 @@ int32_t ssd_selscan_step(const SsdSelStepDims* d, const SsdStepPtrs* p, void* cu
   q.groups = four ? (q.S + 3) / 4 : q.S;
   const long long blocks = (long long)q.groups * q.nx;
   if (blocks > 0x7fffffffLL) { set_error("selscan step: too many blocks for one grid (%lld)", blocks); return SSD_ERR_UNSUPPORTED; }
-  const int es = d->dtype == SSD_BF16 ? 2 : 4;       // four states, and four values of B and C, at a time
+  // four states, and four values of B and C, at a time
   const bool vec = q.N == 4 * lpc && ((uintptr_t)p->state & 15) == 0 && (((uintptr_t)p->Bm | (uintptr_t)p->Cm) & (4 * es - 1)) == 0 && q.bs % 4 == 0 && q.cs % 4 == 0;
   cudaStream_t s = (cudaStream_t)cuda_stream;
 #define SEL_GO(T, LPC, VEC) do { \

@@ -46,7 +46,8 @@ def causal_conv1d_carry(inp, weight, bias=None, history=None, *, lengths=None, a
 
 
 def conv1d_step(history, inp, weight, bias=None, *, activation=True, out=None):
-    """One token per stream, IN PLACE on `history` [streams, width-1, channels]; inp and out [streams, channels]."""
+    """One token per stream, IN PLACE on `history` [streams, width-1, channels]; inp and out [streams, channels].  `out` may be inp itself,
+    and shares no memory with an operand or the history otherwise."""
     return L.host().conv1d_step(history, inp, weight, bias, activation, out)
 
 

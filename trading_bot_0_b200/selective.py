@@ -34,5 +34,6 @@ def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, init_state=None, *, dt_bias
 
 def selective_step(state, x, dt, A, Bm, Cm, D=None, z=None, *, y=None, dt_bias=None, dt_softplus=False):
     """One token per stream, IN PLACE on `state` [streams, channels, dstate] fp32; x, dt, z [streams, channels], B, C
-    [streams, ngroups, dstate] or [streams, dstate].  Returns y."""
+    [streams, ngroups, dstate] or [streams, dstate].  Returns y; a `y` given may be x, dt or z itself, and shares no memory with an operand
+    or the state otherwise."""
     return L.host().selscan_step(state, x, dt, A, Bm, Cm, D, z, y, dt_bias, dt_softplus)
