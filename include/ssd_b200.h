@@ -456,8 +456,9 @@ SSD_API int32_t ssd_conv1d_step(const SsdConvDims* dims, const void* in, const f
  * the tensor cores; all other sizes, strides and fp32 on the CUDA cores in fp32.  `pre` (optional, dense, fp32) receives
  * x W^T + bias for the backward, which needs it where act is not NONE.  Backward: dpre = dout * act'(pre), dx = dpre W,
  * dweight = dpre^T x, dbias = sum of dpre over the rows; each of the three is optional.
- * `out` may be the residual (same address, same row stride), and must
- * not overlap it otherwise, nor x, weight or bias.
+ * `out` may be the residual (same address, same row stride), and must not overlap it otherwise, nor x, weight or bias.
+ * The workspace's first word (4-byte aligned) is a status word as below, cleared by every call before its first product; outputs of a
+ * product whose wait ran out, and of those after it in the call, are NaN.
  */
 typedef enum SsdAct { SSD_ACT_NONE = 0, SSD_ACT_SILU = 1, SSD_ACT_SOFTPLUS = 2, SSD_ACT_RELU2 = 3 } SsdAct;   /* RELU2: max(v,0)^2 */
 typedef struct SsdLinearDims {
@@ -478,6 +479,7 @@ SSD_API int32_t ssd_linear_backward(const SsdLinearDims* dims, const void* x, co
  * Failure detection.  Every wait inside the pipelined kernels (on a TMA transfer, an MMA completion, another warp role)
  * is bounded: when it runs out the kernel writes a code into the first 4 bytes of the workspace (0 = healthy), skips its
  * remaining waits and returns, and later kernels on the same workspace return at once; the context stays usable.
+ * Workspaces of the scan (ssd_workspace_bytes) and of the projection (ssd_linear_workspace_bytes) have that word; the others have none.
  * ssd_selftest_bounded_wait exercises that path without touching a pipeline: one warp waits, for at most `max_cycles`
  * clock cycles, on a barrier nothing arrives on, then writes 99 to *device_status (a device int32 the caller zeroed).
  * No counterpart in the reference.

@@ -50,3 +50,12 @@ def test_step_outputs_that_share_memory_are_refused(lib):
               (at(1), at(2), None, at(4), at(1, -128)), (at(1), at(2), None, at(4), at(2)), (at(1), at(2), at(3), at(4), at(3)),
               (at(4, 256), at(2), None, at(4), at(5)), (at(1), at(4), None, at(4), at(5)), (at(1), at(2), at(4, 512), at(4), at(5))):
         assert step(*a) == -1 and "share" in _err(lib), a
+
+
+def test_projection_workspaces_start_on_a_word(lib):
+    from trading_bot_0_b200 import _lib as L
+    d = L.SsdLinearDims()
+    d.rows, d.in_features, d.out_features, d.dtype, d.device = 100, 64, 96, L.SSD_BF16, -1
+    fwd, bwd = (lib.ssd_linear_workspace_bytes(C.byref(d), p) for p in (0, 1))
+    assert lib.ssd_linear_forward(C.byref(d), at(1), at(2), None, None, at(3), None, at(9, 2), fwd, None) == -2 and "4-byte" in _err(lib)
+    assert lib.ssd_linear_backward(C.byref(d), at(1), at(2), None, at(3), 0, at(4), at(5), None, at(9, 1), bwd, None) == -2 and "4-byte" in _err(lib)

@@ -147,3 +147,34 @@ def test_step_outputs_that_share_memory_are_refused(lib):
             P.conv1d_step(h, x, w, out=out)
     with pytest.raises(T._lib.SsdError, match="share"):
         P.conv1d_step(h, h[:, 2], w)
+
+
+@pytest.mark.parametrize("off", [0, 4])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("M,K,N", [(3, 64, 48), (40, 64, 48), (64, 1536, 128), (300, 64, 520), (50, 33, 40), (64, 1540, 40), (33, 64, 41)])
+def test_status_word_of_the_projection(lib, dtype, M, K, N, off):
+    """The first word of a workspace that held something else is 0 after each call, on every path (few rows, tensor cores with and without
+    splits, CUDA cores), also where the workspace starts off 256 bytes and where no gradient is wanted."""
+    import ctypes as C
+    import trading_bot_0_b200 as T
+    from trading_bot_0_b200.ssd import workspace_status
+    L = T._lib
+    t = torch.float32 if dtype == "fp32" else BF
+    x, w, out, dout, pre, dx, dw, db = (rand(M, K, dtype=t), rand(N, K, dtype=t), rand(M, N, dtype=t), rand(M, N, dtype=t), rand(M, N, dtype=torch.float32),
+                                        rand(M, K, dtype=t), rand(N, K, dtype=t), rand(N, dtype=t))
+    p = lambda v: C.c_void_p(v.data_ptr())
+    s = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    d = L.SsdLinearDims()
+    d.rows, d.in_features, d.out_features, d.dtype, d.device = M, K, N, L.SSD_BF16 if t == BF else L.SSD_F32, 0
+    for act in (0, 1):
+        d.activation = act
+        n = [lib.ssd_linear_workspace_bytes(C.byref(d), k) for k in (0, 1)]
+        ws = torch.empty(max(n) + 8, dtype=torch.uint8, device=DEV)[off:]
+
+        def check(rc):
+            assert rc == 0 and int(ws[:4].view(torch.int32)) == 0 and workspace_status(ws) == 0
+            ws.fill_(0x5a)
+        ws.fill_(0x5a)
+        check(lib.ssd_linear_forward(C.byref(d), p(x), p(w), None, None, p(out), p(pre), p(ws), n[0], s))
+        for want in ((dx, dw, db), (dx, dw, None), (dx, None, None), (None, dw, None), (None, None, db), (None, None, None)):
+            check(lib.ssd_linear_backward(C.byref(d), p(x), p(w), p(pre), p(dout), 0, *(None if v is None else p(v) for v in want), p(ws), n[1], s))

@@ -56,7 +56,12 @@ struct MmArgs {
   int act, splits;
   long long kper;
   float* part;                                      // splits > 1: [splits][M][N] sums, finished by k_join
+  int* status;                                      // first kernel of a call: the workspace's status word, to be cleared; else null
 };
+// The status word is cleared once per call, by its first kernel (whichever path that is), and only ever set after that.
+__device__ __forceinline__ void clear_status(int* status) {
+  if (status && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && threadIdx.y == 0) *status = 0;
+}
 template <typename T> __device__ __forceinline__ void finish(const MmArgs& a, long long m, long long n, float v) {
   if (a.bias) v += ldf((const T*)a.bias + n);
   if (a.pre) a.pre[m * a.N + n] = v;
@@ -73,6 +78,7 @@ __global__ void __launch_bounds__(256) k_mm(MmArgs a) {
   constexpr int BM = 16 * TM, BK = 32, LD = BM + 4, IT = BM * BK / 256;
   __shared__ __align__(16) float sp[BK][LD], sq[BK][LD];
   pdl_wait();
+  clear_status(a.status);
   const int tid = threadIdx.x, tm = tid / 16, tn = tid % 16;
   const long long nn = (a.N + BM - 1) / BM, nm = (a.M + BM - 1) / BM;
   const long long tile = blockIdx.x % (nn * nm), sp_i = blockIdx.x / (nn * nm);
@@ -175,6 +181,7 @@ template <typename T, int RM, int F>
 __global__ void __launch_bounds__(256) k_mm_few(MmArgs a) {
   constexpr int V = 16 / (int)sizeof(T);
   pdl_wait();
+  clear_status(a.status);
   const int lane = threadIdx.x & 31;
   const long long n0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * F;
   if (n0 >= a.N) return;
@@ -209,8 +216,8 @@ __global__ void __launch_bounds__(256) k_mm_few(MmArgs a) {
 // where a CTA on its own would load 48 KB for the same work per SM).  Warp 0 of each CTA issues the loads (five stages), warp 1 of the
 // leader the MMAs, eight warps per CTA read the accumulators (two of them in TMEM, so that a tile's epilogue runs beside the next
 // tile's products).  Pairs walk the units (split of k, tile row, tile column) with a fixed stride; with splits > 1 a unit leaves fp32
-// sums in the workspace and k_mm2_join adds them in order.  Every wait is bounded: when one runs out a code goes to the status word and
-// the outputs become NaN.
+// sums in the workspace and k_mm2_join adds them in order.  Every wait is bounded: when one runs out a code goes to the status word, the
+// outputs become NaN, and a later product of the same call waits for nothing and gives NaN.
 //
 // Measured with cuBLAS beside it in one run: 8192^3 694 us = 1.58 PFLOP/s (647), 16384 x 768 x 3352 76 (72), 4096 x 2048 x 2048 45 (41),
 // 512 x 768 x 1536 14 (8).  8192^3 before and after on one board: 785 us with loads and MMAs issued by `lane == 0`, 677 by an elected
@@ -234,6 +241,7 @@ struct Mm2 {
   __nv_bfloat16* out;
   float *pre, *part;                                     // [splits][out rows][out columns]
   int* status;
+  int first;                                       // the call's first kernel: clears the status word
 };
 
 // unit -> split, tile row, tile column; columns of a group of MM_ROWS tile rows one after the other
@@ -292,9 +300,10 @@ k_mm2(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMa
   u::tc_fence_after();
   const uint32_t tmem = slot;
   pdl_wait();
-  if (blockIdx.x == 0 && tid == 0) *a.status = 0;
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   volatile int* is_dead = &dead;
+  if (a.first) clear_status(a.status);
+  else if (*(volatile int*)a.status) *is_dead = 1;   // an earlier kernel gave up
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
     if (*is_dead) return false;
     if (u::mbar_wait(bar, parity)) return true;
@@ -529,9 +538,10 @@ __global__ void __launch_bounds__(256) k_mm2_join(Mm2 a, long long rows, int col
 // rows of a thread requested together.  V = 16 bytes where all rows start on 16 bytes, else one value.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) k_dpre(long long M, int N, int act, const T* __restrict__ dout, long long dos, const float* __restrict__ pre,
-                                              T* __restrict__ dpre, float* __restrict__ partial) {
+                                              T* __restrict__ dpre, float* __restrict__ partial, int* status) {
   __shared__ float s[8][32 * V];
   pdl_wait();
+  clear_status(status);
   typedef typename std::conditional<V == 1, T, uint4>::type Raw;   // V values as they lie in memory
   constexpr int R = 4;
   const int n = (blockIdx.x * 32 + threadIdx.x) * V;
@@ -672,13 +682,13 @@ size_t part_bytes(const TileShape& t, long long M, long long N) { return t.split
 struct Operand { const void* p; bool kmajor; long long stride; };
 struct Result { __nv_bfloat16* out; float* pre; const __nv_bfloat16 *bias, *residual; long long os, rs; int act; };
 int run_mm2(const char* what, const TileShape& t, Operand P, Operand Q, long long M, long long N, long long K, const Result& o, float* part,
-            int* status, cudaStream_t s) {
+            int* status, bool first, cudaStream_t s) {
   Mm2 a;
   if (t.trans) { const Operand x = P; P = Q; Q = x; }
   a.M = t.trans ? N : M; a.N = t.trans ? M : N;
   a.kb = (int)((K + 63) / 64); a.kper = t.kper; a.splits = t.splits; a.bn = t.bn; a.rt = (int)t.rt; a.ct = (int)t.ct;
   a.units = (int)(t.rt * t.ct * t.splits); a.trans = t.trans; a.act = o.act;
-  a.os = o.os; a.rs = o.rs; a.bias = o.bias; a.residual = o.residual; a.out = o.out; a.pre = o.pre; a.part = part; a.status = status;
+  a.os = o.os; a.rs = o.rs; a.bias = o.bias; a.residual = o.residual; a.out = o.out; a.pre = o.pre; a.part = part; a.status = status; a.first = first;
   if (t.splits > 1) a.vec = !t.trans && N % 4 == 0 && N < (1LL << 36) / M;
   else a.vec = !t.trans && N % 8 == 0 && (((uintptr_t)o.out | (uintptr_t)o.pre | (uintptr_t)o.residual) & 15) == 0 && o.os % 8 == 0 &&
                (!o.residual || o.rs % 8 == 0) && o.os < (1LL << 36) / M;
@@ -825,8 +835,14 @@ template <typename T> int run_few(const MmArgs& a, cudaStream_t s) {
 
 template <typename T>
 int linear_backward(const LinPlan& p, const void* x, const void* w, const void* pre, const void* dout, long long dos, void* dx, void* dw,
-                    void* db, char* ws, cudaStream_t s) {
+                    void* db, char* ws, int* status, cudaStream_t s) {
   const bool need_dpre = p.act && (dx || dw);
+  bool first = true;                                  // no kernel of this call has cleared the status word yet
+  if (!dx && !dw && !db) {
+    const cudaError_t e = cudaMemsetAsync(status, 0, sizeof(int), s);
+    if (e != cudaSuccess) { set_error("linear backward: %s", cudaGetErrorString(e)); return SSD_ERR_CUDA; }
+    return SSD_OK;
+  }
   const void* g = dout;
   long long gs = dos;
   if (need_dpre || db) {
@@ -834,10 +850,11 @@ int linear_backward(const LinPlan& p, const void* x, const void* w, const void* 
     float* partial = db ? (float*)(ws + p.partial) : nullptr;
     constexpr int V = 16 / (int)sizeof(T);
     if (p.N % V == 0 && dos % V == 0 && (((uintptr_t)dout | (p.act ? (uintptr_t)pre : 0)) & 15) == 0)
-      launch<k_dpre<T, V>>(dim3((p.N + 32 * V - 1) / (32 * V), p.parts), dim3(32, 8), 0, s, p.M, p.N, p.act, (const T*)dout, dos, (const float*)pre, dpre, partial);
+      launch<k_dpre<T, V>>(dim3((p.N + 32 * V - 1) / (32 * V), p.parts), dim3(32, 8), 0, s, p.M, p.N, p.act, (const T*)dout, dos, (const float*)pre, dpre, partial, status);
     else
-      launch<k_dpre<T, 1>>(dim3((p.N + 31) / 32, p.parts), dim3(32, 8), 0, s, p.M, p.N, p.act, (const T*)dout, dos, (const float*)pre, dpre, partial);
+      launch<k_dpre<T, 1>>(dim3((p.N + 31) / 32, p.parts), dim3(32, 8), 0, s, p.M, p.N, p.act, (const T*)dout, dos, (const float*)pre, dpre, partial, status);
     SSD_CUDA_CHECK_LAUNCH("linear_dpre");
+    first = false;
     if (db) {
       launch<k_dbias<T>>((p.N + 31) / 32, dim3(32, 32), 0, s, p.N, p.parts, (const float*)partial, (T*)db);
       SSD_CUDA_CHECK_LAUNCH("linear_dbias");
@@ -845,19 +862,23 @@ int linear_backward(const LinPlan& p, const void* x, const void* w, const void* 
     if (need_dpre) { g = dpre; gs = p.N; }
   }
   int rc = SSD_OK;
+  float* part = (float*)(ws + p.part_bwd);
   if (std::is_same<T, __nv_bfloat16>::value && p.tc && map_fits(g, p.M, gs) && map_fits(w, p.N, p.K)) {
     typedef __nv_bfloat16 bf;
-    int* status = (int*)ws;
-    float* part = (float*)(ws + p.part_bwd);
-    if (dx && (rc = run_mm2("linear_dx", p.tdx, {g, true, gs}, {w, false, p.K}, p.M, p.K, p.N, {(bf*)dx, nullptr, nullptr, nullptr, p.K, 0, 0}, part, status, s)))
+    if (dx && (rc = run_mm2("linear_dx", p.tdx, {g, true, gs}, {w, false, p.K}, p.M, p.K, p.N, {(bf*)dx, nullptr, nullptr, nullptr, p.K, 0, 0}, part, status, first,
+                           s)))
       return rc;
     if (!dw) return rc;
+    first = first && !dx;
     if (map_fits(x, p.M, p.xs))
-      return run_mm2("linear_dw", p.tdw, {g, false, gs}, {x, false, p.xs}, p.N, p.K, p.M, {(bf*)dw, nullptr, nullptr, nullptr, p.K, 0, 0}, part, status, s);
+      return run_mm2("linear_dw", p.tdw, {g, false, gs}, {x, false, p.xs}, p.N, p.K, p.M, {(bf*)dw, nullptr, nullptr, nullptr, p.K, 0, 0}, part, status, first, s);
     dx = nullptr;
   }
-  if (dx && (rc = run_mm<T>("linear_dx", MmArgs{g, w, nullptr, nullptr, dx, nullptr, p.M, p.K, p.N, gs, 1, 1, p.K, p.K, 0, 0, 1, 0, (float*)(ws + p.part_bwd)}, s))) return rc;
-  if (dw && (rc = run_mm<T>("linear_dw", MmArgs{g, x, nullptr, nullptr, dw, nullptr, p.N, p.K, p.M, 1, gs, 1, p.xs, p.K, 0, 0, 1, 0, (float*)(ws + p.part_bwd)}, s))) return rc;
+  if (dx && (rc = run_mm<T>("linear_dx", MmArgs{g, w, nullptr, nullptr, dx, nullptr, p.M, p.K, p.N, gs, 1, 1, p.K, p.K, 0, 0, 1, 0, part, first ? status : nullptr}, s)))
+    return rc;
+  first = first && !dx;
+  if (dw && (rc = run_mm<T>("linear_dw", MmArgs{g, x, nullptr, nullptr, dw, nullptr, p.N, p.K, p.M, 1, gs, 1, p.xs, p.K, 0, 0, 1, 0, part, first ? status : nullptr}, s)))
+    return rc;
   return rc;
 }
 
@@ -882,16 +903,17 @@ int32_t ssd_linear_forward(const SsdLinearDims* dims, const void* x, const void*
   int rc = make_lin_plan(dims, SSD_PASS_FWD, &p);
   if (rc || (rc = check_device(dims))) return rc;
   if (!x || !weight || !out || !workspace) { set_error("linear: x, weight, out and workspace must be non-NULL"); return SSD_ERR_NULL_POINTER; }
+  if ((uintptr_t)workspace & 3) { set_error("linear: workspace must be 4-byte aligned (its first word is the status)"); return SSD_ERR_BAD_ALIGNMENT; }
   if (workspace_bytes < p.fwd_bytes) { set_error("linear: workspace too small: %zu < %zu", workspace_bytes, p.fwd_bytes); return SSD_ERR_WORKSPACE_TOO_SMALL; }
   cudaStream_t s = (cudaStream_t)cuda_stream;
   char* ws = aligned_base(workspace);
-  const MmArgs a{x, weight, bias, residual, out, (float*)pre, p.M, p.N, p.K, p.xs, 1, p.K, 1, p.os, p.rs, p.act, 1, 0, (float*)(ws + p.part_fwd)};
+  const MmArgs a{x, weight, bias, residual, out, (float*)pre, p.M, p.N, p.K, p.xs, 1, p.K, 1, p.os, p.rs, p.act, 1, 0, (float*)(ws + p.part_fwd), (int*)workspace};
   const bool bf16 = dims->dtype == SSD_BF16, vectors = (((uintptr_t)x | (uintptr_t)weight) & 15) == 0 && p.K % (16 / p.es) == 0 && (p.M == 1 || p.xs % (16 / p.es) == 0);
   if (p.M <= FEW && vectors) return bf16 ? run_few<__nv_bfloat16>(a, s) : run_few<float>(a, s);
   if (p.tc && map_fits(x, p.M, p.xs) && map_fits(weight, p.N, p.K)) {
     typedef __nv_bfloat16 bf;
     return run_mm2("linear_fwd", p.fwd, {x, true, p.xs}, {weight, true, p.K}, p.M, p.N, p.K,
-                   {(bf*)out, (float*)pre, (const bf*)bias, (const bf*)residual, p.os, p.rs, p.act}, (float*)(ws + p.part_fwd), (int*)ws, s);
+                   {(bf*)out, (float*)pre, (const bf*)bias, (const bf*)residual, p.os, p.rs, p.act}, (float*)(ws + p.part_fwd), (int*)workspace, true, s);
   }
   return bf16 ? run_mm<__nv_bfloat16>("linear_fwd", a, s) : run_mm<float>("linear_fwd", a, s);
 }
@@ -907,11 +929,12 @@ int32_t ssd_linear_backward(const SsdLinearDims* dims, const void* x, const void
   if (p.act && !pre) { set_error("linear backward: an activation needs the forward's pre"); return SSD_ERR_NULL_POINTER; }
   const long long dos = dout_stride_row ? dout_stride_row : p.N;
   if (dos < p.N) { set_error("linear backward: dout's row stride must be at least the row size"); return SSD_ERR_BAD_SHAPE; }
+  if ((uintptr_t)workspace & 3) { set_error("linear: workspace must be 4-byte aligned (its first word is the status)"); return SSD_ERR_BAD_ALIGNMENT; }
   if (workspace_bytes < p.bwd_bytes) { set_error("linear backward: workspace too small: %zu < %zu", workspace_bytes, p.bwd_bytes); return SSD_ERR_WORKSPACE_TOO_SMALL; }
   char* ws = aligned_base(workspace);
   cudaStream_t s = (cudaStream_t)cuda_stream;
-  return dims->dtype == SSD_BF16 ? linear_backward<__nv_bfloat16>(p, x, weight, pre, dout, dos, dx, dweight, dbias, ws, s)
-                                 : linear_backward<float>(p, x, weight, pre, dout, dos, dx, dweight, dbias, ws, s);
+  return dims->dtype == SSD_BF16 ? linear_backward<__nv_bfloat16>(p, x, weight, pre, dout, dos, dx, dweight, dbias, ws, (int*)workspace, s)
+                                 : linear_backward<float>(p, x, weight, pre, dout, dos, dx, dweight, dbias, ws, (int*)workspace, s);
 }
 
 }  // extern "C"

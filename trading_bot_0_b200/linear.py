@@ -3,6 +3,9 @@
 x [.., in_features], weight [out_features, in_features], bias, residual and out in one storage type (bf16 or fp32); products are
 added in fp32 and the result is rounded once.  bf16 rows that start on 16 bytes run on the tensor cores, other sizes and strides and
 fp32 on the CUDA cores.  `activation` is "none", "silu", "softplus" or "relu2" (max(v, 0) squared).
+
+Every wait inside the tensor-core kernel is bounded.  When one runs out the outputs are NaN; these calls own their workspaces, so that is
+the only sign of it here (a caller of the C entry points reads the workspace's status word).
 """
 from __future__ import annotations
 
