@@ -178,3 +178,21 @@ def test_status_word_of_the_projection(lib, dtype, M, K, N, off):
         check(lib.ssd_linear_forward(C.byref(d), p(x), p(w), None, None, p(out), p(pre), p(ws), n[0], s))
         for want in ((dx, dw, db), (dx, dw, None), (dx, None, None), (None, dw, None), (None, None, db), (None, None, None)):
             check(lib.ssd_linear_backward(C.byref(d), p(x), p(w), p(pre), p(dout), 0, *(None if v is None else p(v) for v in want), p(ws), n[1], s))
+
+
+def test_gradients_of_a_history_need_no_alignment(lib):
+    """The gradient of the new history as a view that starts off 16 bytes (states of several layers flattened into one vector)."""
+    from trading_bot_0_b200 import prepost as P
+    B, L, C, K = 2, 9, 24, 4
+    x, w, b, h = rand(B, L, C).requires_grad_(), rand(C, K, dtype=torch.float32).requires_grad_(), rand(C, dtype=torch.float32), rand(B, K - 1, C).requires_grad_()
+    dout, dnew = rand(B, L, C), rand(B, K - 1, C)
+    out, new = P.causal_conv1d_carry(x, w, b, h)
+    off = torch.cat([rand(1), dnew.flatten()])[1:].view(B, K - 1, C)
+    assert off.data_ptr() % 16 and off.is_contiguous()
+    want = torch.autograd.grad([out, new], [x, w, h], [dout, dnew], retain_graph=True)
+    got = torch.autograd.grad([out, new], [x, w, h], [dout, off], retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    flat = torch.cat([rand(3), new.flatten()])            # and as autograd itself makes one
+    g = torch.cat([rand(3), dnew.flatten()])
+    got = torch.autograd.grad([out, flat], [x, w, h], [dout, g])
+    assert all(torch.equal(p, q) for p, q in zip(got, want))

@@ -828,7 +828,8 @@ struct CarryNode : public torch::autograd::Function<CarryNode> {
     Tensor dout = usable_rows(grads[0], v[0], 2);
     const int64_t e = dout.element_size();
     if ((uintptr_t)dout.data_ptr() % 16 || apart(dout, 1) * e % 16 || apart(dout, 0) * e % 16) dout = dout.contiguous().clone();
-    const Tensor dnew = grads[1].defined() ? as_type(grads[1], v[0].scalar_type()).contiguous() : Tensor();
+    Tensor dnew = grads[1].defined() ? as_type(grads[1], v[0].scalar_type()).contiguous() : Tensor();
+    if (dnew.defined() && (uintptr_t)dnew.data_ptr() % 16) dnew = dnew.clone();
     CarryGrads g = carry_backward(v[0], v[1], or_null(v[2]), or_null(v[3]), dout, or_null(dnew), or_null(v[4]), ctx->saved_data["activation"].toBool());
     return {g.din, g.dweight, g.dbias, g.dhist, Tensor(), Tensor()};
   }
