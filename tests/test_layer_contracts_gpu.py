@@ -196,3 +196,40 @@ def test_gradients_of_a_history_need_no_alignment(lib):
     g = torch.cat([rand(3), dnew.flatten()])
     got = torch.autograd.grad([out, flat], [x, w, h], [dout, g])
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def _calls():
+    """The differentiable calls: a function of its first tensor, and that tensor."""
+    from trading_bot_0_b200 import linear as LN, prepost as P, selective as S
+    f, B, L, D, N = torch.float32, 2, 6, 16, 4
+    g = torch.Generator(device=DEV).manual_seed(1)
+    n = lambda *s: torch.randn(*s, device=DEV, generator=g)
+    w, A, bc, W, st = n(D, 4), -n(D, N).abs(), n(B, L, N), n(12, D), n(B, D, N)
+    return {"linear": (lambda x: LN.linear(x, W, activation="silu"), n(B, L, D)),
+            "conv": (lambda x: P.causal_conv1d_carry(x, w)[0], n(B, L, D)),
+            "scan": (lambda x: S.selective_scan(x, x, A, bc, bc, dt_softplus=True)[0], n(B, L, D)),
+            "scan state": (lambda h: S.selective_scan(n(B, L, D), n(B, L, D), A, bc, bc, init_state=h, dt_softplus=True)[1], st)}
+
+
+@pytest.mark.parametrize("which", ["linear", "conv", "scan", "scan state"])
+def test_a_second_derivative_is_refused(lib, which):
+    """The nodes have one derivative.  Its values come with create_graph too; differentiating them again raises (it used to go on as if
+    they were constants)."""
+    f, x = _calls()[which]
+    x = x.requires_grad_()
+    torch.manual_seed(0)
+    y = f(x)
+    want = torch.autograd.grad(y.square().sum(), x, retain_graph=True)[0]
+    g = torch.autograd.grad(y.square().sum(), x, create_graph=True)[0]
+    assert torch.equal(g, want) and g.requires_grad
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad((g * x).sum(), x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (g * x).sum().backward()
+
+
+def test_the_residuals_gradient_is_as_often_differentiable_as_its_source(lib):
+    from trading_bot_0_b200 import linear as LN
+    x, W, r = rand(3, 16), rand(8, 16), rand(3, 8, dtype=BF).requires_grad_()
+    g = torch.autograd.grad(LN.linear(x, W, None, r).pow(2).sum(), r, create_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(g.sum(), r)[0], torch.full_like(r, 2.0))

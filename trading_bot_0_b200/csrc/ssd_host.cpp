@@ -16,6 +16,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
@@ -694,6 +695,20 @@ bool any_requires_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts) if (t && t->requires_grad()) return true;
   return false;
 }
+// What a node's backward returns.  Where a graph of it is wanted (create_graph) the values are made to depend on what they were computed
+// from, the node's operands and incoming gradients, by way of a function that raises: differentiated in turn they do not pass for constants.
+variable_list once(const char* what, variable_list grads, const variable_list& operands, const variable_list& incoming) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list in;
+  for (const Tensor& g : grads) if (g.defined()) in.push_back(g);
+  for (const variable_list* l : {&operands, &incoming})
+    for (const Tensor& t : *l) if (t.defined() && t.requires_grad()) in.push_back(t);
+  const auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", (int64_t)in.size());
+  const variable_list out = (*node)(std::move(in));
+  size_t i = 0;
+  for (Tensor& g : grads) if (g.defined()) g = out[i++];
+  return grads;
+}
 using Opt = std::optional<Tensor>;   // an absent operand of a node: Function::apply takes no undefined tensors
 Opt optional(const Tensor* t) { return t ? Opt(*t) : Opt(); }
 const Tensor* or_null(const Opt& t) { return t.has_value() ? &*t : nullptr; }
@@ -809,7 +824,7 @@ struct SelNode : public torch::autograd::Function<SelNode> {
     Tensor ws = v[10];
     SelGrads g;
     sel_backward(s, dy, or_null(dfin), ws, true, g);
-    return {g.dx, g.ddt, g.dA, g.dB, g.dC, g.dD, g.dz, g.dinit, g.dbias, Tensor(), Tensor()};
+    return once("selective_scan", {g.dx, g.ddt, g.dA, g.dB, g.dC, g.dD, g.dz, g.dinit, g.dbias, Tensor(), Tensor()}, v, grads);
   }
 };
 
@@ -831,7 +846,7 @@ struct CarryNode : public torch::autograd::Function<CarryNode> {
     Tensor dnew = grads[1].defined() ? as_type(grads[1], v[0].scalar_type()).contiguous() : Tensor();
     if (dnew.defined() && (uintptr_t)dnew.data_ptr() % 16) dnew = dnew.clone();
     CarryGrads g = carry_backward(v[0], v[1], or_null(v[2]), or_null(v[3]), dout, or_null(dnew), or_null(v[4]), ctx->saved_data["activation"].toBool());
-    return {g.din, g.dweight, g.dbias, g.dhist, Tensor(), Tensor()};
+    return once("causal_conv1d_carry", {g.din, g.dweight, g.dbias, g.dhist, Tensor(), Tensor()}, v, grads);
   }
 };
 
@@ -854,7 +869,9 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
     if (ctx->needs_input_grad(0) || ctx->needs_input_grad(1) || want_db)
       g = linear_bwd(dout, v[0], v[1], or_null(v[2]), ctx->saved_data["act"].toInt(), ctx->needs_input_grad(0), ctx->needs_input_grad(1), want_db);
     if (want_db) g.db = g.db.view(ctx->saved_data["bias"].toIntVector());
-    return {g.dx, g.dw, g.db, want_dr ? dout : Tensor(), Tensor()};
+    variable_list r = once("linear", {g.dx, g.dw, g.db, Tensor(), Tensor()}, v, grads);
+    if (want_dr) r[3] = dout;                          // (as often differentiable as dout is)
+    return r;
   }
 };
 

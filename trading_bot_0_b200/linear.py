@@ -32,5 +32,5 @@ def linear_backward(dout, x, weight, pre=None, *, activation="none", bias=True, 
 
 
 def linear(x, weight, bias=None, residual=None, *, activation="none"):
-    """Differentiable."""
+    """Differentiable, once."""
     return L.host().linear(x, weight, bias, residual, _act(activation))

@@ -41,7 +41,7 @@ def conv1d_carry_backward(inp, weight, bias, history, dout, dnew_history=None, *
 
 
 def causal_conv1d_carry(inp, weight, bias=None, history=None, *, lengths=None, activation=True):
-    """Differentiable conv1d_carry_forward: returns (out, new_history)."""
+    """Differentiable (once) conv1d_carry_forward: returns (out, new_history)."""
     return L.host().carry(inp, weight, bias, history, lengths, activation)
 
 

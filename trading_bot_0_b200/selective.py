@@ -28,7 +28,7 @@ def selective_scan_backward(dy, x, dt, A, Bm, Cm, D=None, z=None, init_state=Non
 
 
 def selective_scan(x, dt, A, Bm, Cm, D=None, z=None, init_state=None, *, dt_bias=None, dt_softplus=False, lengths=None):
-    """Differentiable: returns (y, final_state)."""
+    """Differentiable, once: returns (y, final_state)."""
     return L.host().selscan(x, dt, A, Bm, Cm, D, z, init_state, dt_bias, dt_softplus, lengths)
 
 
