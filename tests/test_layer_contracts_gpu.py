@@ -233,3 +233,16 @@ def test_the_residuals_gradient_is_as_often_differentiable_as_its_source(lib):
     x, W, r = rand(3, 16), rand(8, 16), rand(3, 8, dtype=BF).requires_grad_()
     g = torch.autograd.grad(LN.linear(x, W, None, r).pow(2).sum(), r, create_graph=True)[0]
     assert torch.equal(torch.autograd.grad(g.sum(), r)[0], torch.full_like(r, 2.0))
+
+
+@pytest.mark.parametrize("which", ["linear", "conv", "scan", "scan state"])
+def test_a_forward_mode_derivative_is_refused(lib, which):
+    """With and without requires_grad: a tangent would be dropped."""
+    import torch.autograd.forward_ad as fwAD
+    f, x = _calls()[which]
+    with fwAD.dual_level():
+        with pytest.raises(ValueError, match="forward-mode"):
+            f(fwAD.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(ValueError, match="forward-mode"):
+            f(fwAD.make_dual(x.clone().requires_grad_(), torch.ones_like(x)))
+        f(x)

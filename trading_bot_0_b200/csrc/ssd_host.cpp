@@ -695,6 +695,10 @@ bool any_requires_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts) if (t && t->requires_grad()) return true;
   return false;
 }
+// The nodes of the layer operators have no forward-mode derivative; a tangent must not be dropped.
+void no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts) if (t && t->_fw_grad(0).defined()) fail(what, ": there is no forward-mode derivative");
+}
 // What a node's backward returns.  Where a graph of it is wanted (create_graph) the values are made to depend on what they were computed
 // from, the node's operands and incoming gradients, by way of a function that raises: differentiated in turn they do not pass for constants.
 variable_list once(const char* what, variable_list grads, const variable_list& operands, const variable_list& incoming) {
@@ -1157,6 +1161,7 @@ PyObject* py_sel_scan(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
   return guarded([&]() -> PyObject* {
     const Args a(argv, argc, 11);
     const Sel s = sel_of(a, 0, 8, 9, 10);
+    no_tangents("selective_scan", {&s.x, &s.dt, &s.A, &s.Bm, &s.Cm, s.D, s.z, s.init, s.bias});
     if (!any_requires_grad({&s.x, &s.dt, &s.A, &s.Bm, &s.Cm, s.D, s.z, s.init, s.bias})) {
       Tensor y, fin, ws;
       sel_forward(s, y, fin, ws, false);
@@ -1238,6 +1243,7 @@ PyObject* py_carry(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     const Args a(argv, argc, 6);
     const Tensor &in = a.tensor(0, "input"), &w = a.tensor(1, "weight");
     const Tensor *b = a.opt(2, "bias"), *h = a.opt(3, "history"), *l = a.opt(4, "lengths");
+    no_tangents("causal_conv1d_carry", {&in, &w, b, h});
     if (!any_requires_grad({&in, &w, b, h})) {
       Tensor out, nh;
       carry_forward(in, w, b, h, l, a.flag(5), out, nh);
@@ -1293,6 +1299,7 @@ PyObject* py_linear(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     const Args a(argv, argc, 5);
     const Tensor &x = a.tensor(0, "x"), &w = a.tensor(1, "weight");
     const Tensor *b = a.opt(2, "bias"), *r = a.opt(3, "residual");
+    no_tangents("linear", {&x, &w, b, r});
     if (!any_requires_grad({&x, &w, b, r})) {
       Tensor out, pre;
       linear_fwd(x, w, b, r, a.integer(4), false, out, pre);
