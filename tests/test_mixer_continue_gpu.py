@@ -1,0 +1,99 @@
+"""mamba2_mixer continued: a prompt, then tokens; a sequence in pieces; gradients through the history and the state."""
+import pytest
+import torch
+
+from tests._util import assert_close
+from tests.test_mixer_gpu import DEV, TD, _mamba2
+
+pytestmark = pytest.mark.gpu
+
+
+def _layer(dtype, L, **size):
+    p, kw = _mamba2(dtype, **size)
+    g = torch.Generator().manual_seed(2)
+    u = torch.randn(3, L, 64, generator=g).to(TD[dtype]).to(DEV)
+    return u, {k: v.to(DEV) for k, v in p.items()}, kw
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("H,P,N", [(8, 32, 64), (3, 8, 16)])     # rows of the projection on 16 bytes, and off them
+@pytest.mark.parametrize("cut", [1, 2, 3, 25])                   # prompts shorter than the window, as long, longer
+def test_a_prompt_then_tokens(lib, dtype, H, P, N, cut):
+    """The prompt's history and state, stepped on in place, give what the whole sequence gives."""
+    import trading_bot_0_b200 as T
+    L = 33
+    u, p, kw = _layer(dtype, L, H=H, P=P, N=N)
+    more = dict(algo="fp32_cores")
+    whole, final = T.mamba2_mixer(u, **p, **kw, residual=u, **more)
+    out, history, state = T.mamba2_mixer(u[:, :cut], **p, **kw, residual=u[:, :cut], return_history=True, **more)
+    assert_close("prompt", out, whole[:, :cut], dtype)
+    ys = [T.mamba2_mixer_step(u[:, t], history, state, **p, **kw, residual=u[:, t]) for t in range(cut, L)]
+    assert_close("tokens", torch.stack(ys, 1), whole[:, cut:], dtype)
+    assert_close("state", state, final, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_a_sequence_in_pieces(lib, dtype):
+    import trading_bot_0_b200 as T
+    u, p, kw = _layer(dtype, 70)
+    whole, hist, final = T.mamba2_mixer(u, **p, **kw, return_history=True, chunk=64)
+    outs, history, state = [], None, None
+    for lo, hi in ((0, 2), (2, 3), (3, 40), (40, 70)):
+        out, history, state = T.mamba2_mixer(u[:, lo:hi], **p, **kw, history=history, state=state, return_history=True, chunk=64)
+        outs.append(out)
+    assert_close("out", torch.cat(outs, 1), whole, dtype)
+    assert torch.equal(history, hist)
+    assert_close("state", state, final, dtype)
+    two = T.mamba2_mixer(u[:, 40:], **p, **kw, history=torch.zeros_like(hist), state=torch.zeros_like(final), chunk=64)
+    assert len(two) == 2 and len(T.mamba2_mixer(u, **p, **kw)) == 2
+    fresh, _ = T.mamba2_mixer(u[:, 40:], **p, **kw, chunk=64)
+    assert_close("a history and a state of zeros", two[0], fresh, dtype)
+
+
+def test_gradients_through_the_pieces(lib):
+    """fp32: the gradients of a loss over the pieces are those of the same loss over the whole, for the input and every parameter."""
+    import trading_bot_0_b200 as T
+    u, p, kw = _layer("fp32", 37)
+    g = torch.Generator().manual_seed(3)
+    dout, dfin = torch.randn(3, 37, 64, generator=g).to(DEV), torch.randn(3, kw["nheads"], kw["headdim"], kw["dstate"], generator=g).to(DEV)
+    leaves = [u.requires_grad_(), *(v.requires_grad_() for v in p.values())]
+    out, hist, fin = T.mamba2_mixer(u, **p, **kw, residual=u, return_history=True)
+    dh = torch.randn(hist.shape, generator=g).to(DEV)
+    want = torch.autograd.grad([out, hist, fin], leaves, [dout, dh, dfin])
+    outs, history, state = [], None, None
+    for lo, hi in ((0, 2), (2, 20), (20, 37)):
+        o, history, state = T.mamba2_mixer(u[:, lo:hi], **p, **kw, residual=u[:, lo:hi], history=history, state=state, return_history=True)
+        outs.append(o)
+    got = torch.autograd.grad([torch.cat(outs, 1), history, state], leaves, [dout, dh, dfin])
+    for k, a, b in zip(["u", *p], got, want):
+        assert_close(k, a, b, "fp32")
+
+
+def test_a_piece_and_a_step_in_captured_graphs(lib):
+    import trading_bot_0_b200 as T
+    u, p, kw = _layer("bf16", 20)
+    _, history, state = T.mamba2_mixer(u[:, :9], **p, **kw, return_history=True)
+    h, s, x, tok = history.clone(), state.clone(), u[:, 9:19].clone(), u[:, 19].clone()
+
+    def on():
+        out, h2, s2 = T.mamba2_mixer(x, **p, **kw, history=h, state=s, return_history=True)
+        return [out, T.mamba2_mixer_step(tok, h2, s2, **p, **kw), h2, s2]
+    on()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = on()
+    x.copy_(x.flip(1))
+    h.neg_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(held, on()))
+
+
+def test_histories_and_states_that_do_not_fit_are_refused(lib):
+    import trading_bot_0_b200 as T
+    u, p, kw = _layer("bf16", 8)
+    _, h, s = T.mamba2_mixer(u, **p, **kw, return_history=True)
+    for bad in (dict(history=h[:, 1:]), dict(history=h.float()), dict(history=h[:2]), dict(state=s[:2]), dict(state=s.bfloat16()),
+                dict(history=h, state=s[:, 1:])):
+        with pytest.raises(ValueError):
+            T.mamba2_mixer(u, **p, **kw, **bad)

@@ -13,10 +13,12 @@ during the capture: autograd then waits on the stream of that graph's accumulati
 """
 from __future__ import annotations
 
+import torch
+
 from .linear import linear
-from .prepost import causal_conv1d_carry, conv1d_step, mamba2_mixer_core, rmsnorm_forward
+from .prepost import causal_conv1d_carry, conv1d_step, mamba2_mixer_core, rmsnorm, rmsnorm_forward
 from .selective import selective_scan, selective_step
-from .ssd import state_update
+from .ssd import ssd_scan, state_update
 
 
 def _aligned(t):
@@ -31,15 +33,33 @@ def _mamba2_parts(zxbcdt, hp, gn):
     return _aligned(z), _aligned(xBC), dt
 
 
+def _last_rows(t, n):
+    """The last n rows of t [batch, rows, channels], zeros before its first: the history that a convolution leaves."""
+    rows = t.shape[1]
+    return (t[:, rows - n:] if rows >= n else torch.nn.functional.pad(t, (0, 0, n - rows, 0))).contiguous()
+
+
 def mamba2_mixer(u, in_proj, conv_weight, conv_bias, dt_bias, A, D, norm_weight, out_proj, *, nheads, headdim, dstate, ngroups, residual=None,
-                 in_bias=None, out_bias=None, chunk=128, eps=1e-5, algo="auto"):
+                 in_bias=None, out_bias=None, chunk=128, eps=1e-5, algo="auto", history=None, state=None, return_history=False):
     """Differentiable.  in_proj gives the columns z (nheads*headdim) | x, B, C (nheads*headdim + 2*ngroups*dstate) | dt (nheads).
-    Returns out [batch, seqlen, out features] and the scan's final state."""
-    hp, gn = nheads * headdim, ngroups * dstate
+    `history` [batch, width-1, conv channels] and `state` [batch, nheads, headdim, dstate] continue an earlier call.  Returns out
+    [batch, seqlen, out features] and the scan's final state; with `return_history` out, the new history and the state, which are what
+    mamba2_mixer_step goes on with.  All rows of a batch are of one length (the scan takes no lengths)."""
+    hp, gn, heads = nheads * headdim, ngroups * dstate, (nheads, headdim)
     z, xBC, dt = _mamba2_parts(linear(u, in_proj, in_bias), hp, gn)
-    y, final = mamba2_mixer_core(xBC, dt, z.unflatten(-1, (nheads, headdim)), conv_weight, conv_bias, dt_bias, A, D, norm_weight,
-                                 nheads=nheads, headdim=headdim, dstate=dstate, ngroups=ngroups, chunk=chunk, eps=eps, algo=algo)
-    return linear(y, out_proj, out_bias, residual), final
+    if history is None:
+        y, final = mamba2_mixer_core(xBC, dt, z.unflatten(-1, heads), conv_weight, conv_bias, dt_bias, A, D, norm_weight, nheads=nheads,
+                                     headdim=headdim, dstate=dstate, ngroups=ngroups, chunk=chunk, eps=eps, algo=algo, init_state=state)
+        if return_history:
+            history = _last_rows(xBC, conv_weight.shape[1] - 1)
+    else:
+        c, history = causal_conv1d_carry(xBC, conv_weight, conv_bias, history)
+        x, Bm, Cm = c.split([hp, gn, gn], -1)
+        y, final = ssd_scan(x.unflatten(-1, heads), dt, A, Bm.unflatten(-1, (ngroups, dstate)), Cm.unflatten(-1, (ngroups, dstate)), D,
+                            z.unflatten(-1, heads), state, chunk=chunk, algo=algo, dt_bias=dt_bias, dt_softplus=True)
+        y = rmsnorm(y.flatten(2), norm_weight, eps=eps)
+    out = linear(y, out_proj, out_bias, residual)
+    return (out, history, final) if return_history else (out, final)
 
 
 def mamba2_mixer_step(u, history, state, in_proj, conv_weight, conv_bias, dt_bias, A, D, norm_weight, out_proj, *, nheads, headdim, dstate,
