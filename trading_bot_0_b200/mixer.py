@@ -15,10 +15,16 @@ from __future__ import annotations
 
 import torch
 
-from .linear import linear
+from .linear import linear, linear_forward
 from .prepost import causal_conv1d_carry, conv1d_step, mamba2_mixer_core, rmsnorm, rmsnorm_forward
 from .selective import selective_scan, selective_step
 from .ssd import ssd_scan, state_update
+
+
+def _project(x, weight, bias=None, residual=None):
+    """linear outside of autograd: a step's convolution and scan have no gradient, and a graph of its projections alone would give
+    part of one."""
+    return linear_forward(x, weight, bias, residual)[0]
 
 
 def _aligned(t):
@@ -64,20 +70,21 @@ def mamba2_mixer(u, in_proj, conv_weight, conv_bias, dt_bias, A, D, norm_weight,
 
 def mamba2_mixer_step(u, history, state, in_proj, conv_weight, conv_bias, dt_bias, A, D, norm_weight, out_proj, *, nheads, headdim, dstate,
                       ngroups, residual=None, in_bias=None, out_bias=None, eps=1e-5):
-    """One token per stream, IN PLACE on `history` [streams, width-1, conv channels] and `state` [streams, nheads, headdim, dstate]."""
+    """One token per stream, IN PLACE on `history` [streams, width-1, conv channels] and `state` [streams, nheads, headdim, dstate].  No
+    part of an autograd graph."""
     hp, gn = nheads * headdim, ngroups * dstate
-    z, xBC, dt = _mamba2_parts(linear(u, in_proj, in_bias), hp, gn)
+    z, xBC, dt = _mamba2_parts(_project(u, in_proj, in_bias), hp, gn)
     c = conv1d_step(history, xBC, conv_weight, conv_bias)
     y = state_update(state, c[:, :hp].unflatten(1, (nheads, headdim)), dt, A, c[:, hp:hp + gn].unflatten(1, (ngroups, dstate)),
                      c[:, hp + gn:].unflatten(1, (ngroups, dstate)), D, z.unflatten(1, (nheads, headdim)), dt_bias=dt_bias, dt_softplus=True)
     y, _ = rmsnorm_forward(y.view(-1, hp), norm_weight, eps=eps)
-    return linear(y, out_proj, out_bias, residual)
+    return _project(y, out_proj, out_bias, residual)
 
 
-def _selective_parts(x, x_proj, dt_proj, dstate):
-    dbc = linear(x, x_proj)
+def _selective_parts(x, x_proj, dt_proj, dstate, project):
+    dbc = project(x, x_proj)
     rank = dbc.shape[-1] - 2 * dstate
-    return linear(dbc[..., :rank], dt_proj), dbc[..., rank:rank + dstate], dbc[..., rank + dstate:]
+    return project(dbc[..., :rank], dt_proj), dbc[..., rank:rank + dstate], dbc[..., rank + dstate:]
 
 
 def selective_mixer(u, in_proj, conv_weight, conv_bias, x_proj, dt_proj, dt_bias, A, D, out_proj, *, residual=None, history=None, state=None,
@@ -88,16 +95,17 @@ def selective_mixer(u, in_proj, conv_weight, conv_bias, x_proj, dt_proj, dt_bias
     D_, N = A.shape
     xz = linear(u, in_proj)
     x, history = causal_conv1d_carry(_aligned(xz[..., :D_]), conv_weight, conv_bias, history, lengths=lengths)
-    dt, Bm, Cm = _selective_parts(x, x_proj, dt_proj, N)
+    dt, Bm, Cm = _selective_parts(x, x_proj, dt_proj, N, linear)
     y, state = selective_scan(x, dt, A, Bm, Cm, D, xz[..., D_:], state, dt_bias=dt_bias, dt_softplus=True, lengths=lengths)
     return linear(y, out_proj, None, residual), history, state
 
 
 def selective_mixer_step(u, history, state, in_proj, conv_weight, conv_bias, x_proj, dt_proj, dt_bias, A, D, out_proj, *, residual=None):
-    """One token per stream, IN PLACE on `history` [streams, width-1, channels] and `state` [streams, channels, dstate]."""
+    """One token per stream, IN PLACE on `history` [streams, width-1, channels] and `state` [streams, channels, dstate].  No part of an
+    autograd graph."""
     D_, N = A.shape
-    xz = linear(u, in_proj)
+    xz = _project(u, in_proj)
     x = conv1d_step(history, _aligned(xz[:, :D_]), conv_weight, conv_bias)
-    dt, Bm, Cm = _selective_parts(x, x_proj, dt_proj, N)
+    dt, Bm, Cm = _selective_parts(x, x_proj, dt_proj, N, _project)
     y = selective_step(state, x, dt, A, Bm, Cm, D, xz[:, D_:], dt_bias=dt_bias, dt_softplus=True)
-    return linear(y, out_proj, None, residual)
+    return _project(y, out_proj, None, residual)
