@@ -986,11 +986,16 @@ struct SelPlan {
   size_t ckpt, segst, segdt, part_bc, part_par, fwd_bytes, bwd_bytes;   // offsets and totals
 };
 
-// Parts of the sequence.  n blocks walk the tokens one after the other; below about two of them to an SM the SMs mostly wait, and the
-// sequence is cut into parts, which costs a pass over the steps for the states (or gradients) that the parts begin with.  Measured
-// (us, forward with that pass; parts 1, 6, 12, 24): 1 x 4096 x 1536 (24 blocks) 636, 188, 126, 102; 4 x 2048 x 1536 (96) 337, 184,
-// 183, 191; 64 x 512 x 512 (512) 154 with one part, 195 with two.  Backward (parts 1, 4, 8, 16): 4 x 2048 x 1536 (192 blocks) 655,
-// 467, 446, 434; 2 x 512 x 768 (48) 125, 59, 43, 45; 64 x 512 x 512 (1024) 541, 551, 575, 647.
+// Parts of the sequence.  n blocks walk the tokens one after the other; where they are few the SMs mostly wait, and the sequence is cut into
+// parts, which costs a pass over the steps for the states (or gradients) that the parts begin with: about eight blocks to an SM in all, as
+// far as a part keeps `least_tiles` tiles.  Measured (us of the call, L2 flushed; parts, the rule's choice in brackets), 16 states, bf16, gated:
+//   forward    1 x 4096 x 1536 (24 blocks)  1: 621, 12: 114, 24: 93, [43: 95], 64: 108     12 x 1024 x 1024 (192)  1: 188, 4: 165, [6: 158], 8: 162
+//              4 x 2048 x 1536 (96)         1: 316, 4: 197, [12: 167], 24: 169             14 x 1024 x 1024 (224)  1: 188, 4: 190, [5: 184]
+//              2 x 512 x 768 (24)           1: 84, 4: 42, 8: 32, [16: 26]                  16 x 1024 x 1024 (256)  [1: 188], 4: 201; 8 x 4096 x 2048 (256)  [1: 727], 4: 758
+//   backward   1 x 4096 x 1536 (48 blocks)  1: 1183, 8: 270, [24: 223], 48: 231            12 x 1024 x 1024 (384)  1: 427, 2: 486, [3: 396], 4: 407
+//              4 x 2048 x 1536 (192)        1: 707, 3: 417, 4: 485, [6: 406], 16: 417      14 x 1024 x 1024 (448)  [1: 483], 2: 513, 4: 496
+//              2 x 512 x 768 (48)           1: 159, 4: 67, [8: 47], 16: 48                 64 x 512 x 512 (1024)   [1: 474], 2: 502, 4: 513
+// so one part from 1.7 blocks to an SM on in the forward and from 2.8 in the backward.
 int choose_parts(long long n, int L, long long below, int least_tiles) {
   const int tiles = cdiv(L, SEL_T);
   if (n >= below) return 1;
@@ -1033,8 +1038,8 @@ int make_sel_plan(const SsdSelDims* d, SelPlan* o) {
     return SSD_ERR_BAD_SHAPE;
   }
   const long long nf = (long long)q.B * q.G * q.nb, nb = (long long)q.B * q.G * o->nb_bwd;
-  o->segs_fwd = choose_parts(nf, q.L, 2 * 148, 2);
-  o->segs_bwd = choose_parts(nb, q.L, 4 * 148, 4);
+  o->segs_fwd = choose_parts(nf, q.L, 246, 2);
+  o->segs_bwd = choose_parts(nb, q.L, 414, 4);
   if (nf * o->segs_fwd > 0x7fffffffLL || nb * o->segs_bwd > 0x7fffffffLL) { set_error("selscan: too many blocks for one grid"); return SSD_ERR_UNSUPPORTED; }
   q.segs = 1; q.seg_len = 0;
   const int most = o->segs_fwd > o->segs_bwd ? o->segs_fwd : o->segs_bwd;
