@@ -24,6 +24,8 @@ LARGE = [
     (2100, 40, 1300, "fp32", "silu"),        # 187 tiles of 128 x 128 on the CUDA cores
     (2600, 1288, 130, "fp32", "softplus"),   # dx on tiles of 128 x 128
     (2100, 41, 1300, "bf16", "relu2"),       # the same for bf16 rows that no tensor map takes
+    (200, 2048, 131, "bf16", "silu"),        # splits whose sums no tensor map takes
+    (90, 1544, 133, "bf16", "softplus"),     # the same with the weights as the tiles' rows
     (3, 64, 8200, "bf16", "silu"),           # few rows: two features to a warp, the last warps with one and none
     (8, 72, 8193, "fp32", "softplus"),
     (1, 40, 9001, "bf16", "none"),
