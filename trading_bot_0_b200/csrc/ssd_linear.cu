@@ -219,7 +219,8 @@ __global__ void __launch_bounds__(256) k_mm_few(MmArgs a) {
 // sums in the workspace and k_mm2_join adds them in order.  Every wait is bounded: when one runs out a code goes to the status word, the
 // outputs become NaN, and a later product of the same call waits for nothing and gives NaN.
 //
-// Measured with cuBLAS beside it in one run: 8192^3 694 us = 1.58 PFLOP/s (647), 16384 x 768 x 3352 76 (72), 4096 x 2048 x 2048 45 (41),
+// Measured with cuBLAS beside it in one run, bare calls after an L2 flush (one after the other, as a layer makes them, the second takes 86
+// to 89): 8192^3 694 us = 1.58 PFLOP/s (647), 16384 x 768 x 3352 76 (72), 4096 x 2048 x 2048 45 (41),
 // 512 x 768 x 1536 14 (8).  8192^3 before and after on one board: 785 us with loads and MMAs issued by `lane == 0`, 677 by an elected
 // lane, whatever the tile's width; four stages are as fast as five, three 10 % slower;
 // both accumulators as one tile of 256 x 512, which loads a quarter less, 670 us, but 103 against 77 us at 16384 x 768 x 3352, where
@@ -533,9 +534,12 @@ __global__ void __launch_bounds__(256) k_mm2_join(Mm2 a, long long rows, int col
   }
 }
 
-// dpre = dout act'(pre), rounded to the storage type (what the two products read), and the column sums of the unrounded dpre over a
+// dpre = dout act'(pre), rounded to the storage type, and the column sums of the unrounded dpre over a
 // part of the rows (`parts` of them on the y axis).  Thread = V neighbouring columns, block = 32 V columns x 8 rows at a time, four
 // rows of a thread requested together.  V = 16 bytes where all rows start on 16 bytes, else one value.
+// The rounding is what bf16 operands of the two products mean: dx and dweight carry it beside the rounding of the result, each 0.0017 rms of
+// the gradient, 0.0023 to 0.0024 together (16384 x 1536 x 768).  Without it dpre would be two bf16 parts and both products twice as long
+// (43 us each there).  fp32 storage rounds nothing here.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) k_dpre(long long M, int N, int act, const T* __restrict__ dout, long long dos, const float* __restrict__ pre,
                                               T* __restrict__ dpre, float* __restrict__ partial, int* status) {

@@ -515,8 +515,9 @@ template <class S> struct ChannelSum {
   }
 };
 
-// Four blocks to an SM.  4 x 2048 x 1536 of 16 states, bf16, gated: 322 us; three blocks 360; when it took 343, five spilled and took
-// 418.  Keeping eight tokens' decays beside their states took 383 where recomputing them took 358, eight states a thread 424 to 491.
+// Four blocks to an SM, so 128 registers, with 56 bytes of spills for 16 states in bf16, gated (12 to 84 for the other shapes of 128 threads).
+// 4 x 2048 x 1536 of 16 states, bf16, gated: 322 us; three blocks 360; when it took 343, five spilled more and took 418.  From 33 states on
+// the shared memory leaves room for two blocks, and the bound costs 320 to 588 bytes of spills for nothing (fp32 of 8 states: for three).  Keeping eight tokens' decays beside their states took 383 where recomputing them took 358, eight states a thread 424 to 491.
 // At a quarter of the length: issue slots 52 % busy, the shared-memory path 63 %, special functions 31 %.
 template <typename T, class S, bool GATED>
 __global__ void __launch_bounds__(S::TH, S::TH == 128 ? 4 : 1) k_sel_bwd(SelGeo q, SelBwd p) {

@@ -27,7 +27,9 @@ def linear_forward(x, weight, bias=None, residual=None, *, activation="none", fo
 
 
 def linear_backward(dout, x, weight, pre=None, *, activation="none", bias=True, want_dx=True, want_dweight=True):
-    """dx, dweight, dbias (None where not wanted); the gradient of the residual is dout."""
+    """dx, dweight, dbias (None where not wanted); the gradient of the residual is dout.  In bf16 with an activation dout act'(pre) is rounded
+    to bf16 as the products' operand, which adds as much to the error of dx and dweight as rounding them does (0.0023 of their size in all
+    where the latter alone gives 0.0017); dbias is summed before that."""
     return L.host().linear_backward(dout, x, weight, pre, _act(activation), want_dx, want_dweight, bias)
 
 

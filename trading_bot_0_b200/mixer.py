@@ -91,7 +91,8 @@ def selective_mixer(u, in_proj, conv_weight, conv_bias, x_proj, dt_proj, dt_bias
                     lengths=None):
     """Differentiable.  in_proj gives the columns x | z (channels each), x_proj dt's factor (rank) | B | C (dstate each), dt_proj the
     channels' step sizes.  `history` [batch, width-1, channels] and `state` [batch, channels, dstate] continue an earlier call; `lengths`
-    (int32 [batch] on the device) ends rows early.  Returns out, the new history and the new state."""
+    (int32 [batch] on the device) ends rows early: out is the residual there, or zero, and gradients are zeros; u has to be finite there all
+    the same, since its rows take part in the projections' products.  Returns out, the new history and the new state."""
     D_, N = A.shape
     xz = linear(u, in_proj)
     x, history = causal_conv1d_carry(_aligned(xz[..., :D_]), conv_weight, conv_bias, history, lengths=lengths)
