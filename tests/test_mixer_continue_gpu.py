@@ -97,3 +97,22 @@ def test_histories_and_states_that_do_not_fit_are_refused(lib):
                 dict(history=h, state=s[:, 1:])):
         with pytest.raises(ValueError):
             T.mamba2_mixer(u, **p, **kw, **bad)
+
+
+@pytest.mark.parametrize("B,L,H,P", [(1, 9, 8, 32), (1, 9, 3, 8), (2, 3, 3, 8), (1, 1, 8, 32)])
+@pytest.mark.parametrize("K", [2, 4])
+def test_the_history_is_memory_of_its_own(lib, B, L, H, P, K):
+    """Stepping on with a prompt's history leaves the prompt's graph as it was, whatever the rows' layout, and holds nothing of the
+    projection's output."""
+    import trading_bot_0_b200 as T
+    p, kw = _mamba2("fp32", H=H, P=P, N=16)
+    p["conv_weight"] = p["conv_weight"][:, :K].contiguous()
+    p = {k: v.to(DEV) for k, v in p.items()}
+    u = torch.randn(B, L, 64, generator=torch.Generator().manual_seed(6)).to(DEV)
+    leaf = p["in_proj"].requires_grad_()
+    out, history, state = T.mamba2_mixer(u, **p, **kw, return_history=True)
+    want = torch.autograd.grad(out.sum(), leaf, retain_graph=True)[0]
+    h = history.detach()
+    assert h.untyped_storage().nbytes() == h.numel() * 4
+    T.mamba2_mixer_step(u[:, 0], h, state.detach().clone(), **p, **kw)
+    assert torch.equal(torch.autograd.grad(out.sum(), leaf)[0], want)

@@ -42,7 +42,8 @@ def _mamba2_parts(zxbcdt, hp, gn):
 def _last_rows(t, n):
     """The last n rows of t [batch, rows, channels], zeros before its first: the history that a convolution leaves."""
     rows = t.shape[1]
-    return (t[:, rows - n:] if rows >= n else torch.nn.functional.pad(t, (0, 0, n - rows, 0))).contiguous()
+    last = t[:, rows - n:] if rows >= n else torch.nn.functional.pad(t, (0, 0, n - rows, 0))
+    return last.clone(memory_format=torch.contiguous_format)     # (some rows of one sequence are contiguous where they are)
 
 
 def mamba2_mixer(u, in_proj, conv_weight, conv_bias, dt_bias, A, D, norm_weight, out_proj, *, nheads, headdim, dstate, ngroups, residual=None,
