@@ -116,3 +116,20 @@ def test_the_history_is_memory_of_its_own(lib, B, L, H, P, K):
     assert h.untyped_storage().nbytes() == h.numel() * 4
     T.mamba2_mixer_step(u[:, 0], h, state.detach().clone(), **p, **kw)
     assert torch.equal(torch.autograd.grad(out.sum(), leaf)[0], want)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("H,P", [(3, 8), (5, 8), (8, 32)])
+def test_one_row_whose_stride_is_off_16_bytes(lib, dtype, H, P):
+    """A prompt of one token of one sequence: its row has no neighbour, whatever the strides say.  As in a batch of two."""
+    import trading_bot_0_b200 as T
+    u, p, kw = _layer(dtype, 1, H=H, P=P, N=16)
+    both, hists, finals = T.mamba2_mixer(u[:2], **p, **kw, return_history=True)
+    for i in range(2):
+        out, history, final = T.mamba2_mixer(u[i:i + 1], **p, **kw, return_history=True)
+        assert torch.equal(out[0], both[i]) and torch.equal(history[0], hists[i]) and torch.equal(final[0], finals[i])
+        again, h2, f2 = T.mamba2_mixer(u[i:i + 1], **p, **kw, history=torch.zeros_like(history), state=torch.zeros_like(final), return_history=True)
+        assert torch.equal(h2, history)
+        assert_close("with a history of zeros", again, out, dtype)
+        step = T.mamba2_mixer_step(u[i], torch.zeros_like(history), torch.zeros_like(final), **p, **kw)
+        assert_close("as a step", step, out[:, 0], dtype)

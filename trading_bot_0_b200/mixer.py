@@ -28,10 +28,11 @@ def _project(x, weight, bias=None, residual=None):
 
 
 def _aligned(t):
-    """`t` itself where its rows start on 16 bytes (what the conv and the tensor-core scan take), else a copy."""
+    """`t` itself where its rows start on 16 bytes (what the conv and the tensor-core scan take), else a copy; a single row too has a
+    stride that they look at."""
     e = t.element_size()
-    rows = [t.stride(i) for i in range(t.dim() - 1) if t.size(i) > 1]
-    return t if t.data_ptr() % 16 == 0 and all(r * e % 16 == 0 for r in rows) else t.contiguous()
+    ok = t.data_ptr() % 16 == 0 and all(t.stride(i) * e % 16 == 0 for i in range(t.dim() - 1))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def _mamba2_parts(zxbcdt, hp, gn):
