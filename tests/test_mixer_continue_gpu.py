@@ -133,3 +133,40 @@ def test_one_row_whose_stride_is_off_16_bytes(lib, dtype, H, P):
         assert_close("with a history of zeros", again, out, dtype)
         step = T.mamba2_mixer_step(u[i], torch.zeros_like(history), torch.zeros_like(final), **p, **kw)
         assert_close("as a step", step, out[:, 0], dtype)
+
+
+@pytest.mark.parametrize("B,L", [(1, 1), (2, 1), (1, 2), (1, 5), (4, 3)])
+@pytest.mark.parametrize("odd", [False, True])
+def test_the_smallest_batches_train(lib, B, L, odd):
+    """Both mixers with a handful of tokens, columns on 16 bytes and off them, against 64 bits; with and without the pieces' operands."""
+    import trading_bot_0_b200 as T
+    from tests.test_mixer_gpu import _mamba2_ref, _selective, _selective_ref
+    size = dict(D=40, N=12, rank=3) if odd else {}
+    u, p, dout = _selective("fp32", B=B, L=L, **size)
+    leaves = [u.double().requires_grad_(), *(v.double().requires_grad_() for v in p.values())]
+    ref, _ = _selective_ref(leaves[0], dict(zip(p, leaves[1:])), leaves[0])
+    want = torch.autograd.grad(ref, leaves, dout.double())
+    mine = [u.to(DEV).requires_grad_(), *(v.to(DEV).requires_grad_() for v in p.values())]
+    D, N = p["A"].shape
+    for extra in ({}, dict(history=torch.zeros(B, 3, D, device=DEV), state=torch.zeros(B, D, N, device=DEV))):
+        out, _, _ = T.selective_mixer(mine[0], **dict(zip(p, mine[1:])), residual=mine[0], **extra)
+        assert_close("out", out.detach(), ref.detach(), "fp32")
+        for k, a, b in zip(["u", *p], torch.autograd.grad(out, mine, dout.to(DEV)), want):
+            assert_close(k, a, b, "fp32")
+    H, P, N = (3, 8, 16) if odd else (8, 32, 64)
+    p, kw = _mamba2("fp32", H=H, P=P, N=N)
+    g = torch.Generator().manual_seed(1)
+    u, dout = torch.randn(B, L, 64, generator=g), torch.randn(B, L, 64, generator=g)
+    leaves = [u.double().requires_grad_(), *(v.double().requires_grad_() for v in p.values())]
+    ref, _ = _mamba2_ref(leaves[0], dict(zip(p, leaves[1:])), H, P, N, 1, leaves[0])
+    want = torch.autograd.grad(ref, leaves, dout.double())
+    mine = [u.to(DEV).requires_grad_(), *(v.to(DEV).requires_grad_() for v in p.values())]
+    for extra in ({}, dict(history=torch.zeros(B, 3, p["conv_weight"].shape[0], device=DEV), state=torch.zeros(B, H, P, N, device=DEV))):
+        out, _ = T.mamba2_mixer(mine[0], **dict(zip(p, mine[1:])), **kw, residual=mine[0], **extra)
+        assert_close("out", out.detach(), ref.detach(), "fp32")
+        grads = dict(zip(["u", *p], torch.autograd.grad(out, mine, dout.to(DEV))))
+        if L == 1:      # the decay meets a state of zeros: dA is 0, the difference of sums whose size is that of dD's; no size of its own to go by
+            assert grads.pop("A").abs().max() <= 1e-4 * grads["D"].abs().max()
+        for k, b in zip(["u", *p], want):
+            if k in grads:
+                assert_close(k, grads[k], b, "fp32")
