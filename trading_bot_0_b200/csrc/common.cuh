@@ -82,6 +82,11 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 // The sums of R values over groups of LPR lanes, R values at a time: every exchange folds two values into one, so a tile row
 // set costs R - 1 + log2(LPR / R) shuffles instead of R log2(LPR).  Lane `lir` ends up with the sum of value `u` (returned);
 // all lanes whose lir agrees in its log2(R) top bits hold the same one.

@@ -101,11 +101,19 @@ template <> __device__ __forceinline__ float sig_<__nv_bfloat16>(float a) {
 }
 template <> __device__ __forceinline__ float sig_<float>(float a) { return __fdividef(1.f, 1.f + __expf(-a)); }
 // The silu of the convolution with a history, in either storage type: exp and a reciprocal without the cases of denormals, as exact as
-// the latter of these (16 x 4096 x 1792 bf16: 105 us, with sig_<float> 117, with tanh.approx 98 to 103).
+// the latter of these (16 x 4096 x 1792 bf16: 103 us, 105 with one value at a time, 117 with sig_<float>, 101 with tanh.approx).
 __device__ __forceinline__ float silu_(float a) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + umma::ex2(-LOG2E * a)));
   return a * r;
+}
+__device__ __forceinline__ void silu2_(f32x2 a, float& lo, float& hi) {   // the same of a pair, the same bits
+  float x, y;
+  unpack2(mul2(a, pack2(-LOG2E, -LOG2E)), x, y);
+  unpack2(add2(pack2(umma::ex2(x), umma::ex2(y)), pack2(1.f, 1.f)), x, y);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(y));
+  unpack2(mul2(a, pack2(x, y)), lo, hi);
 }
 
 // NC storage elements -> NC/2 packed pairs
@@ -239,7 +247,7 @@ __device__ __forceinline__ int carry_ext(const SsdConvDims& d, const Carry& q, i
   return K - 1 + (q.lengths ? min(max(__ldg(q.lengths + b), 0), d.seqlen - (K - 1)) : d.seqlen - (K - 1));
 }
 // CARRY: rows before the sequence's first come from the history, and the CTAs of a sequence's first tile write the new one.
-// 16 x 4096 x 1792 bf16: 105 us, 4.5 TB/s, issue slots 66 % busy, special functions 50 %; 64 x 1000 x 384 fp32: 35 us (under ncu).
+// 16 x 4096 x 1792 bf16: 103 us, 4.5 TB/s, issue slots 63 % busy, special functions 52 %; 64 x 1000 x 384 fp32: 34 us (under ncu).
 template <typename T, int K, bool CARRY>
 __global__ void __launch_bounds__(CONVS_THREADS, CONVS_CTAS_PER_SM)
 k_conv_fwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__ weight, const float* __restrict__ bias,
@@ -330,10 +338,11 @@ k_conv_fwd_sm(SsdConvDims d, const T* __restrict__ in, const float* __restrict__
         f32x2 a2 = bs[j];
 #pragma unroll
         for (int k = 0; k < K; ++k) a2 = fma2(w[j][k], win[k][j], a2);
+        if (CARRY && d.activation) { silu2_(a2, o[2 * j], o[2 * j + 1]); continue; }
         float a, b;
         unpack2(a2, a, b);
-        o[2 * j] = d.activation ? (CARRY ? silu_(a) : a * sig_<T>(a)) : a;
-        o[2 * j + 1] = d.activation ? (CARRY ? silu_(b) : b * sig_<T>(b)) : b;
+        o[2 * j] = d.activation ? a * sig_<T>(a) : a;
+        o[2 * j + 1] = d.activation ? b * sig_<T>(b) : b;
       }
       if (CARRY && t0 + i >= len) {                  // (the same for a whole warp)
 #pragma unroll

@@ -65,11 +65,6 @@ __device__ __forceinline__ float sel_step_d(float raw, float bias, int softplus,
   return fmaxf(v, 0.f) + log1p01(e);
 }
 __device__ __forceinline__ float sig(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 __device__ __forceinline__ float hsum(f32x2 v) { float a, b; unpack2(v, a, b); return a + b; }
 __device__ __forceinline__ f32x2 dup2(float v) { return pack2(v, v); }
 __device__ __forceinline__ f32x2 ex2_2(f32x2 v) { float a, b; unpack2(v, a, b); return pack2(ex2(a), ex2(b)); }
