@@ -189,3 +189,21 @@ def test_rows_end_inside_a_tile(lib, dtype, N):
         for k in ("dx", "ddt", "dz", "dB", "dC"):
             assert torch.equal(g1[k][0], gr[k][i, :m]), (k, m)
         assert torch.equal(g1["dinit"][0], gr["dinit"][i]), m
+
+
+@pytest.mark.parametrize("D,N,L", [(256, 16, 50), (512, 8, 50), (64, 64, 50), (256, 16, 200)])    # the last one in parts
+def test_a_scans_decays_are_unbiased(lib, D, N, L):
+    """The same over a sequence, forward (the final state) and backward (the gradient of the initial one); steps that vary from token to
+    token, and a decay of at least exp(-50) over all.  Bound as above, the state's roundings 2^-24 / sqrt(3) / sqrt(L D N) each."""
+    from trading_bot_0_b200 import selective as S
+    g = torch.Generator().manual_seed(D + N + L)
+    A = -torch.exp(torch.rand(D, N, generator=g) * 2.0 - 2.0)
+    s = (0.02 + 0.48 * torch.rand(1, L, D, generator=g)) * 50 / max(L, 50)
+    h0 = 1.0 + torch.rand(1, D, N, generator=g)
+    z, bc = torch.zeros(1, L, D, device=DEV), torch.zeros(1, L, N, device=DEV)
+    _, fin, _ = S.selective_scan_forward(z, dev(s), dev(A), bc, bc, init_state=dev(h0))
+    dinit = S.selective_scan_backward(z, z, dev(s), dev(A), bc, bc, init_state=dev(h0), dfinal_state=dev(h0))["dinit"]
+    ref = h0.double() * torch.exp(s.double().sum(1)[..., None] * A.double())
+    for name, got in (("final state", fin), ("gradient of the initial state", dinit)):
+        off = ((got.double().cpu() - ref) / ref).mean().item() / L
+        assert abs(off) <= 0.6e-8 + 3 * 6e-10 + 1e-9, (name, off)

@@ -13,6 +13,7 @@ namespace ssd {
 namespace {
 
 __device__ __forceinline__ float relu(float v) { return v < 0.f ? 0.f : v; }   // (fmaxf would turn NaN into 0)
+// The sigmoids' relative error is (4 + 1.2 |v|) 2^-23: 1e-6 at 5; 3e-6 at -20, where silu is 4e-8.
 __device__ __forceinline__ float act_of(float v, int act) {
   if (act == SSD_ACT_SILU) return v * __fdividef(1.f, 1.f + __expf(-v));
   if (act == SSD_ACT_SOFTPLUS) return softplusf_(v);

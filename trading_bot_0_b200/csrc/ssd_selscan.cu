@@ -64,6 +64,7 @@ __device__ __forceinline__ float sel_step_d(float raw, float bias, int softplus,
   d = __fdividef(v >= 0.f ? 1.f : e, 1.f + e);
   return fmaxf(v, 0.f) + log1p01(e);
 }
+// relative error (4 + 1.2 |v|) 2^-23 (1e-6 at 5; 3e-6 at -20, where silu is 4e-8)
 __device__ __forceinline__ float sig(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
 __device__ __forceinline__ float hsum(f32x2 v) { float a, b; unpack2(v, a, b); return a + b; }
 __device__ __forceinline__ f32x2 dup2(float v) { return pack2(v, v); }
