@@ -28,6 +28,14 @@
 namespace ssd {
 namespace umma {
 
+// Calls `f`, which encodes a tensor map.  Encoding wants a current context, which a host thread has only from its first call that needs one
+// (a launch, say) on: where there is none yet, the current device's is made current and `f` called again.
+template <class F> CUresult in_context(F f) {
+  const CUresult r = f();
+  int dev = 0;
+  return r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess ? f() : r;
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // ---- mbarrier ------------------------------------------------------------------------------
