@@ -118,3 +118,60 @@ def test_scans_cut_into_parts_with_lengths(lib, dtype, B, L, D, N, G):
     terms = dict(dx=N, ddt=N, dz=N, dA=B * L, dD=B * L, ddt_bias=B * L + N, dB=D, dC=D, dinit=0)
     for k in g:
         TS.assert_near(k, g[k], ref[k], mag[k], T_, terms[k])
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_time_major_operands(lib, dtype):
+    """Operands laid out [tokens, batch, channels]: batch rows nearer than tokens.  The bits of dense ones."""
+    from trading_bot_0_b200 import linear as LN, prepost as P, selective as S
+    B, L, D, N = 3, 75, 136, 16
+    o, kw, dy, _ = TS._operands(B, L, D, N, 1, dtype, gate=True, bias=True, skip=True, init=True)
+    d = {k: dev(v) for k, v in o.items()}
+    turn = lambda v: v.transpose(0, 1).contiguous().transpose(0, 1)
+    kd = dict(dt_bias=dev(kw["dt_bias"]), dt_softplus=True, lengths=torch.tensor([75, 20, 64], dtype=torch.int32, device=DEV))
+
+    def scan(f):
+        a = (f(d["x"]), f(d["dt"]), d["A"], f(d["Bm"]), f(d["Cm"]), d["D"], f(d["z"]), d["init_state"])
+        y, fin, ws = S.selective_scan_forward(*a, for_backward=True, **kd)
+        g = S.selective_scan_backward(f(dev(dy)), *a, workspace=ws, **kd)
+        return [y, fin] + [g[k] for k in sorted(g)]
+    assert all(torch.equal(p, q) for p, q in zip(scan(turn), scan(lambda v: v)))
+    w = torch.randn(D, 4, device=DEV)
+
+    def conv(f):
+        return [*P.conv1d_carry_forward(f(d["x"]), w, lengths=kd["lengths"]),
+                *P.conv1d_carry_backward(f(d["x"]), w, None, None, f(dev(dy)), lengths=kd["lengths"])[:2]]
+    assert all(torch.equal(p, q) for p, q in zip(conv(turn), conv(lambda v: v)))
+    W = torch.randn(24, D, device=DEV).to(TD[dtype])
+    assert torch.equal(LN.linear(turn(d["x"]), W), LN.linear(d["x"], W))
+
+
+def test_layers_side_by_side_on_two_streams(lib):
+    """Training steps of both mixers at the same time on two streams, several times over: the bits of one after the other.  (Tensor memory,
+    shared memory and the SMs are shared; workspaces are not.)"""
+    import trading_bot_0_b200 as T
+    from tests.test_mixer_gpu import _mamba2, _selective
+    u, p, dout = _selective("bf16", B=4, L=512, d_model=256, D=512, rank=16)
+    q, kw = _mamba2("bf16", d_model=256, H=16)
+    u, dout = dev(u), dev(dout)
+    lp, lq = [dev(v).requires_grad_() for v in p.values()], [dev(v).requires_grad_() for v in q.values()]
+
+    def one():
+        out, _, _ = T.selective_mixer(u, **dict(zip(p, lp)), residual=u)
+        return [out, *torch.autograd.grad(out, lp, dout)]
+
+    def two():
+        out, _ = T.mamba2_mixer(u, **dict(zip(q, lq)), **kw, residual=u)
+        return [out, *torch.autograd.grad(out, lq, dout)]
+    want = one(), two()
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(DEV), torch.cuda.Stream(DEV)
+    got = [], []
+    for _ in range(8):
+        for s, f, keep in zip(streams, (one, two), got):
+            with torch.cuda.stream(s):
+                keep.append(f())
+    torch.cuda.synchronize()
+    for keep, ref in zip(got, want):
+        for run in keep:
+            assert all(torch.equal(a, b) for a, b in zip(run, ref))
