@@ -27,6 +27,7 @@ def _on_a_new_thread(f):
 
 
 def _calls():
+    import trading_bot_0_b200 as T
     from trading_bot_0_b200 import linear as LN, prepost as P, selective as S
     torch.manual_seed(0)
     x, W, dout, pre = rand(300, 64), rand(136, 64), rand(300, 136), rand(300, 136, dtype=F32)
@@ -41,6 +42,12 @@ def _calls():
     yield "scan backward", lambda: list(S.selective_scan_backward(u, u, u, A, bc, bc, dt_softplus=True).values())
     yield "convolution", lambda: P.conv1d_carry_forward(u, w)
     yield "convolution backward", lambda: P.conv1d_carry_backward(u, w, None, None, u)[:2]
+    s4 = dict(x=rand(2, 256, 8, 64), dt=rand(2, 256, 8).abs() * 0.1, A=-torch.ones(8, device=DEV), Bm=rand(2, 256, 1, 128), Cm=rand(2, 256, 1, 128))
+    yield "SSD scan", lambda: T.forward(**s4, chunk=128)[:2]
+    _, _, ws = T.forward(**s4, chunk=128, for_backward=True)
+    dy = rand(2, 256, 8, 64)
+    yield "SSD backward", lambda: [v for k, v in T.backward(dy, **s4, chunk=128).items() if k in ("dx", "dB", "dC", "ddt")]
+    yield "SSD backward from what the forward kept", lambda: [v for k, v in T.backward(dy, **s4, chunk=128, workspace=ws, fwd_saved=True).items() if k in ("dx", "dB", "dC", "ddt")]
 
 
 def test_first_work_of_a_thread(lib):
